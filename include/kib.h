@@ -259,6 +259,100 @@ int kib_attention_f32_f16_kv(kib_ctx* ctx, const float* query, const uint16_t* k
                              const uint16_t* value_cache, uint64_t layer, uint64_t position, uint64_t capacity_tokens,
                              uint64_t heads, uint64_t kv_heads, uint64_t head_dim, float* output);
 
+/* --------------------------------------------- paged 8-bit KV cache
+ * No counterpart in the reference (its cache is one F16 slab per sequence).
+ * A page holds page_tokens consecutive positions of one sequence, for every KV
+ * head.  Per page and KV head, keys and values are codes in [-127, 127] with
+ * one fp32 scale each: value = code * scale.  Half the bytes of the F16 cache,
+ * and sequences grow page by page.
+ *
+ * stream: a cudaStream_t on which the op is only enqueued (the caller orders
+ * it; (void*)1 is CUDA's legacy default stream), or NULL for the context's own
+ * stream, where the call waits outside a graph scope like every op above.  All
+ * pointers are device memory; 16-byte alignment is needed of codes and rows. */
+typedef struct kib_kvq8_cache {
+  int8_t *k, *v;            /* code of (page, head, token, d): page * page_stride + head * head_stride + token * token_stride + d */
+  float *k_scale, *v_scale; /* [pages][kv_heads] */
+  uint64_t pages, kv_heads;
+  uint64_t page_tokens;     /* 16, 32, 64 or 128 */
+  uint64_t head_dim;        /* 64, 128 or 256 */
+  uint64_t page_stride, head_stride, token_stride; /* multiples of 16; all 0: packed [pages][kv_heads][page_tokens][head_dim] */
+} kib_kvq8_cache;
+
+/* The sequences of one call and their rows (new tokens), packed one after
+ * another: sequence s has rows row_start[s] .. row_start[s + 1] - 1, the last
+ * of them at position lengths[s] - 1.  Block-table entries outside [0, pages)
+ * are absent pages: rows that fall on them are not stored, keys on them are
+ * not attended to. */
+typedef struct kib_kvq8_batch {
+  const int32_t* block_table; /* [sequences][table_stride]: page of positions i * page_tokens .. */
+  const int32_t* lengths;     /* [sequences] positions of each sequence, the new rows included */
+  const int32_t* row_start;   /* [sequences + 1] */
+  uint64_t sequences;         /* at most 65535 */
+  uint64_t table_stride;
+  uint64_t rows;              /* row_start[sequences], on the host */
+  uint64_t max_rows;          /* bound of any sequence's rows: rows past it may be left out */
+  uint64_t max_length;        /* bound of lengths (0: the table's span): keys past it are not attended to */
+  uint64_t total_length;      /* bound of the sum of lengths (0: sequences * max_length); sizes the workspace */
+} kib_kvq8_batch;
+
+/* Rotation of the leading 2 * pairs dimensions of a head, elements (i, i +
+ * pairs) by the angle position * inv_freq[i], the product in fp32: with
+ * inv_freq[i] = 1 / theta^(i / pairs) the rotation of kib_mrope_f32_in_place.
+ * sections: as s0..s3 there, choosing one of the four position streams per
+ * pair (all 0: stream 0). */
+typedef struct kib_rope {
+  const float* inv_freq;
+  uint64_t pairs;            /* 2 * pairs <= head_dim; 0: no rotation */
+  uint64_t sections[4];
+  const int32_t* positions;  /* [4][rows], or NULL: each row's position in the cache */
+} kib_rope;
+
+/* Rotates and quantises rows k, v [rows][kv_heads][head_dim] (type F32 or F16,
+ * row strides in elements, 0: packed) into the cache, and writes the rotated
+ * queries q [rows][heads][head_dim] to q_out (both NULL: none; q_out may be q).
+ * Rows before position 0 (more rows than positions) are skipped.  A page's scale is max(old, largest finite |x| of its new rows / 127); where
+ * it grows, the codes before the new rows are rounded again to it.  A page
+ * whose first position is new starts afresh.  Infinities saturate, NaN gives
+ * code 0.  rope may be NULL.  No two sequences may append to one page. */
+int kib_kvq8_append(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_batch* batch, const kib_rope* rope,
+                    int type, uint64_t heads, const void* q, uint64_t q_stride, const void* k, uint64_t k_stride,
+                    const void* v, uint64_t v_stride, void* q_out, uint64_t q_out_stride, void* stream);
+/* The values (F32 or F16) of whole pages: k_out, v_out [count][kv_heads]
+ * [page_tokens][head_dim]; zeros for ids outside [0, pages). */
+int kib_kvq8_read_pages(kib_ctx* ctx, const kib_kvq8_cache* cache, const int32_t* page_ids, uint64_t count, int type,
+                        void* k_out, void* v_out, void* stream);
+/* Causal attention of every row over its sequence's keys 0 .. its own
+ * position: out = softmax(scale * q . K) V per head, query head h on KV head
+ * h / (heads / kv_heads).  Rows without any key give zeros.  q and out
+ * [rows][heads][head_dim] of one type: F32 rows are computed to fp32 accuracy,
+ * F16 rows with the softmax weights rounded to half for the product with V
+ * (sums and statistics in fp32).  workspace: kib_kvq8_attention_workspace
+ * bytes, 256-byte aligned; calls that may overlap need one each. */
+int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_batch* batch, int type,
+                                 uint64_t heads, uint64_t* bytes);
+int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_batch* batch, int type,
+                       uint64_t heads, const void* q, uint64_t q_stride, float scale, void* out, uint64_t out_stride,
+                       void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------- sampling
+ * One token per row of logits [rows][vocab] (row_stride in elements, 0:
+ * packed; vocab <= 2^23).  With M the row's largest logit, e_i = exp((l_i - M)
+ * / temperature) and the weight w_i = trunc(e_i * 2^40), an integer: sums are
+ * exact, so the token depends on no order of addition.  Candidates are ordered
+ * by logit, equal ones by index.  top_k > 0 keeps the first k; top_p < 1 keeps
+ * those of them whose predecessors weigh less than top_p of their total; min_p
+ * keeps those with e_i >= min_p; the first always stays.  The token is the
+ * first in index order whose running weight exceeds uniform * total, uniform
+ * in [0, 1).  temperature <= 1e-6: the argmax (lowest index).  NaN logits count
+ * as -infinity; a row of nothing but -infinity gives token -1, probability 0.
+ * temperature, top_k, top_p, min_p: one value per row, or NULL for 1, 0, 1, 0.
+ * prob_out (may be NULL): the token's share of the kept weight.  stream as for
+ * the paged cache. */
+int kib_sample_f32(kib_ctx* ctx, const float* logits, uint64_t rows, uint64_t vocab, uint64_t row_stride,
+                   const float* uniform, const float* temperature, const int32_t* top_k, const float* top_p,
+                   const float* min_p, int32_t* token_out, float* prob_out, void* stream);
+
 /* ================================================================ runtime */
 
 typedef struct kib_qwen35 kib_qwen35;

@@ -28,6 +28,7 @@ KIB_ERR_INTERNAL = 3
 KIB_ERR_TIMEOUT = 4
 
 Q4_K, Q5_K, Q6_K = 12, 13, 14
+TYPE_F32, TYPE_F16 = 0, 1
 BLOCK_BYTES = {Q4_K: 144, Q5_K: 176, Q6_K: 210}
 
 
@@ -166,6 +167,21 @@ class SynthConfig(ctypes.Structure):
         ("qkv_type", c_uint32)]
 
 
+class _KvQ8CacheC(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p)] + [
+        (n, c_uint64) for n in ("pages", "kv_heads", "page_tokens", "head_dim", "page_stride", "head_stride",
+                                "token_stride")]
+
+
+class _KvQ8BatchC(ctypes.Structure):
+    _fields_ = [("block_table", c_void_p), ("lengths", c_void_p), ("row_start", c_void_p)] + [
+        (n, c_uint64) for n in ("sequences", "table_stride", "rows", "max_rows", "max_length", "total_length")]
+
+
+class _RopeC(ctypes.Structure):
+    _fields_ = [("inv_freq", c_void_p), ("pairs", c_uint64), ("sections", c_uint64 * 4), ("positions", c_void_p)]
+
+
 _U64 = c_uint64
 _P = c_void_p
 
@@ -221,6 +237,14 @@ def _declare(lib):
         "kib_rms_norm_f32_f32": (c_int, [_P, _P, _P, _U64, c_float, _P]),
         "kib_qk_norm_f32_f32": (c_int, [_P, _P, _P, _U64, _U64, c_float]),
         "kib_attention_f32_f16_kv": (c_int, [_P, _P, _P, _P, _U64, _U64, _U64, _U64, _U64, _U64, _P]),
+        "kib_kvq8_append": (c_int, [_P, POINTER(_KvQ8CacheC), POINTER(_KvQ8BatchC), POINTER(_RopeC), c_int, _U64, _P,
+                                    _U64, _P, _U64, _P, _U64, _P, _U64, _P]),
+        "kib_kvq8_read_pages": (c_int, [_P, POINTER(_KvQ8CacheC), _P, _U64, c_int, _P, _P, _P]),
+        "kib_kvq8_attention_workspace": (c_int, [_P, POINTER(_KvQ8CacheC), POINTER(_KvQ8BatchC), c_int, _U64,
+                                                 POINTER(c_uint64)]),
+        "kib_kvq8_attention": (c_int, [_P, POINTER(_KvQ8CacheC), POINTER(_KvQ8BatchC), c_int, _U64, _P, _U64, c_float,
+                                       _P, _U64, _P, _U64, _P]),
+        "kib_sample_f32": (c_int, [_P, _P, _U64, _U64, _U64, _P, _P, _P, _P, _P, _P, _P, _P]),
         "kib_qwen35_load": (c_int, [_P, c_char_p, POINTER(Qwen35Options), POINTER(c_void_p)]),
         "kib_qwen35_free": (None, [_P]),
         "kib_qwen35_get_plan": (c_int, [_P, POINTER(Qwen35Plan)]),
@@ -282,6 +306,85 @@ def ptr(x):
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
+def _stream(s):
+    """None: the context's stream (the call waits).  A cudaStream_t as an
+    integer: enqueue there; 0, torch's default stream, is CUDA's legacy default
+    stream, whose explicit handle is 1."""
+    return None if s is None else (int(s) or 1)
+
+
+def _row_type(x):
+    """(KIB_TYPE, row stride in elements) of a [rows][heads][head_dim] tensor
+    whose heads are packed within a row."""
+    code = {"float32": TYPE_F32, "float16": TYPE_F16}.get(str(x.dtype).split(".")[-1])
+    if code is None:
+        raise TypeError(f"rows must be float32 or float16, not {x.dtype}")
+    rows, heads, hd = x.shape
+    st = x.stride()
+    if st[2] != 1 or (heads > 1 and st[1] != hd):
+        raise ValueError("the heads of a row must be contiguous")
+    return code, (st[0] if rows > 1 else 0)
+
+
+def _vector(x, name, dtype, size):
+    if x is None:
+        return None
+    if str(x.dtype).split(".")[-1] != dtype or not x.is_contiguous() or x.numel() != size:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {size} values")
+    return x.data_ptr()
+
+
+class KvQ8Cache:
+    """A paged 8-bit KV cache over the caller's tensors (kib_kvq8_cache): codes
+    k, v int8 [pages][kv_heads][page_tokens][head_dim] with any strides whose
+    last is 1 (equal for k and v), scales float32 [pages][kv_heads]."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        for x in (k, v):
+            if str(x.dtype) != "torch.int8" or x.dim() != 4 or x.stride(3) != 1:
+                raise ValueError("codes must be int8 [pages][kv_heads][page_tokens][head_dim], the last stride 1")
+        if k.shape != v.shape or k.stride() != v.stride():
+            raise ValueError("k and v must have the same shape and strides")
+        pages, kv, page, hd = k.shape
+        self.shape = (pages, kv, page, hd)
+        self.tensors = (k, v, k_scale, v_scale)  # kept alive
+        self.c = _KvQ8CacheC(k.data_ptr(), v.data_ptr(), _vector(k_scale, "k_scale", "float32", pages * kv),
+                             _vector(v_scale, "v_scale", "float32", pages * kv), pages, kv, page, hd, *k.stride()[:3])
+
+
+class KvQ8Batch:
+    """The sequences of one call (kib_kvq8_batch): block_table int32
+    [sequences][pages of a sequence], lengths int32 [sequences] with the new
+    rows included, row_start int32 [sequences + 1]; rows, max_rows, max_length
+    and total_length are the host's bounds (see kib.h)."""
+
+    def __init__(self, block_table, lengths, row_start, rows, max_rows, max_length=0, total_length=0):
+        n = lengths.numel()
+        if block_table.dim() != 2 or block_table.shape[0] != n or str(block_table.dtype) != "torch.int32" or (
+                block_table.shape[1] > 1 and block_table.stride(1) != 1):
+            raise ValueError("block_table must be int32 [sequences][pages], rows contiguous")
+        self.tensors = (block_table, lengths, row_start)
+        if n > 1 and block_table.stride(0) != block_table.shape[1]:
+            raise ValueError("block_table must be contiguous")
+        self.rows = rows
+        self.c = _KvQ8BatchC(block_table.data_ptr(), _vector(lengths, "lengths", "int32", n),
+                             _vector(row_start, "row_start", "int32", n + 1), n, block_table.shape[1], rows, max_rows,
+                             max_length, total_length)
+
+
+class Rope:
+    """Rotation of heads by position (kib_rope): inv_freq float32 [pairs],
+    sections as in kib_mrope_f32_in_place, positions int32 [4][rows] or None
+    for the positions in the cache."""
+
+    def __init__(self, inv_freq, sections=(0, 0, 0, 0), positions=None):
+        pairs = inv_freq.numel()
+        self.tensors = (inv_freq, positions)
+        self.positions = positions
+        self.c = _RopeC(_vector(inv_freq, "inv_freq", "float32", pairs), pairs, (c_uint64 * 4)(*sections),
+                        None if positions is None else _vector(positions, "positions", "int32", positions.numel()))
+
+
 class Context:
     """A device context: one CUDA stream, like MpsContext's one command queue."""
 
@@ -293,11 +396,14 @@ class Context:
             raise KibError(rc, "kib_create failed (no sm_100 device?)")
         self.h = h
         self.children = weakref.WeakSet()  # models on this context: freed before it
+        self._workspace = (None, 0)  # attention's, grown on demand
 
     def close(self):
         if getattr(self, "h", None):
             for c in list(self.children):
                 c.close()
+            if self._workspace[0]:
+                self.lib.kib_free_buffer(self.h, self._workspace[0])
             self.lib.kib_destroy(self.h)
             self.h = None
 
@@ -337,6 +443,86 @@ class Context:
     def dequantize_rows(self, qtype, weight, rows, ids, count, cols, out):
         self.check(self.lib.kib_dequantize_rows_kquant_f32(self.h, qtype, ptr(weight), rows, ptr(ids), count, cols,
                                                            ptr(out)))
+
+
+    # paged 8-bit KV cache.  stream: see _stream
+    def kvq8_append(self, cache: KvQ8Cache, batch: KvQ8Batch, k, v, q=None, q_out=None, rope=None, stream=None):
+        """k, v [rows][kv_heads][head_dim] rotated, quantised and stored; q
+        [rows][heads][head_dim] rotated into q_out (which may be q)."""
+        kind, ks = _row_type(k)
+        vkind, vs = _row_type(v)
+        qs = os_ = heads = 0
+        want = (batch.rows, cache.shape[1], cache.shape[3])
+        if tuple(k.shape) != want or tuple(v.shape) != want or vkind != kind:
+            raise ValueError(f"k and v must be {want} of one type")
+        if (q is None) != (q_out is None):
+            raise ValueError("q and q_out go together")
+        if q is not None:
+            (qkind, qs), (okind, os_) = _row_type(q), _row_type(q_out)
+            heads = q.shape[1]
+            if qkind != kind or okind != kind or q.shape != q_out.shape or q.shape[0] != batch.rows or (
+                    q.shape[2] != cache.shape[3]):
+                raise ValueError("q and q_out must be [rows][heads][head_dim] of the type of k")
+        if rope is not None and rope.positions is not None and rope.positions.numel() != 4 * batch.rows:
+            raise ValueError("positions must be [4][rows]")
+        self.check(self.lib.kib_kvq8_append(self.h, byref(cache.c), byref(batch.c), byref(rope.c) if rope else None,
+                                            kind, heads, ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(q_out), os_,
+                                            _stream(stream)))
+
+    def kvq8_read_pages(self, cache: KvQ8Cache, page_ids, k_out, v_out, stream=None):
+        """The values of whole pages, [count][kv_heads][page_tokens][head_dim]."""
+        want = (page_ids.numel(),) + tuple(cache.shape[1:])
+        kind = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16}.get(str(k_out.dtype), -1)
+        for x in (k_out, v_out):
+            if tuple(x.shape) != want or not x.is_contiguous() or x.dtype != k_out.dtype:
+                raise ValueError(f"outputs must be contiguous {want} of one type")
+        self.check(self.lib.kib_kvq8_read_pages(self.h, byref(cache.c), _vector(page_ids, "page_ids", "int32", want[0]),
+                                                want[0], kind, ptr(k_out), ptr(v_out), _stream(stream)))
+
+    def kvq8_attention_workspace(self, cache: KvQ8Cache, batch: KvQ8Batch, q) -> int:
+        """Bytes of workspace that kvq8_attention needs for these arguments."""
+        need = c_uint64()
+        self.check(self.lib.kib_kvq8_attention_workspace(self.h, byref(cache.c), byref(batch.c), _row_type(q)[0],
+                                                         q.shape[1], byref(need)))
+        return need.value
+
+    def kvq8_attention(self, cache: KvQ8Cache, batch: KvQ8Batch, q, out, scale, workspace=None, stream=None):
+        """Causal attention of q [rows][heads][head_dim] over the cache.
+        workspace: a device tensor of kvq8_attention_workspace bytes; None: one
+        that this context keeps and grows (then calls must not overlap)."""
+        kind, qs = _row_type(q)
+        okind, os_ = _row_type(out)
+        if okind != kind or q.shape != out.shape or q.shape[0] != batch.rows or q.shape[2] != cache.shape[3]:
+            raise ValueError("q and out must be [rows][heads][head_dim] of one type")
+        if workspace is None:
+            need = self.kvq8_attention_workspace(cache, batch, q)
+            if need > self._workspace[1]:
+                old, self._workspace = self._workspace[0], (None, 0)
+                if old:
+                    self.check(self.lib.kib_free_buffer(self.h, old))
+                h = c_void_p()
+                self.check(self.lib.kib_make_buffer(self.h, need, byref(h)))
+                self._workspace = (h.value, need)
+            where, size = self._workspace
+        else:
+            where, size = ptr(workspace), workspace.numel() * workspace.element_size()
+        self.check(self.lib.kib_kvq8_attention(self.h, byref(cache.c), byref(batch.c), kind, q.shape[1], ptr(q), qs,
+                                               scale, ptr(out), os_, where, size, _stream(stream)))
+
+    def sample(self, logits, uniform, token_out, prob_out=None, temperature=None, top_k=None, top_p=None, min_p=None,
+               stream=None):
+        """A token per row of logits [rows][vocab] (float32, last stride 1);
+        the per-row tensors as in kib_sample_f32, None for the default."""
+        rows, vocab = logits.shape
+        if str(logits.dtype) != "torch.float32" or (vocab > 1 and logits.stride(1) != 1):
+            raise ValueError("logits must be float32 [rows][vocab], the last stride 1")
+        self.check(self.lib.kib_sample_f32(self.h, ptr(logits), rows, vocab, logits.stride(0) if rows > 1 else 0,
+                                           _vector(uniform, "uniform", "float32", rows),
+                                           _vector(temperature, "temperature", "float32", rows),
+                                           _vector(top_k, "top_k", "int32", rows), _vector(top_p, "top_p", "float32", rows),
+                                           _vector(min_p, "min_p", "float32", rows),
+                                           _vector(token_out, "token_out", "int32", rows),
+                                           _vector(prob_out, "prob_out", "float32", rows), _stream(stream)))
 
 
 class Qwen35:

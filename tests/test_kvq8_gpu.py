@@ -1,0 +1,510 @@
+"""The paged 8-bit KV cache (kib_kvq8_*) against plain forms in 64 bits: append
+with rotation, reading pages, ragged causal attention, and their refusals.
+
+Tolerances.  Codes: the quotient x / scale is known to 2e-4 (127 times the
+rounding of the rotated value, 12 half-ulps of fp32, of its scale and of the
+reciprocal), so a code equals the 64-bit one unless that quotient lies within
+2e-4 of a half-integer, and is off by at most one there; a code that is rounded
+again to a grown scale has twice that.  Attention: a score carries at most 2^-20 of
+sum |q_i k_i| * scale (16 half-ulps of fp32 over the absolute sum), a softmax
+weight twice that relatively, the sums 2^-19; half rows add 2^-11 for the
+weights and 2^-11 for the result.  All relative to the largest |v| attended."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kib
+
+gpu = pytest.mark.gpu
+DT = {"f32": torch.float32, "f16": torch.float16}
+
+
+class Case:
+    """Sequences with lengths (new rows included) and new rows, their cache on
+    the GPU, and copies of everything in numpy for the oracle."""
+
+    def __init__(self, lengths, new, heads=4, kv=2, hd=64, page=16, dtype="f32", seed=0, layout="packed", spread=1.0):
+        r = np.random.default_rng(seed)
+        self.lengths, self.new, self.heads, self.kv, self.hd, self.page = lengths, new, heads, kv, hd, page
+        n = len(lengths)
+        need = [max(0, -(-x // page)) for x in lengths]
+        self.pages = sum(need) + 2
+        self.width = max(need + [1]) + 1
+        order = r.permutation(self.pages)
+        self.table = np.full((n, self.width), -1, np.int32)
+        at = 0
+        for i in range(n):
+            self.table[i, :need[i]] = order[at:at + need[i]]
+            at += need[i]
+        self.codes = [r.integers(-127, 128, (self.pages, kv, page, hd)).astype(np.int8) for _ in range(2)]
+        self.scales = [(0.01 + 0.02 * r.random((self.pages, kv))).astype(np.float32) for _ in range(2)]
+        self.start = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        rows = int(self.start[-1])
+        rnd = lambda h: torch.from_numpy((r.standard_normal((rows, h, hd)) * spread).astype(np.float32)).to(DT[dtype])  # noqa: E731
+        self.q, self.k, self.v = rnd(heads), rnd(kv), rnd(kv)
+        self.dtype, self.rows = dtype, rows
+        dev = []
+        for c in self.codes:
+            if layout == "packed":
+                dev.append(torch.from_numpy(c).cuda())
+            elif layout == "token_major":  # [page][token][head][d] in memory
+                dev.append(torch.from_numpy(c).permute(0, 2, 1, 3).contiguous().cuda().permute(0, 2, 1, 3))
+            else:  # padded rows, and other layers' pages in between
+                big = torch.zeros(self.pages, 3, kv, page, hd + 16, dtype=torch.int8, device="cuda")
+                view = big[:, 1, :, :, :hd]
+                view.copy_(torch.from_numpy(c))
+                dev.append(view)
+        self.dev = dev + [torch.from_numpy(s.copy()).cuda() for s in self.scales]
+        self.cache = kib.KvQ8Cache(*self.dev)
+        cuda = lambda a: torch.from_numpy(np.asarray(a, np.int32)).cuda()  # noqa: E731
+        self.lengths_dev = cuda(lengths)
+        self.batch = kib.KvQ8Batch(cuda(self.table), self.lengths_dev, cuda(self.start), rows, max(list(new) + [0]))
+
+    def positions(self, i):
+        """Cache positions of sequence i's new rows."""
+        return np.arange(self.lengths[i] - self.new[i], self.lengths[i])
+
+
+def rotate64(x, angle):
+    x, half = x.astype(np.float64).copy(), angle.shape[-1]
+    c, s = np.cos(angle)[:, None, :], np.sin(angle)[:, None, :]
+    a, b = x[..., :half].copy(), x[..., half:2 * half].copy()
+    x[..., :half], x[..., half:2 * half] = a * c - b * s, b * c + a * s
+    return x
+
+
+def oracle_append(c, x, codes, scales):
+    """Quotients (before rounding) and scales after the rows x (64-bit) are
+    stored; quotients of everything not touched are its codes."""
+    quo, scales = codes.astype(np.float64), scales.astype(np.float64)
+    fresh = np.zeros(codes.shape, bool)
+    for i in range(len(c.lengths)):
+        p, stop, row = max(0, c.lengths[i] - c.new[i]), c.lengths[i], c.start[i] + max(0, c.new[i] - c.lengths[i])
+        while p < stop:
+            end = min(stop, (p // c.page + 1) * c.page)
+            page, lo = c.table[i, p // c.page], p % c.page
+            part = x[row:row + end - p]  # [rows][kv][hd]
+            row, n, p = row + end - p, end - p, end
+            if page < 0:
+                continue
+            big = np.where(np.isfinite(part), np.abs(part), 0).max((0, 2))
+            old = scales[page] if lo else np.zeros_like(big)
+            now = np.maximum(old, big / 127)
+            with np.errstate(all="ignore"):
+                ratio = np.where(now > 0, old / now, 0)
+                inv = np.where(now > 0, 1 / now, 0)
+                quo[page, :, :lo] *= ratio[:, None, None]
+                y = part * inv[None, :, None]
+            quo[page, :, lo:lo + n] = np.where(np.isnan(part), 0, np.clip(np.nan_to_num(y, nan=0), -127, 127)).transpose(1, 0, 2)
+            fresh[page, :, lo:lo + n] = True
+            scales[page] = now
+    return quo, scales, fresh
+
+
+def check_codes(got, quo, fresh):
+    want = np.rint(quo)
+    edge = np.abs(np.abs(quo - np.floor(quo)) - 0.5)
+    diff = np.abs(got.astype(np.int64) - want)
+    assert diff.max() <= 1
+    assert not (diff[fresh] > 0)[edge[fresh] > 2e-4].any()
+    assert not (diff[~fresh] > 0)[edge[~fresh] > 4e-4].any()
+
+
+def inv_freq(pairs, theta=1e4):
+    return (1.0 / theta ** (np.arange(pairs) / pairs)).astype(np.float32)
+
+
+def run_append(ctx, c, pairs=8, sections=(0, 0, 0, 0), positions=None, in_place=False, stream=None):
+    q, k, v = c.q.cuda(), c.k.cuda(), c.v.cuda()
+    q_out = q if in_place else torch.empty_like(q)
+    rope = None
+    if pairs:
+        rope = kib.Rope(torch.from_numpy(inv_freq(pairs)).cuda(), sections,
+                        None if positions is None else torch.from_numpy(positions).cuda())
+    torch.cuda.synchronize()
+    ctx.kvq8_append(c.cache, c.batch, k, v, q=q, q_out=q_out, rope=rope, stream=stream)
+    torch.cuda.synchronize()
+    return q_out.cpu().float().numpy()
+
+
+def check_append(ctx, c, pairs=8, sections=(0, 0, 0, 0), positions=None, **kw):
+    got_q = run_append(ctx, c, pairs, sections, positions, **kw)
+    pos = np.concatenate([c.positions(i) for i in range(len(c.lengths))])
+    if positions is None:
+        per = np.repeat(pos[:, None], max(pairs, 1), 1)
+    else:
+        tot = sum(sections)
+        stream = [0 if not tot else (0 if j % tot < sections[0] else 1 if j % tot < sum(sections[:2]) else
+                                     2 if j % tot < sum(sections[:3]) else 3) for j in range(pairs)]
+        per = np.stack([positions[s] for s in stream], 1)
+    angle = (per[:, :pairs].astype(np.float32) * inv_freq(pairs)[None] if pairs else np.zeros((c.rows, 0))).astype(np.float64)
+    kept = pos >= 0
+    q, k = rotate64(c.q.float().numpy(), angle), rotate64(c.k.float().numpy(), angle)
+    tol = 1e-6 * np.abs(q).max(-1, keepdims=True) + (2.0 ** -11 * np.abs(q) + 2.0 ** -25 if c.dtype == "f16" else 0)
+    assert (np.abs(got_q - q) <= tol)[kept].all()
+    for x, at in ((k, 0), (c.v.float().numpy().astype(np.float64), 1)):
+        quo, scales, fresh = oracle_append(c, x, c.codes[at], c.scales[at])
+        assert np.allclose(c.dev[2 + at].cpu().numpy(), scales, rtol=2e-6, atol=0)
+        check_codes(c.dev[at].cpu().numpy(), quo, fresh)
+    # read back: code * scale
+    ids = torch.arange(-1, c.pages + 1, dtype=torch.int32, device="cuda")
+    shape = (c.pages + 2, c.kv, c.page, c.hd)
+    out = [torch.full(shape, 7.0, dtype=DT[c.dtype], device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    ctx.kvq8_read_pages(c.cache, ids, out[0], out[1])
+    for x, codes, scales in zip(out, c.dev[:2], c.dev[2:]):
+        assert (x[0] == 0).all() and (x[-1] == 0).all()
+        assert torch.equal(x[1:-1], (codes.float() * scales[:, :, None, None]).to(DT[c.dtype]))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd,page,layout", [(64, 16, "packed"), (128, 32, "token_major"), (256, 64, "padded"),
+                                            (256, 128, "packed"), (128, 16, "padded")])
+def test_append(ctx, dtype, hd, page, layout):
+    # runs inside a page, ending at its edge, over many pages, one row, none, from the first position
+    c = Case([5, page, 3 * page + 7, 2 * page, 1, 40], [5, 1, 2 * page + 9, 0, 1, 3], heads=6, kv=2, hd=hd, page=page,
+             dtype=dtype, seed=hd + page, layout=layout)
+    check_append(ctx, c, pairs=hd // 8)
+
+
+@gpu
+def test_append_rotation_positions_and_in_place(ctx):
+    c = Case([33, 20], [30, 20], hd=64, seed=5)
+    r = np.random.default_rng(1)
+    check_append(ctx, c, pairs=32, sections=(11, 11, 10, 0), positions=r.integers(0, 200000, (4, 50)).astype(np.int32),
+                 in_place=True)
+    check_append(ctx, Case([33, 20], [30, 20], hd=64, seed=6), pairs=0)
+    check_append(ctx, Case([9], [9], hd=64, seed=7, dtype="f16"), pairs=5, in_place=True)
+
+
+@gpu
+def test_append_positions_before_the_first_are_dropped(ctx):
+    # more new rows than positions: the first rows have no place
+    check_append(ctx, Case([10, 3], [14, 3], seed=8))
+
+
+@gpu
+def test_append_one_by_one_grows_the_scale(ctx):
+    """Rows of growing size: each one enlarges the scale, the codes before it
+    are rounded again; the page stays within the sum of the roundings."""
+    c = Case([1], [1], kv=1, heads=1, hd=64, seed=3)
+    r = np.random.default_rng(0)
+    rows = r.standard_normal((16, 64)) * (1.0 + np.arange(16)[:, None])
+    rows = rows.astype(np.float32)
+    for i in range(16):
+        c.lengths_dev.fill_(i + 1)
+        x = torch.from_numpy(rows[i]).cuda().reshape(1, 1, 64)
+        torch.cuda.synchronize()
+        ctx.kvq8_append(c.cache, c.batch, x, x)
+    page = c.table[0, 0]
+    s = float(c.dev[2][page, 0])
+    assert s == pytest.approx(np.abs(rows).max() / 127, rel=1e-6)
+    got = c.dev[0][page, 0].cpu().numpy() * s
+    # each of at most 16 roundings costs half a unit of a scale no larger than the last
+    assert np.abs(got - rows).max() <= 16 * 0.5 * s
+    assert np.abs(got[15] - rows[15]).max() <= 0.5 * s * (1 + 1e-5)
+
+
+@gpu
+def test_append_values_that_are_not_finite(ctx):
+    c = Case([20], [20], kv=1, heads=1, seed=4)
+    c.k[3, 0, 20], c.k[4, 0, 21], c.k[5, 0, 22] = math.inf, -math.inf, math.nan
+    c.v[:] = 0
+    run_append(ctx, c, pairs=0)
+    quo, scales, fresh = oracle_append(c, c.k.numpy().astype(np.float64), c.codes[0], c.scales[0])
+    check_codes(c.dev[0].cpu().numpy(), quo, fresh)
+    page = c.table[0, 0]
+    assert [int(c.dev[0][page, 0, t, d]) for t, d in ((3, 20), (4, 21), (5, 22))] == [127, -127, 0]
+    assert np.allclose(c.dev[2].cpu().numpy(), scales, rtol=2e-6)
+    # all zeros: scale 0, codes 0
+    assert float(c.dev[3][page, 0]) == 0.0 and not c.dev[1][page, 0].any()
+
+
+@gpu
+def test_append_skips_absent_pages_and_strided_rows(ctx):
+    c = Case([40], [40], kv=2, heads=4, seed=9)
+    c.table[0, 1] = -1
+    c.batch.tensors[0].copy_(torch.from_numpy(c.table))
+    before = [x.clone() for x in c.dev]
+    joined = torch.cat([c.q, c.k, c.v], 1).cuda()  # one row holds q | k | v
+    q, k, v = joined[:, :4], joined[:, 4:6], joined[:, 6:]
+    torch.cuda.synchronize()
+    ctx.kvq8_append(c.cache, c.batch, k, v, q=q, q_out=q)
+    for x, at in ((c.k, 0), (c.v, 1)):
+        quo, scales, fresh = oracle_append(c, x.numpy().astype(np.float64), c.codes[at], c.scales[at])
+        check_codes(c.dev[at].cpu().numpy(), quo, fresh)
+        lost = [p for p in range(c.pages) if p not in c.table[0]]
+        assert torch.equal(c.dev[at][lost], before[at][lost]) and torch.equal(c.dev[2 + at][lost], before[2 + at][lost])
+
+
+def oracle_attend(c, scale):
+    """Outputs and the largest error allowed, per row and head."""
+    q = c.q.float().numpy().astype(np.float64)
+    out, tol = np.zeros_like(q), np.zeros(q.shape[:2])
+    codes = [x.cpu().numpy().astype(np.float64) for x in c.dev[:2]]
+    scales = [x.cpu().numpy().astype(np.float64) for x in c.dev[2:]]
+    for i in range(len(c.lengths)):
+        L, n = max(0, c.lengths[i]), c.new[i]
+        pos = np.arange(L)
+        page = c.table[i][pos // c.page] if L else np.zeros(0, np.int64)
+        here = (page >= 0) & (page < c.pages)
+        pos, page = pos[here], page[here]
+        key, val = ((x[page, :, pos % c.page] * s[page][..., None]) for x, s in zip(codes, scales))  # [L][kv][hd]
+        for t in range(n):
+            row, end = c.start[i] + t, np.searchsorted(pos, c.lengths[i] - n + t, side="right")
+            if end == 0:
+                continue
+            for h in range(c.heads):
+                g = h // (c.heads // c.kv)
+                sc = key[:end, g] @ q[row, h] * scale
+                big = np.abs(key[:end, g]) @ np.abs(q[row, h]) * abs(scale)
+                p = np.exp(sc - sc.max())
+                p /= p.sum()
+                out[row, h] = p @ val[:end, g]
+                tol[row, h] = (2 * 2.0 ** -20 * big.max() + 2.0 ** -19 + (2.0 ** -10 if c.dtype == "f16" else 0)) * np.abs(
+                    val[:end, g]).max()
+    return out, tol
+
+
+def run_attend(ctx, c, scale, stream=None, workspace=None):
+    q = c.q.cuda()
+    out = torch.full_like(q, 77.0)
+    torch.cuda.synchronize()
+    ctx.kvq8_attention(c.cache, c.batch, q, out, scale, stream=stream, workspace=workspace)
+    torch.cuda.synchronize()
+    return out
+
+
+def check_attend(ctx, c, scale=None):
+    scale = scale if scale is not None else 1.0 / math.sqrt(c.hd)
+    got = run_attend(ctx, c, scale).cpu().float().numpy()
+    want, tol = oracle_attend(c, scale)
+    err = np.abs(got - want).max(-1)
+    assert (err <= tol).all(), float((err - tol).max())
+    return got
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("heads,kv,hd,page,layout", [(8, 2, 256, 64, "packed"), (4, 4, 64, 16, "token_major"),
+                                                     (6, 2, 128, 32, "padded"), (16, 1, 256, 128, "packed"),
+                                                     (5, 1, 64, 16, "padded"), (8, 8, 128, 16, "packed")])
+def test_attention_single_rows(ctx, dtype, heads, kv, hd, page, layout):
+    lengths = [1, 17, 0, page, 3 * page + 1, 700, 63]
+    check_attend(ctx, Case(lengths, [1] * 7, heads, kv, hd, page, dtype, seed=heads + hd, layout=layout, spread=1.5))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd,page", [(256, 64), (128, 16), (64, 128)])
+def test_attention_few_rows(ctx, dtype, hd, page):
+    # verify runs of several rows, sequences without rows, more rows than positions
+    check_attend(ctx, Case([5, 100, 300, 2, 64, 33], [5, 3, 0, 4, 8, 2], 8, 2, hd, page, dtype, seed=hd))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("heads,kv,hd,page", [(8, 2, 256, 64), (4, 4, 128, 16), (6, 1, 64, 32), (8, 2, 256, 16),
+                                              (16, 2, 128, 128)])
+def test_attention_many_rows(ctx, dtype, heads, kv, hd, page):
+    # prompts from their first position, chunks late in a sequence, ragged with single rows
+    check_attend(ctx, Case([77, 300, 1, 513, 130], [77, 44, 1, 150, 129], heads, kv, hd, page, dtype, seed=hd + page))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 90])
+def test_attention_absent_pages_and_masked_junk(ctx, rows):
+    """Absent pages are left out; codes past the length and the scales of
+    pages that are not reached (NaN, infinity) change nothing."""
+    c = Case([200, 150], [rows, rows], seed=11, hd=128)
+    c.table[0, 2] = c.pages + 5
+    c.table[1, 0] = -7
+    c.batch.tensors[0].copy_(torch.from_numpy(c.table))
+    used = set(c.table[0]) | set(c.table[1])
+    for p in range(c.pages):
+        if p not in used:
+            c.dev[2][p], c.dev[3][p] = math.nan, math.inf
+    a = check_attend(ctx, c)
+    last = c.table[0, 199 // c.page]
+    for x in c.dev[:2]:
+        x[last, :, 199 % c.page + 1:] = -128
+    assert np.array_equal(check_attend(ctx, c), a)
+
+
+@gpu
+def test_attention_rows_whose_every_key_is_absent_are_zero(ctx):
+    c = Case([40, 40], [1, 40], seed=12)
+    c.table[:] = -1
+    c.batch.tensors[0].copy_(torch.from_numpy(c.table))
+    assert not run_attend(ctx, c, 0.125).any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attention_scales_far_apart(ctx, dtype, rows):
+    """Pages whose scales differ by factors of 1e5, zero scales, and scores so
+    sharp that one key takes all the weight."""
+    c = Case([400, 129], [rows, rows], hd=128, seed=13, dtype=dtype)
+    r = np.random.default_rng(3)
+    c.dev[3].copy_(torch.from_numpy((10.0 ** r.uniform(-6, -1, c.scales[1].shape)).astype(np.float32)))
+    c.dev[3][c.table[0, 3]] = 0.0
+    c.dev[2][c.table[0, 1]] = 0.0
+    check_attend(ctx, c)
+    check_attend(ctx, c, scale=2.0)
+    check_attend(ctx, c, scale=-0.1)
+    check_attend(ctx, c, scale=0.0)
+
+
+@gpu
+def test_attention_is_the_same_every_time_and_on_another_stream(ctx):
+    c = Case([3000, 1, 777, 2048], [1, 1, 6, 1], 8, 2, 256, 64, seed=14)
+    a = run_attend(ctx, c, 0.06)
+    for _ in range(3):
+        assert torch.equal(run_attend(ctx, c, 0.06), a)
+    side = torch.cuda.Stream()
+    q = c.q.cuda()
+    need = ctx.kvq8_attention_workspace(c.cache, c.batch, q)
+    ws = torch.empty(max(need, 256), dtype=torch.uint8, device="cuda")
+    assert torch.equal(run_attend(ctx, c, 0.06, stream=side.cuda_stream, workspace=ws), a)
+    assert torch.equal(run_attend(ctx, c, 0.06, stream=0), a)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 100])
+def test_append_and_attention_in_a_captured_graph(ctx, rows):
+    """Enqueued on a capturing stream and replayed on new inputs."""
+    c = Case([300, 140], [rows, rows], 8, 2, 128, 32, seed=15)
+    q, k, v = c.q.cuda(), c.k.cuda(), c.v.cuda()
+    out = torch.empty_like(q)
+    ws = torch.empty(max(ctx.kvq8_attention_workspace(c.cache, c.batch, q), 256), dtype=torch.uint8, device="cuda")
+
+    def step(stream):
+        ctx.kvq8_append(c.cache, c.batch, k, v, stream=stream)
+        ctx.kvq8_attention(c.cache, c.batch, q, out, 0.09, workspace=ws, stream=stream)
+
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    step(side.cuda_stream)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        step(torch.cuda.current_stream().cuda_stream)
+    q.mul_(0.5)
+    k.mul_(1.5)
+    g.replay()
+    torch.cuda.synchronize()
+    replayed = out.clone()
+    out.zero_()
+    torch.cuda.synchronize()
+    step(None)
+    assert torch.equal(out, replayed)
+
+
+@gpu
+def test_refusals(ctx):
+    c = Case([33, 20], [1, 2], 8, 2, 64, 16, seed=1)
+    q, k, v = c.q.cuda(), c.k.cuda(), c.v.cuda()
+    out = torch.empty_like(q)
+    lib = ctx.lib
+
+    def refused(rc, word):
+        assert rc == kib.KIB_ERR_INVALID_ARGUMENT
+        assert word in lib.kib_last_error(ctx.h).decode()
+
+    def attend(cache=c.cache, batch=c.batch, kind=0, heads=8, qp=q.data_ptr(), qs=0, scale=0.1, op=out.data_ptr(), os_=0,
+               ws=None, size=0):
+        need = ctx.kvq8_attention_workspace(c.cache, c.batch, q)
+        if ws is None:
+            attend.ws = torch.empty(need + 256, dtype=torch.uint8, device="cuda")
+            ws, size = attend.ws.data_ptr(), need
+        return lib.kib_kvq8_attention(ctx.h, cache.c, batch.c, kind, heads, qp, qs, scale, op, os_, ws, size, None)
+
+    def with_cache(**kw):
+        x = kib.KvQ8Cache(*c.dev)
+        for n, val in kw.items():
+            setattr(x.c, n, val)
+        return x
+
+    def with_batch(**kw):
+        x = kib.KvQ8Batch(*c.batch.tensors, c.rows, 2)
+        for n, val in kw.items():
+            setattr(x.c, n, val)
+        return x
+
+    assert attend() == kib.KIB_OK
+    refused(attend(cache=with_cache(head_dim=96)), "head_dim")
+    refused(attend(cache=with_cache(page_tokens=48)), "page_tokens")
+    refused(attend(cache=with_cache(kv_heads=0)), "kv_heads")
+    refused(attend(cache=with_cache(pages=0)), "pages")
+    refused(attend(cache=with_cache(k=None)), "null")
+    refused(attend(cache=with_cache(token_stride=72)), "16")
+    refused(attend(cache=with_cache(token_stride=32)), "smaller")
+    refused(attend(cache=with_cache(v=c.dev[1].data_ptr() + 1)), "16")
+    refused(attend(batch=with_batch(lengths=None)), "null")
+    refused(attend(batch=with_batch(block_table=None)), "block table")
+    refused(attend(batch=with_batch(max_rows=0)), "max_rows")
+    refused(attend(batch=with_batch(max_rows=4)), "max_rows")
+    refused(attend(batch=with_batch(sequences=1 << 20)), "sequences")
+    refused(attend(batch=with_batch(table_stride=1 << 29)), "2^31")
+    refused(attend(kind=12), "type")
+    refused(attend(heads=7), "heads")
+    refused(attend(heads=0), "heads")
+    refused(attend(qp=None), "null")
+    refused(attend(qp=q.data_ptr() + 4), "16")
+    refused(attend(qs=100), "smaller")
+    refused(attend(os_=514), "16")
+    refused(attend(scale=math.nan), "finite")
+    need = ctx.kvq8_attention_workspace(c.cache, c.batch, q)
+    if need:
+        refused(attend(ws=attend.ws.data_ptr(), size=need - 1), "workspace")
+        refused(attend(ws=attend.ws.data_ptr() + 16, size=need), "workspace")
+
+    def append(cache=c.cache, rope=None, kind=0, heads=8, qp=q.data_ptr(), kp=k.data_ptr(), op=out.data_ptr(), ks=0, os_=0):
+        return lib.kib_kvq8_append(ctx.h, cache.c, c.batch.c, rope.c if rope else None, kind, heads, qp, 0, kp, ks,
+                                   v.data_ptr(), 0, op, os_, None)
+
+    freq = torch.ones(40, device="cuda")
+    refused(append(kind=14), "type")
+    refused(append(kp=None), "null")
+    refused(append(op=None), "together")
+    refused(append(heads=0), "heads")
+    refused(append(ks=64), "smaller")
+    refused(append(op=q.data_ptr(), os_=1024), "in-place")
+    refused(append(rope=kib.Rope(freq)), "pairs")
+    refused(append(rope=kib.Rope(freq[:8], sections=(1000, 0, 0, 0))), "sections")
+    ids = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x = torch.empty(1, 2, 16, 64, device="cuda")
+    refused(lib.kib_kvq8_read_pages(ctx.h, c.cache.c, ids.data_ptr(), 1, 7, x.data_ptr(), x.data_ptr(), None), "type")
+    refused(lib.kib_kvq8_read_pages(ctx.h, c.cache.c, None, 1, 0, x.data_ptr(), x.data_ptr(), None), "null")
+    refused(lib.kib_kvq8_read_pages(ctx.h, c.cache.c, ids.data_ptr(), 1, 0, x.data_ptr() + 4, x.data_ptr(), None), "16")
+    # nothing to do is not an error
+    empty = kib.KvQ8Batch(torch.zeros(0, 1, dtype=torch.int32, device="cuda"), ids[:0], ids, 0, 0)
+    ctx.kvq8_append(c.cache, empty, k[:0], v[:0])
+    ctx.kvq8_attention(c.cache, empty, q[:0], out[:0], 0.1)
+    ctx.kvq8_read_pages(c.cache, ids[:0], x[:0], x[:0])
+
+
+def test_wrapper_checks_shapes_and_types():
+    z = lambda *s, t=torch.int8: torch.zeros(*s, dtype=t)  # noqa: E731
+    s = z(4, 2, t=torch.float32)
+    kib.KvQ8Cache(z(4, 2, 16, 64), z(4, 2, 16, 64), s, s)
+    for bad in ((z(4, 2, 16, 64), z(4, 2, 16, 128), s, s), (z(4, 2, 16, 64, t=torch.uint8), z(4, 2, 16, 64), s, s),
+                (z(4, 2, 64, 16).transpose(2, 3), z(4, 2, 64, 16).transpose(2, 3), s, s),
+                (z(4, 2, 16, 64), z(4, 2, 16, 64), s[:3], s), (z(4, 2, 16, 64), z(4, 2, 16, 64), s, s.double())):
+        with pytest.raises(ValueError):
+            kib.KvQ8Cache(*bad)
+    i = lambda *n: torch.zeros(*n, dtype=torch.int32)  # noqa: E731
+    kib.KvQ8Batch(i(3, 5), i(3), i(4), 7, 3)
+    for bad in ((i(2, 5), i(3), i(4)), (i(3, 5).float(), i(3), i(4)), (i(3, 5), i(3), i(3)), (i(3, 10)[:, ::2], i(3), i(4)),
+                (i(3, 10)[:, :5], i(3), i(4))):
+        with pytest.raises(ValueError):
+            kib.KvQ8Batch(*bad, 7, 3)
+    with pytest.raises(TypeError):
+        kib._row_type(torch.zeros(2, 3, 64, dtype=torch.float64))
+    with pytest.raises(ValueError):
+        kib._row_type(torch.zeros(2, 3, 128)[:, :, ::2])
+    assert kib._row_type(torch.zeros(5, 10, 64)[:, 2:6]) == (kib.TYPE_F32, 640)
