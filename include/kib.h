@@ -288,7 +288,7 @@ typedef struct kib_kvq8_batch {
   const int32_t* block_table; /* [sequences][table_stride]: page of positions i * page_tokens .. */
   const int32_t* lengths;     /* [sequences] positions of each sequence, the new rows included */
   const int32_t* row_start;   /* [sequences + 1] */
-  uint64_t sequences;         /* at most 65535 */
+  uint64_t sequences;         /* at most 4096 */
   uint64_t table_stride;
   uint64_t rows;              /* row_start[sequences], on the host */
   uint64_t max_rows;          /* bound of any sequence's rows: rows past it may be left out */

@@ -3,10 +3,11 @@
 // entry; nothing is launched for arguments outside the documented ranges.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <string>
 
 #include "kib_ctx.cuh"
-#include "kvq8.cuh"
+#include "kvq8_few.cuh"
 
 namespace kib {
 namespace {
@@ -199,65 +200,36 @@ __global__ void kvq8_read_kernel(const __grid_constant__ Kvq8Cache c, const int3
 
 // --------------------------------------------------------------- attention
 
-struct Kvq8AttnParams {
-  Kvq8Cache c;
-  Kvq8Batch b;
-  const void* q;
-  void* out;
-  int heads;
-  int64_t q_stride, out_stride;
-  float scale_log2;  // softmax scale times log2(e)
-};
+// Dynamic shared memory above 48 KB has to be asked for, once per kernel.
+template <typename... KArgs>
+cudaError_t allow_smem(void (*kernel)(KArgs...), size_t bytes, bool* done) {
+  if (*done) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  *done = e == cudaSuccess;
+  return e;
+}
 
-// One warp per (row, query head), online softmax over its keys.
-template <typename T, int HD>
-__global__ void kvq8_attention_rows_kernel(const __grid_constant__ Kvq8AttnParams p) {
-  constexpr int V = HD / 32;
-  const int lane = threadIdx.x & 31, head = blockIdx.y;
-  const int row = static_cast<int>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (row >= p.b.rows) return;
-  int seq = -1;
-  Kvq8Seq s{0, 0, 0};
-  for (int i = 0; i < p.b.sequences; ++i) {
-    s = kvq8_seq(p.b, i);
-    if (row >= s.first && row < s.first + s.n) {
-      seq = i;
-      break;
-    }
-  }
-  float acc[V] = {}, m = -INFINITY, l = 0.0f;
-  if (seq >= 0) {
-    float q[V];
-    load_vec<T, V>(static_cast<const T*>(p.q) + row * p.q_stride + head * HD + lane * V, q);
-    const int kv_head = head / (p.heads / p.c.kv_heads);
-    const int end = min(s.length - s.n + row - s.first + 1, p.b.max_length);
-    for (int base = 0; base < end; base += p.c.page_tokens) {
-      const int page = kvq8_page(p.c, p.b, seq, base >> p.c.page_shift);
-      if (page < 0) continue;
-      const int64_t off = page * p.c.page_stride + kv_head * p.c.head_stride + lane * V;
-      const float ks = p.c.k_scale[static_cast<int64_t>(page) * p.c.kv_heads + kv_head] * p.scale_log2;
-      const float vs = p.c.v_scale[static_cast<int64_t>(page) * p.c.kv_heads + kv_head];
-      const int n = min(p.c.page_tokens, end - base);
-      for (int t = 0; t < n; ++t) {
-        int k[V], v[V];
-        load_codes<V>(p.c.k + off + t * p.c.token_stride, k);
-        load_codes<V>(p.c.v + off + t * p.c.token_stride, v);
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) dot += q[e] * static_cast<float>(k[e]);
-        dot = warp_sum(dot) * ks;
-        const float mn = fmaxf(m, dot), f = exp2f(m - mn), w = exp2f(dot - mn);
-        l = l * f + w;
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] = acc[e] * f + w * vs * static_cast<float>(v[e]);
-        m = mn;
-      }
-    }
-  }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] *= inv;
-  store_vec<T, V>(static_cast<T*>(p.out) + row * p.out_stride + head * HD + lane * V, acc);
+template <typename T, int HD, int NT>
+cudaError_t few_launch(const Kvq8AttnParams& p, int num_sms, cudaStream_t st) {
+  static bool ready = false;
+  cudaError_t e = allow_smem(kvq8_few_kernel<T, HD, NT>, few_smem<T, HD, NT>(), &ready);
+  if (e != cudaSuccess) return e;
+  const int ctas = std::min(num_sms * few_ctas_per_sm<HD>(), kMergeMaxCtas);
+  kvq8_few_kernel<T, HD, NT><<<ctas, kFewWarps * 32, few_smem<T, HD, NT>(), st>>>(p);
+  const int64_t rows = std::min<int64_t>(static_cast<int64_t>(p.b.max_rows) * p.group, p.few_limit);
+  const int groups = static_cast<int>((rows + 8 * NT - 1) / (8 * NT));
+  const dim3 grid(static_cast<unsigned>(p.b.sequences) * p.c.kv_heads * groups, static_cast<unsigned>(std::min<int64_t>(rows, 8 * NT)));
+  return launch_pdl(kvq8_merge_kernel<T, HD, NT>, grid, dim3(HD), 0, st, p, ctas, groups);
+}
+
+// Units of 8 rows while they hold all of a sequence's rows, else of 16: the
+// cache is read once per unit.
+bool few_wide(const Kvq8Batch& b, int group) { return static_cast<int64_t>(b.max_rows) * group > 8; }
+
+size_t few_workspace(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_sms) {
+  const size_t rows = few_wide(b, group) ? 16 : 8;
+  const size_t ctas = std::min(num_sms * (c.head_dim == 256 ? 1 : c.head_dim == 128 ? 2 : 3), kMergeMaxCtas);
+  return ctas * 2 * rows * static_cast<size_t>(c.head_dim + 2) * sizeof(float);
 }
 
 // -------------------------------------------------------------- host side
@@ -303,8 +275,8 @@ int make_cache(kib_ctx* ctx, const kib_kvq8_cache* in, Kvq8Cache* c) {
 
 int make_batch(kib_ctx* ctx, const kib_kvq8_batch* in, const Kvq8Cache& c, Kvq8Batch* b) {
   KIB_ARG(in, "kvq8: null batch");
-  KIB_ARG(in->sequences < (1ull << 16) && in->rows < (1ull << 31) && in->table_stride < (1ull << 31),
-          "kvq8: batch dimensions out of range (at most 65535 sequences)");
+  KIB_ARG(in->sequences <= kFewMaxSeqs && in->rows < (1ull << 31) && in->table_stride < (1ull << 31),
+          "kvq8: batch dimensions out of range (at most 4096 sequences)");
   KIB_ARG(in->max_rows <= in->rows, "kvq8: max_rows exceeds rows");
   KIB_ARG(in->rows == 0 || in->max_rows > 0, "kvq8: max_rows must be positive");
   KIB_ARG(in->sequences == 0 || (in->lengths && in->row_start), "kvq8: null batch pointer");
@@ -448,7 +420,7 @@ int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, cons
   KIB_ARG(elem_size(type), "kvq8_attention: type must be F32(0) or F16(1)");
   KIB_ARG(heads > 0 && heads <= 4096 && heads % static_cast<uint64_t>(c.kv_heads) == 0,
           "kvq8_attention: heads must be a multiple of kv_heads, at most 4096");
-  *bytes = 0;
+  *bytes = few_workspace(c, b, static_cast<int>(heads) / c.kv_heads, ctx->num_sms);
   return KIB_OK;
 }
 
@@ -472,11 +444,17 @@ int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8
   p.q = q;
   p.out = out;
   p.heads = static_cast<int>(heads);
+  p.group = p.heads / p.c.kv_heads;
   p.scale_log2 = scale * 1.4426950408889634f;
-  const dim3 grid(static_cast<unsigned>((p.b.rows + 7) / 8), static_cast<unsigned>(p.heads));
-#define CALL(T, HD) kvq8_attention_rows_kernel<T, HD><<<grid, 256, 0, op_stream(ctx, stream)>>>(p)
+  p.partial = static_cast<float*>(workspace);
+  p.few_limit = 0x7fffffff;
+  cudaError_t e;
+#define CALL(T, HD)                                                                            \
+  e = few_wide(p.b, p.group) ? few_launch<T, HD, 2>(p, ctx->num_sms, op_stream(ctx, stream))   \
+                             : few_launch<T, HD, 1>(p, ctx->num_sms, op_stream(ctx, stream))
   KVQ8_DISPATCH(type, p.c.head_dim, CALL);
 #undef CALL
+  if (e != cudaSuccess) return check_cuda(ctx, e, "kvq8_attention");
   return finish(ctx, stream, "kvq8_attention");
 }
 
