@@ -45,9 +45,10 @@ struct RowScale {
   float top, inv_t;
 };
 KIB_DEV float logit_weight(float l, const RowScale& r) {
-  // +infinity on top: only such logits have weight
-  if (l == -INFINITY) return 0.0f;
-  const float z = l == r.top ? 0.0f : __fmul_rn(__fsub_rn(l, r.top), r.inv_t);
+  // infinitely far below the top (with +infinity on top: all but such logits)
+  const float d = l == r.top ? 0.0f : __fsub_rn(l, r.top);
+  if (d == -INFINITY) return 0.0f;
+  const float z = __fmul_rn(d, r.inv_t);
   return expf(z);
 }
 // trunc(e * 2^40) for e in [0, 1] by shifting the significand (conversions to
@@ -247,35 +248,40 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(const __grid
 // ------------------------------------------------------------- by clusters
 //
 // A cluster of C CTAs takes one row: each CTA keeps its slice of the logits in
-// shared memory, so the row is read from HBM once, and every later pass runs
-// out of shared memory.  Cuts are found by histograms of kBins bins: the first
-// over z = (l - M) / T, which spreads the logits evenly (the leading bits of
-// a float would put most of a vocabulary in a few bins, and atomics on one
-// word run one after another), the next over the order keys inside the bin
-// that holds the boundary, until a bin is one key.  Counts take one 32-bit
-// shared atomic a logit, masses the non-zero ones of three (14 + 14 + 12
-// bits: a slice of 2^14 logits cannot overflow a word).  The CTAs add up their
-// histograms over distributed shared memory: CTA r sums share r of the bins,
-// then everyone gathers the sums and scans them redundantly.
+// shared memory, so the row is read from HBM once.  One pass turns the logits
+// into e_i; every later pass runs on those.
+//
+// Cuts are found by histograms of kBins bins over the bits of e, which are
+// ordered like e and near-uniform in log e (16 bins an octave, so a vocabulary
+// spreads over hundreds of bins; atomics on one word run one after another).
+// Counts take one 32-bit shared atomic a logit, masses the non-zero ones of
+// three (14 + 14 + 13 bits: a slice of 2^14 logits cannot overflow a word).
+// The tokens of the bin with the boundary go to a list, on which further
+// histograms narrow the bin to one value of e.  Where a cut falls inside a
+// group of equal e, the group is ordered by its logits (different logits may
+// round to one e), then by index.  The CTAs add up their histograms over
+// distributed shared memory: CTA r sums share r of the bins, then everyone
+// gathers the sums and scans them redundantly.
 
 constexpr int kSliceMax = 16384;
 constexpr int kClusterMax = 16;
 constexpr int kClThreads = 512;
 constexpr int kBins = 1024;
-constexpr float kBinsPerZ = kBins / 28.0f;  // below z = -28 every weight is 0 (2^-40 = e^-27.7)
+constexpr int kBinShift = 19;  // of the bits of e: 16 bins an octave, 40 octaves
+constexpr int kListMax = 2048;
+constexpr uint32_t kOneBits = 0x3f800000u;
 
 struct ClusterShared {
   uint32_t hist[3][kBins];
   u64 share[kBins];  // this CTA's summed bins (kBins / C of them)
   u64 sums[kBins];   // all of them, gathered
   u64 scan[kClThreads / 32];
+  uint16_t list[kListMax];
   u64 total;
-  float top;
-  int first;
-  uint32_t kmin, kmax;
-  int index;
   u64 before;
-  int bin;
+  float top;
+  int first, bin, index, listed;
+  uint32_t kmin, kmax;
 };
 
 template <typename T>
@@ -306,7 +312,7 @@ KIB_DEV u64 block_scan(u64 v, u64* s, u64* total) {
 }
 
 __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __grid_constant__ SampleParams p, int slice) {
-  extern __shared__ __align__(16) float xs[];
+  extern __shared__ __align__(16) float xs[];  // the slice's logits, then its e
   __shared__ ClusterShared sh;
   cg::cluster_group cl = cg::this_cluster();
   const unsigned C = cl.num_blocks(), rank = cl.block_rank();
@@ -326,6 +332,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   float* fs = reinterpret_cast<float*>(sh.scan);
   if (lane == 0) fs[warp] = top;
   if (tid == 0) sh.first = 0x7fffffff;
+  for (int b = tid; b < 3 * kBins; b += kClThreads) (&sh.hist[0][0])[b] = 0;
   __syncthreads();
   if (tid == 0) {
     for (int w = 1; w < kClThreads / 32; ++w) top = fmaxf(top, fs[w]);
@@ -357,121 +364,122 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   const int k = p.top_k ? p.top_k[row] : 0;
   const float top_p = p.top_p ? p.top_p[row] : 1.0f;
   const float min_p = p.min_p && p.min_p[row] > 0.0f ? fminf(p.min_p[row], 1.0f) : 0.0f;
-  auto key_logit = [](uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); };
-  auto z_bin = [&](float l) {
-    if (l == rs.top) return 0;
-    const float z = __fmul_rn(__fsub_rn(rs.top, l), rs.inv_t) * kBinsPerZ;
-    return z < kBins - 1 ? static_cast<int>(z) : kBins - 1;
+  const bool by_k = k > 0 && k < p.vocab, by_p = !(top_p >= 1.0f);
+
+  auto e_bits = [&](int i) { return __float_as_uint(xs[i]); };
+  auto logit_key = [&](int i) { return order_key(clean_logit(__ldg(x + i))); };
+  auto e_bin = [](uint32_t bits) { return static_cast<int>(min((kOneBits - bits) >> kBinShift, kBins - 1u)); };
+  auto add_mass = [&](int b, u64 w) {
+    const uint32_t w0 = static_cast<uint32_t>(w) & 0x3fffu, w1 = static_cast<uint32_t>(w >> 14) & 0x3fffu,
+                   w2 = static_cast<uint32_t>(w >> 28);
+    if (w0) atomicAdd(&sh.hist[0][b], w0);
+    if (w1) atomicAdd(&sh.hist[1][b], w1);
+    if (w2) atomicAdd(&sh.hist[2][b], w2);
   };
 
-  Cut cut{0u, 0x7fffffff};
-  bool partial = false;  // the cut keeps only some of the tokens with its key
-  // One selection: by count (the first `want` tokens) or by mass (the shortest
-  // prefix of what `cut` keeps that reaches the fraction top_p of its mass).
-  auto select = [&](bool by_count, u64 want) {
-    const Cut in = cut;
-    const u64 in_tied = by_count || in.key == 0 ? 0 : static_cast<u64>(in.ties) * fixed_weight(logit_weight(key_logit(in.key), rs));
-    u64 before = 0;
-    uint32_t klo = 0, khi = 0xffffffffu;  // the keys that are left
-    int level = 0, shift = 0;
-    for (;;) {
-      for (int b = tid; b < kBins; b += kClThreads) sh.hist[0][b] = sh.hist[1][b] = sh.hist[2][b] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kClThreads) {
-        const float l = xs[i];
-        const uint32_t key = order_key(l);
-        if (key < klo || key > khi) continue;
-        if (!by_count && key <= in.key) continue;
-        const int b = level == 0 ? z_bin(l) : static_cast<int>((khi - key) >> shift);
-        if (by_count) {
-          atomicAdd(&sh.hist[0][b], 1u);
-        } else {
-          const u64 w = fixed_weight(logit_weight(l, rs));
-          const uint32_t w0 = static_cast<uint32_t>(w) & 0x3fffu, w1 = static_cast<uint32_t>(w >> 14) & 0x3fffu,
-                         w2 = static_cast<uint32_t>(w >> 28);
-          if (w0) atomicAdd(&sh.hist[0][b], w0);
-          if (w1) atomicAdd(&sh.hist[1][b], w1);
-          if (w2) atomicAdd(&sh.hist[2][b], w2);
-        }
+  // logits to weights, with the first histogram on the way
+  for (int i = tid; i < n; i += kClThreads) {
+    const float e = logit_weight(xs[i], rs);
+    xs[i] = e;
+    if (by_k) atomicAdd(&sh.hist[0][e_bin(__float_as_uint(e))], 1u);
+    else if (by_p) add_mass(e_bin(__float_as_uint(e)), fixed_weight(e));
+  }
+
+  // What is kept: bits of e above cut.bits; of those equal to it, all, or
+  // (partial) those with a logit key above cut.key, and with it up to index cut.last.
+  struct {
+    uint32_t bits, key;
+    int last;
+    bool partial;
+  } cut = {0u, 0u, 0x7fffffff, false};
+  auto in_cut = [&](int i) {
+    const uint32_t b = e_bits(i);
+    if (b != cut.bits || !cut.partial) return b >= cut.bits;
+    const uint32_t key = logit_key(i);
+    return key > cut.key || (key == cut.key && i0 + i <= cut.last);
+  };
+
+  // The cluster's sums of the histogram (of counts or of masses) in sh.sums;
+  // the bin at which they reach want_of(their total), with what lies before it.
+  auto find_bin = [&](bool masses, u64 before, auto want_of, u64* want, u64* here) -> int {
+    cl.sync();
+    const int per = kBins / static_cast<int>(C), b0 = static_cast<int>(rank) * per;
+    for (int j = tid; j < per; j += kClThreads) {
+      u64 v = 0;
+#pragma unroll 4
+      for (unsigned r = 0; r < C; ++r) {
+        const uint32_t* h = peer(cl, &sh.hist[0][0], r);
+        v += h[b0 + j];
+        if (masses) v += (static_cast<u64>(h[kBins + b0 + j]) << 14) + (static_cast<u64>(h[2 * kBins + b0 + j]) << 28);
       }
-      cl.sync();
-      const int per = kBins / static_cast<int>(C), b0 = static_cast<int>(rank) * per;
-      for (int j = tid; j < per; j += kClThreads) {
-        u64 v = 0;
-        for (unsigned r = 0; r < C; ++r) {
-          const uint32_t* h = peer(cl, &sh.hist[0][0], r);
-          v += h[b0 + j];
-          if (!by_count) v += (static_cast<u64>(h[kBins + b0 + j]) << 14) + (static_cast<u64>(h[2 * kBins + b0 + j]) << 28);
-        }
-        sh.share[j] = v;
-      }
-      cl.sync();
-      for (int b = tid; b < kBins; b += kClThreads) sh.sums[b] = *peer(cl, &sh.share[b % per], static_cast<unsigned>(b / per));
-      __syncthreads();
-      constexpr int PER = kBins / kClThreads;
-      u64 v[PER], mine = 0, total = 0;
+      sh.share[j] = v;
+    }
+    cl.sync();
+    constexpr int PER = kBins / kClThreads;
+    u64 v[PER], mine = 0, total = 0;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) v[e] = sh.sums[tid * PER + e], mine += v[e];
-      u64 acc = before + block_scan(mine, sh.scan, &total);
-      if (level == 0 && !by_count) {
-        const double limit = static_cast<double>(total + in_tied) * static_cast<double>(top_p);
-        want = limit > 1.0 ? static_cast<u64>(limit) : 1;
-        if (total < want) {  // the boundary lies among the ties of the enclosing cut
-          const u64 w = fixed_weight(logit_weight(key_logit(in.key), rs));
-          const int ties = static_cast<int>(min((want - total + w - 1) / w, static_cast<u64>(in.ties)));
-          partial = partial || ties < in.ties;
-          cut.ties = ties;
-          return;
-        }
-      }
+    for (int e = 0; e < PER; ++e) {
+      const int b = tid * PER + e;
+      v[e] = *peer(cl, &sh.share[b % per], static_cast<unsigned>(b / per));
+      mine += v[e];
+    }
+    for (int b = tid; b < 3 * kBins; b += kClThreads) (&sh.hist[0][0])[b] = 0;  // for the next histogram
+    if (tid == 0) sh.bin = kBins - 1, sh.before = before;
+    u64 acc = before + block_scan(mine, sh.scan, &total);
+    *want = want_of(total);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        if (acc < want && want <= acc + v[e]) sh.bin = tid * PER + e, sh.before = acc;
-        acc += v[e];
-      }
-      __syncthreads();
-      const int bin = sh.bin;
-      before = sh.before;
-      const u64 here = sh.sums[bin];
-      if (level == 0) {
-        // the range of keys in the bin
-        uint32_t lo = 0xffffffffu, hi = 0;
-        for (int i = tid; i < n; i += kClThreads) {
-          const float l = xs[i];
-          const uint32_t key = order_key(l);
-          if ((by_count || key > in.key) && z_bin(l) == bin) lo = min(lo, key), hi = max(hi, key);
-        }
-        lo = __reduce_min_sync(0xffffffffu, lo);
-        hi = __reduce_max_sync(0xffffffffu, hi);
-        if (tid == 0) sh.kmin = 0xffffffffu, sh.kmax = 0;
-        __syncthreads();
-        if (lane == 0) atomicMin(&sh.kmin, lo), atomicMax(&sh.kmax, hi);
-        cl.sync();
-        klo = __reduce_min_sync(0xffffffffu, lane < static_cast<int>(C) ? *peer(cl, &sh.kmin, lane) : 0xffffffffu);
-        khi = __reduce_max_sync(0xffffffffu, lane < static_cast<int>(C) ? *peer(cl, &sh.kmax, lane) : 0u);
-      } else {
-        // bin = (khi - key) >> shift
-        const uint32_t h = khi - (static_cast<uint32_t>(bin) << shift);
-        const uint32_t size = 1u << shift;
-        klo = h - klo >= size - 1 ? h - (size - 1) : klo;
-        khi = h;
-      }
-      if (klo >= khi || level == 8) {  // at most five levels: 2^32 keys, 2^10 a level
-        const u64 w = by_count ? 1 : max(fixed_weight(logit_weight(key_logit(klo), rs)), 1ull);
-        const u64 ties = (want - before + w - 1) / w, group = here / w;
-        cut.key = klo;
-        cut.ties = static_cast<int>(ties);
-        partial = ties < group;
-        return;
-      }
-      ++level;
-      const uint32_t range = khi - klo;
-      shift = max(0, 22 - __clz(range));  // range >> shift < 1024
-      __syncthreads();                    // sh.bin and the histogram are written again
+    for (int e = 0; e < PER; ++e) {
+      sh.sums[tid * PER + e] = v[e];
+      if (acc < *want && *want <= acc + v[e]) sh.bin = tid * PER + e, sh.before = acc;
+      acc += v[e];
+    }
+    __syncthreads();
+    *here = sh.sums[sh.bin];
+    return sh.bin;
+  };
+  // The listed tokens, or all that `member` holds of where the list is too short.
+  bool short_list = false;
+  auto make_list = [&](auto member) {
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kClThreads) {
+      if (!member(i)) continue;
+      const int at = atomicAdd(&sh.listed, 1);
+      if (at < kListMax) sh.list[at] = static_cast<uint16_t>(i);
+    }
+    __syncthreads();
+    short_list = sh.listed <= kListMax;
+  };
+  auto for_list = [&](auto member, auto what) {
+    if (short_list) {
+      for (int j = tid; j < sh.listed; j += kClThreads) what(sh.list[j]);
+    } else {
+      for (int i = tid; i < n; i += kClThreads)
+        if (member(i)) what(i);
     }
   };
-  if (k > 0 && k < p.vocab) select(true, static_cast<u64>(k));
-  if (!(top_p >= 1.0f)) select(false, 0);
+  // Narrows [klo, khi] to the value at which the running sum (from `before`,
+  // values in descending order) reaches want.
+  auto narrow = [&](bool masses, auto member, auto value, uint32_t klo, uint32_t khi, u64 want, u64* before, u64* here) -> uint32_t {
+    for (int level = 0; klo < khi && level < 8; ++level) {  // five at most: 2^32 values, 2^10 a level
+      const int shift = max(0, 22 - __clz(khi - klo));
+      for_list(member, [&](int i) {
+        const uint32_t v = value(i);
+        if (v < klo || v > khi) return;
+        const int b = static_cast<int>((khi - v) >> shift);
+        if (masses) add_mass(b, fixed_weight(xs[i]));
+        else atomicAdd(&sh.hist[0][b], 1u);
+      });
+      u64 w;
+      const int bin = find_bin(masses, *before, [&](u64) { return want; }, &w, here);
+      *before = sh.before;
+      const uint32_t h = khi - (static_cast<uint32_t>(bin) << shift), size = 1u << shift;
+      klo = h - klo >= size - 1 ? h - (size - 1) : klo;
+      khi = h;
+      __syncthreads();  // sh.bin is written again
+    }
+    return klo;
+  };
 
   // Weights summed in index order: the token (relative to the slice) at which
   // the running sum exceeds aim(total), in the CTA that holds it (-1 in the
@@ -482,66 +490,109 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     block_scan(mine, sh.scan, &all);
     if (tid == 0) sh.total = all;
     cl.sync();
-    u64 sum = 0;
-    for (unsigned r = 0; r < C; ++r) sum += *peer(cl, &sh.total, r);
-    *total = sum;
-    const u64 aim = aim_of(sum);
-    u64 base = 0;
-    *owner = C - 1;
-    for (unsigned r = 0; r < C; ++r) {
-      const u64 v = *peer(cl, &sh.total, r);
-      if (aim < base + v) {
-        *owner = r;
-        break;
-      }
-      base += v;
-    }
-    if (*owner != rank) return -1;
-    constexpr int W = kClThreads / 32;
-    const int rounds = (n + kClThreads - 1) / kClThreads;
-    u64* table = sh.sums;
-    for (int j = 0; j < rounds; ++j) {
-      const int i = j * kClThreads + tid;
-      u64 v = i < n ? weight(i) : 0;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) table[j * W + warp] = v;
-    }
-    __syncthreads();
-    const u64 v = tid < rounds * W ? table[tid] : 0;
-    const u64 acc = base + block_scan(v, sh.scan, &all);
-    if (acc <= aim && aim < acc + v) sh.bin = tid, sh.before = acc;
-    __syncthreads();
-    const int i = sh.bin / W * kClThreads + sh.bin % W * 32 + lane;
-    const u64 w = i < n ? weight(i) : 0;
-    u64 inc = w;
+    const u64 theirs = lane < static_cast<int>(C) ? *peer(cl, &sh.total, lane) : 0;
+    u64 inc = theirs;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const u64 u = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += u;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, sh.before + inc > aim);
-    return __shfl_sync(0xffffffffu, i, __ffs(past) - 1);
+    *total = __shfl_sync(0xffffffffu, inc, 31);
+    const u64 aim = aim_of(*total);
+    *owner = min(static_cast<unsigned>(__ffs(__ballot_sync(0xffffffffu, inc > aim)) - 1), C - 1);
+    const u64 base = __shfl_sync(0xffffffffu, inc - theirs, *owner);
+    if (*owner != rank) return -1;
+    constexpr int W = kClThreads / 32;
+    const int rounds = (n + kClThreads - 1) / kClThreads;
+    for (int j = 0; j < rounds; ++j) {
+      const int i = j * kClThreads + tid;
+      u64 v = i < n ? weight(i) : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) sh.sums[j * W + warp] = v;
+    }
+    if (tid == 0) sh.bin = 0, sh.before = base;
+    __syncthreads();
+    const u64 v = tid < rounds * W ? sh.sums[tid] : 0;
+    const u64 acc = base + block_scan(v, sh.scan, &all);
+    if (acc <= aim && aim < acc + v) sh.bin = tid, sh.before = acc;
+    __syncthreads();
+    const int i = sh.bin / W * kClThreads + sh.bin % W * 32 + lane;
+    u64 run = i < n ? weight(i) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 u = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += u;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, sh.before + run > aim);
+    return __shfl_sync(0xffffffffu, i, max(__ffs(past) - 1, 0));
   };
 
-  int last_tie = 0x7fffffff;  // index of the last token that is kept with the cut's key
-  unsigned owner;
-  u64 total;
-  if (partial) {
-    const int at = locate([&](int i) -> u64 { return order_key(xs[i]) == cut.key; },
-                          [&](u64) -> u64 { return static_cast<u64>(cut.ties - 1); }, &owner, &total);
+  // Cuts at the running sum `want_of(total)` of the histogram that is ready in shared memory.
+  auto select = [&](bool masses, auto want_of) {
+    u64 want, here;
+    const int bin = find_bin(masses, 0, want_of, &want, &here);
+    u64 before = sh.before;
+    const uint32_t khi = kOneBits - (static_cast<uint32_t>(bin) << kBinShift);
+    const uint32_t klo = bin == kBins - 1 ? 0u : khi - ((1u << kBinShift) - 1);
+    auto member = [&](int i) {
+      const uint32_t b = e_bits(i);
+      return b >= klo && b <= khi && (!masses || in_cut(i));
+    };
+    make_list(member);
+    const uint32_t bits = narrow(masses, member, [&](int i) { return e_bits(i); }, klo, khi, want, &before, &here);
+    const u64 w = masses ? max(fixed_weight(__uint_as_float(bits)), 1ull) : 1;
+    u64 ties = (want - before + w - 1) / w;
+    // (tokens without weight need no order)
+    const bool partial = fixed_weight(__uint_as_float(bits)) > 0 && (ties < here / w || (masses && cut.partial && bits == cut.bits));
+    cut.bits = bits;
+    cut.partial = partial;
+    if (!partial) return;
+    // the first `ties` of the tokens with this e: by logit, then by index
+    auto equal = [&](int i) { return e_bits(i) == bits; };
+    if (tid == 0) sh.kmin = 0xffffffffu, sh.kmax = 0;
+    make_list(equal);
+    uint32_t lo = 0xffffffffu, hi = 0;
+    for_list(equal, [&](int i) {
+      const uint32_t key = logit_key(i);
+      lo = min(lo, key), hi = max(hi, key);
+    });
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) atomicMin(&sh.kmin, lo), atomicMax(&sh.kmax, hi);
+    cl.sync();
+    lo = __reduce_min_sync(0xffffffffu, lane < static_cast<int>(C) ? *peer(cl, &sh.kmin, lane) : 0xffffffffu);
+    hi = __reduce_max_sync(0xffffffffu, lane < static_cast<int>(C) ? *peer(cl, &sh.kmax, lane) : 0u);
+    before = 0;
+    cut.key = narrow(false, equal, logit_key, lo, hi, ties, &before, &here);
+    ties -= before;
+    unsigned owner;
+    u64 total;
+    const uint32_t key = cut.key;
+    const int at = locate([&](int i) -> u64 { return equal(i) && logit_key(i) == key; }, [&](u64) { return ties - 1; }, &owner, &total);
     if (at >= 0 && tid == 0) sh.index = i0 + at;
     cl.sync();
-    last_tie = *peer(cl, &sh.index, owner);
+    cut.last = *peer(cl, &sh.index, owner);
+  };
+  if (by_k) select(false, [&](u64) { return static_cast<u64>(k); });
+  if (by_p) {
+    if (by_k) {
+      for (int i = tid; i < n; i += kClThreads)
+        if (in_cut(i)) add_mass(e_bin(e_bits(i)), fixed_weight(xs[i]));
+    }
+    select(true, [&](u64 total) {
+      const double limit = static_cast<double>(total) * static_cast<double>(top_p);
+      return limit > 1.0 ? static_cast<u64>(limit) : 1ull;
+    });
   }
+
   auto kept = [&](int i) -> u64 {
-    const float l = xs[i];
-    const uint32_t key = order_key(l);
-    if (key < cut.key || (key == cut.key && i0 + i > last_tie)) return 0;
-    const float e = logit_weight(l, rs);
-    return e >= min_p || l == top ? fixed_weight(e) : 0;
+    const float e = xs[i];
+    return e >= min_p && in_cut(i) ? fixed_weight(e) : 0;
   };
   const float u = p.uniform[row];
+  unsigned owner;
+  u64 total;
   const int token = locate(kept,
                            [&](u64 all) -> u64 {
                              const double f = static_cast<double>(all) * static_cast<double>(u);
