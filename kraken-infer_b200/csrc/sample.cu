@@ -260,8 +260,12 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(const __grid
 // histograms narrow the bin to one value of e.  Where a cut falls inside a
 // group of equal e, the group is ordered by its logits (different logits may
 // round to one e), then by index.  The CTAs add up their histograms over
-// distributed shared memory: CTA r sums share r of the bins, then everyone
-// gathers the sums and scans them redundantly.
+// distributed shared memory: each adds its non-zero bins to share b / (kBins / C)
+// of CTA r by remote 64-bit atomics (integers: in any order the same), then
+// everyone gathers the shares and scans them redundantly, one cluster barrier
+// a histogram.  Three copies of a share take turns: a copy is cleared behind
+// the barrier after the one it was gathered behind, a barrier before its next
+// use.
 
 constexpr int kSliceMax = 16384;
 constexpr int kClusterMax = 16;
@@ -273,8 +277,7 @@ constexpr uint32_t kOneBits = 0x3f800000u;
 
 struct ClusterShared {
   uint32_t hist[3][kBins];
-  u64 share[kBins];  // this CTA's summed bins (kBins / C of them)
-  u64 sums[kBins];   // all of them, gathered
+  u64 sums[kBins];  // the cluster's bins, gathered
   u64 scan[kClThreads / 32];
   uint16_t list[kListMax];
   u64 total;
@@ -312,7 +315,9 @@ KIB_DEV u64 block_scan(u64 v, u64* s, u64* total) {
 }
 
 __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __grid_constant__ SampleParams p, int slice) {
-  extern __shared__ __align__(16) float xs[];  // the slice's logits, then its e
+  extern __shared__ __align__(16) float xs[];  // the slice's logits, then its e; padded with weightless tokens
+  float4* x4 = reinterpret_cast<float4*>(xs);
+  u64* shares = reinterpret_cast<u64*>(xs + slice);  // [3][kBins / C]
   __shared__ ClusterShared sh;
   cg::cluster_group cl = cg::this_cluster();
   const unsigned C = cl.num_blocks(), rank = cl.block_rank();
@@ -320,14 +325,33 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   const int i0 = static_cast<int>(rank) * slice, n = max(0, min(slice, p.vocab - i0));
   const float* x = p.logits + static_cast<int64_t>(row) * p.row_stride + i0;
 
+  const float t = p.temperature ? __ldg(p.temperature + row) : 1.0f;
+  const int k = p.top_k ? __ldg(p.top_k + row) : 0;
+  const float top_p = p.top_p ? __ldg(p.top_p + row) : 1.0f;
+  const float min_p0 = p.min_p ? __ldg(p.min_p + row) : 0.0f;
+  const float min_p = min_p0 > 0.0f ? fminf(min_p0, 1.0f) : 0.0f;
+  const float u = __ldg(p.uniform + row), inv_t = __fdiv_rn(1.0f, t);
+  const int n4 = slice / 4, per = kBins / static_cast<int>(C);
+
   // the slice, cleaned, and its maximum
   float top = -INFINITY;
+  if (i0 + slice <= p.vocab && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+#pragma unroll 4
+    for (int i = tid; i < n4; i += kClThreads) {
+      float4 l = __ldg(reinterpret_cast<const float4*>(x) + i);
+      l = make_float4(clean_logit(l.x), clean_logit(l.y), clean_logit(l.z), clean_logit(l.w));
+      x4[i] = l;
+      top = fmaxf(fmaxf(top, fmaxf(l.x, l.y)), fmaxf(l.z, l.w));
+    }
+  } else {
 #pragma unroll 8
-  for (int i = tid; i < n; i += kClThreads) {
-    const float l = clean_logit(__ldg(x + i));
-    xs[i] = l;
-    top = fmaxf(top, l);
+    for (int i = tid; i < slice; i += kClThreads) {
+      const float l = i < n ? clean_logit(__ldg(x + i)) : -INFINITY;
+      xs[i] = l;
+      top = fmaxf(top, l);
+    }
   }
+  for (int j = tid; j < 3 * per; j += kClThreads) shares[j] = 0;
   top = warp_max(top);
   float* fs = reinterpret_cast<float*>(sh.scan);
   if (lane == 0) fs[warp] = top;
@@ -341,7 +365,6 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   cl.sync();
   top = warp_max(lane < static_cast<int>(C) ? *peer(cl, &sh.top, lane) : -INFINITY);
 
-  const float t = p.temperature ? p.temperature[row] : 1.0f;
   if (top == -INFINITY || !(t > 1e-6f)) {
     int best = 0x7fffffff;
     if (top > -INFINITY)
@@ -360,14 +383,11 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     cl.sync();
     return;
   }
-  const RowScale rs{top, __fdiv_rn(1.0f, t)};
-  const int k = p.top_k ? p.top_k[row] : 0;
-  const float top_p = p.top_p ? p.top_p[row] : 1.0f;
-  const float min_p = p.min_p && p.min_p[row] > 0.0f ? fminf(p.min_p[row], 1.0f) : 0.0f;
+  const RowScale rs{top, inv_t};
   const bool by_k = k > 0 && k < p.vocab, by_p = !(top_p >= 1.0f);
 
   auto e_bits = [&](int i) { return __float_as_uint(xs[i]); };
-  auto logit_key = [&](int i) { return order_key(clean_logit(__ldg(x + i))); };
+  auto logit_key = [&](int i) { return order_key(i < n ? clean_logit(__ldg(x + i)) : -INFINITY); };
   auto e_bin = [](uint32_t bits) { return static_cast<int>(min((kOneBits - bits) >> kBinShift, kBins - 1u)); };
   auto add_mass = [&](int b, u64 w) {
     const uint32_t w0 = static_cast<uint32_t>(w) & 0x3fffu, w1 = static_cast<uint32_t>(w >> 14) & 0x3fffu,
@@ -378,11 +398,17 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   };
 
   // logits to weights, with the first histogram on the way
-  for (int i = tid; i < n; i += kClThreads) {
-    const float e = logit_weight(xs[i], rs);
-    xs[i] = e;
-    if (by_k) atomicAdd(&sh.hist[0][e_bin(__float_as_uint(e))], 1u);
-    else if (by_p) add_mass(e_bin(__float_as_uint(e)), fixed_weight(e));
+  for (int i = tid; i < n4; i += kClThreads) {
+    const float4 l = x4[i];
+    const float e[4] = {logit_weight(l.x, rs), logit_weight(l.y, rs), logit_weight(l.z, rs), logit_weight(l.w, rs)};
+    x4[i] = make_float4(e[0], e[1], e[2], e[3]);
+    if (by_k) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) atomicAdd(&sh.hist[0][e_bin(__float_as_uint(e[j]))], 1u);
+    } else if (by_p) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) add_mass(e_bin(__float_as_uint(e[j])), fixed_weight(e[j]));
+    }
   }
 
   // What is kept: bits of e above cut.bits; of those equal to it, all, or
@@ -401,29 +427,31 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
 
   // The cluster's sums of the histogram (of counts or of masses) in sh.sums;
   // the bin at which they reach want_of(their total), with what lies before it.
+  int turn = 0;
   auto find_bin = [&](bool masses, u64 before, auto want_of, u64* want, u64* here) -> int {
-    cl.sync();
-    const int per = kBins / static_cast<int>(C), b0 = static_cast<int>(rank) * per;
-    for (int j = tid; j < per; j += kClThreads) {
-      u64 v = 0;
-#pragma unroll 4
-      for (unsigned r = 0; r < C; ++r) {
-        const uint32_t* h = peer(cl, &sh.hist[0][0], r);
-        v += h[b0 + j];
-        if (masses) v += (static_cast<u64>(h[kBins + b0 + j]) << 14) + (static_cast<u64>(h[2 * kBins + b0 + j]) << 28);
+    u64* mine_at = shares + turn * per;
+    turn = turn == 2 ? 0 : turn + 1;
+    __syncthreads();
+    for (int b = tid; b < kBins; b += kClThreads) {
+      u64 v = sh.hist[0][b];
+      sh.hist[0][b] = 0;  // for the next histogram
+      if (masses) {
+        v += (static_cast<u64>(sh.hist[1][b]) << 14) + (static_cast<u64>(sh.hist[2][b]) << 28);
+        sh.hist[1][b] = sh.hist[2][b] = 0;
       }
-      sh.share[j] = v;
+      if (v) atomicAdd(peer(cl, mine_at + b % per, static_cast<unsigned>(b / per)), v);
     }
     cl.sync();
+    // the copy of the histogram before last has been gathered by everyone
+    for (int j = tid; j < per; j += kClThreads) shares[(turn == 2 ? 0 : turn + 1) * per + j] = 0;
     constexpr int PER = kBins / kClThreads;
     u64 v[PER], mine = 0, total = 0;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
       const int b = tid * PER + e;
-      v[e] = *peer(cl, &sh.share[b % per], static_cast<unsigned>(b / per));
+      v[e] = *peer(cl, mine_at + b % per, static_cast<unsigned>(b / per));
       mine += v[e];
     }
-    for (int b = tid; b < 3 * kBins; b += kClThreads) (&sh.hist[0][0])[b] = 0;  // for the next histogram
     if (tid == 0) sh.bin = kBins - 1, sh.before = before;
     u64 acc = before + block_scan(mine, sh.scan, &total);
     *want = want_of(total);
@@ -439,13 +467,18 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   };
   // The listed tokens, or all that `member` holds of where the list is too short.
   bool short_list = false;
-  auto make_list = [&](auto member) {
+  auto make_list = [&](uint32_t klo, uint32_t khi, auto member) {
     if (tid == 0) sh.listed = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kClThreads) {
-      if (!member(i)) continue;
-      const int at = atomicAdd(&sh.listed, 1);
-      if (at < kListMax) sh.list[at] = static_cast<uint16_t>(i);
+    for (int q = tid; q < n4; q += kClThreads) {
+      const uint4 b = reinterpret_cast<const uint4*>(xs)[q];
+      const uint32_t bits[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (bits[j] < klo || bits[j] > khi || !member(4 * q + j)) continue;
+        const int at = atomicAdd(&sh.listed, 1);
+        if (at < kListMax) sh.list[at] = static_cast<uint16_t>(4 * q + j);
+      }
     }
     __syncthreads();
     short_list = sh.listed <= kListMax;
@@ -454,7 +487,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     if (short_list) {
       for (int j = tid; j < sh.listed; j += kClThreads) what(sh.list[j]);
     } else {
-      for (int i = tid; i < n; i += kClThreads)
+      for (int i = tid; i < slice; i += kClThreads)
         if (member(i)) what(i);
     }
   };
@@ -485,8 +518,12 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   // the running sum exceeds aim(total), in the CTA that holds it (-1 in the
   // others); *owner is that CTA's rank.
   auto locate = [&](auto weight, auto aim_of, unsigned* owner, u64* total) -> int {
-    u64 mine = 0, all = 0;
-    for (int i = tid; i < n; i += kClThreads) mine += weight(i);
+    // weight(q, w): the weights of tokens 4 q .. 4 q + 3
+    u64 mine = 0, all = 0, w[4];
+    for (int q = tid; q < n4; q += kClThreads) {
+      weight(q, w);
+      mine += (w[0] + w[1]) + (w[2] + w[3]);
+    }
     block_scan(mine, sh.scan, &all);
     if (tid == 0) sh.total = all;
     cl.sync();
@@ -503,10 +540,14 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     const u64 base = __shfl_sync(0xffffffffu, inc - theirs, *owner);
     if (*owner != rank) return -1;
     constexpr int W = kClThreads / 32;
-    const int rounds = (n + kClThreads - 1) / kClThreads;
+    const int rounds = (n4 + kClThreads - 1) / kClThreads;
     for (int j = 0; j < rounds; ++j) {
-      const int i = j * kClThreads + tid;
-      u64 v = i < n ? weight(i) : 0;
+      const int q = j * kClThreads + tid;
+      u64 v = 0;
+      if (q < n4) {
+        weight(q, w);
+        v = (w[0] + w[1]) + (w[2] + w[3]);
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       if (lane == 0) sh.sums[j * W + warp] = v;
@@ -517,15 +558,25 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     const u64 acc = base + block_scan(v, sh.scan, &all);
     if (acc <= aim && aim < acc + v) sh.bin = tid, sh.before = acc;
     __syncthreads();
-    const int i = sh.bin / W * kClThreads + sh.bin % W * 32 + lane;
-    u64 run = i < n ? weight(i) : 0;
+    const int q = sh.bin / W * kClThreads + sh.bin % W * 32 + lane;
+    w[0] = w[1] = w[2] = w[3] = 0;
+    if (q < n4) weight(q, w);
+    const u64 four = (w[0] + w[1]) + (w[2] + w[3]);
+    u64 run = four;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const u64 u = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += u;
+      const u64 u2 = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += u2;
     }
     const unsigned past = __ballot_sync(0xffffffffu, sh.before + run > aim);
-    return __shfl_sync(0xffffffffu, i, max(__ffs(past) - 1, 0));
+    run += sh.before - four;
+    int at = 4 * q;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      run += w[j];
+      at += run <= aim;
+    }
+    return __shfl_sync(0xffffffffu, at, max(__ffs(past) - 1, 0));
   };
 
   // Cuts at the running sum `want_of(total)` of the histogram that is ready in shared memory.
@@ -539,7 +590,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
       const uint32_t b = e_bits(i);
       return b >= klo && b <= khi && (!masses || in_cut(i));
     };
-    make_list(member);
+    make_list(klo, khi, [&](int i) { return !masses || in_cut(i); });
     const uint32_t bits = narrow(masses, member, [&](int i) { return e_bits(i); }, klo, khi, want, &before, &here);
     const u64 w = masses ? max(fixed_weight(__uint_as_float(bits)), 1ull) : 1;
     u64 ties = (want - before + w - 1) / w;
@@ -551,7 +602,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     // the first `ties` of the tokens with this e: by logit, then by index
     auto equal = [&](int i) { return e_bits(i) == bits; };
     if (tid == 0) sh.kmin = 0xffffffffu, sh.kmax = 0;
-    make_list(equal);
+    make_list(bits, bits, [](int) { return true; });
     uint32_t lo = 0xffffffffu, hi = 0;
     for_list(equal, [&](int i) {
       const uint32_t key = logit_key(i);
@@ -569,7 +620,12 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     unsigned owner;
     u64 total;
     const uint32_t key = cut.key;
-    const int at = locate([&](int i) -> u64 { return equal(i) && logit_key(i) == key; }, [&](u64) { return ties - 1; }, &owner, &total);
+    const int at = locate(
+        [&](int q, u64(&w4)[4]) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w4[j] = equal(4 * q + j) && logit_key(4 * q + j) == key;
+        },
+        [&](u64) { return ties - 1; }, &owner, &total);
     if (at >= 0 && tid == 0) sh.index = i0 + at;
     cl.sync();
     cut.last = *peer(cl, &sh.index, owner);
@@ -577,8 +633,13 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   if (by_k) select(false, [&](u64) { return static_cast<u64>(k); });
   if (by_p) {
     if (by_k) {
-      for (int i = tid; i < n; i += kClThreads)
-        if (in_cut(i)) add_mass(e_bin(e_bits(i)), fixed_weight(xs[i]));
+      for (int q = tid; q < n4; q += kClThreads) {
+        const uint4 b = reinterpret_cast<const uint4*>(xs)[q];
+        const uint32_t bits[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (bits[j] >= cut.bits && in_cut(4 * q + j)) add_mass(e_bin(bits[j]), fixed_weight(__uint_as_float(bits[j])));
+      }
     }
     select(true, [&](u64 total) {
       const double limit = static_cast<double>(total) * static_cast<double>(top_p);
@@ -586,11 +647,16 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     });
   }
 
-  auto kept = [&](int i) -> u64 {
-    const float e = xs[i];
-    return e >= min_p && in_cut(i) ? fixed_weight(e) : 0;
+  const uint32_t low = max(cut.bits, __float_as_uint(min_p));
+  auto kept = [&](int q, u64(&w)[4]) {
+    const uint4 b = reinterpret_cast<const uint4*>(xs)[q];
+    const uint32_t bits[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = 0;
+      if (bits[j] >= low && (bits[j] != cut.bits || !cut.partial || in_cut(4 * q + j))) w[j] = fixed_weight(__uint_as_float(bits[j]));
+    }
   };
-  const float u = p.uniform[row];
   unsigned owner;
   u64 total;
   const int token = locate(kept,
@@ -601,7 +667,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
                            &owner, &total);
   if (token >= 0 && tid == 0) {
     p.token[row] = i0 + token;
-    if (p.prob) p.prob[row] = static_cast<float>(static_cast<double>(kept(token)) / static_cast<double>(total));
+    if (p.prob) p.prob[row] = static_cast<float>(static_cast<double>(fixed_weight(xs[token])) / static_cast<double>(total));
   }
   cl.sync();  // no CTA leaves while another may read its shared memory
 }
@@ -610,7 +676,8 @@ cudaError_t sample_cluster_launch(const SampleParams& p, int num_sms, cudaStream
   static bool ready = false;
   cudaError_t e;
   if (!ready) {
-    e = cudaFuncSetAttribute(sample_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceMax * 4);
+    e = cudaFuncSetAttribute(sample_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceMax * 4 + 3 * kBins * 8);
+    pin_carveout(sample_cluster_kernel);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_cluster_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     ready = true;
@@ -619,11 +686,11 @@ cudaError_t sample_cluster_launch(const SampleParams& p, int num_sms, cudaStream
   int c = 1;
   while (c * kSliceMax < p.vocab) c *= 2;
   while (c < kClusterMax && static_cast<int64_t>(p.rows) * c * 2 <= num_sms && p.vocab / (2 * c) >= 2048) c *= 2;
-  const int slice = ((p.vocab + c - 1) / c + 31) / 32 * 32;
+  const int slice = ((p.vocab + c - 1) / c + 127) / 128 * 128;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * static_cast<unsigned>(c));
   cfg.blockDim = dim3(kClThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(slice) * sizeof(float);
+  cfg.dynamicSmemBytes = static_cast<size_t>(slice) * sizeof(float) + 3 * kBins / c * sizeof(u64);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
