@@ -7,7 +7,9 @@
 #include <string>
 
 #include "kib_ctx.cuh"
-#include "kvq8_few.cuh"
+#include <cudaTypedefs.h>
+
+#include "kvq8_many.cuh"
 
 namespace kib {
 namespace {
@@ -232,6 +234,91 @@ size_t few_workspace(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_
   return ctas * 2 * rows * static_cast<size_t>(c.head_dim + 2) * sizeof(float);
 }
 
+// Rows (times the group) up to which a sequence is the few-row kernel's.
+constexpr int kFewLimit = 64;
+bool any_many(const Kvq8Batch& b, int group) { return static_cast<int64_t>(b.max_rows) * group > kFewLimit; }
+
+// The workspace of the many-row path, in this order behind the records.
+struct ManyLayout {
+  size_t partial, k16, v16, scales, seq_off, units, cum, cta_unit, count, bytes;
+  int64_t tot_pad, max_units;
+};
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_length, int group, int num_sms) {
+  ManyLayout m = {};
+  const int64_t bound = static_cast<int64_t>(b.max_length) * b.sequences;
+  if (total_length <= 0 || total_length > bound) total_length = bound;
+  m.tot_pad = (total_length + kManyKeys - 1) / kManyKeys * kManyKeys + static_cast<int64_t>(b.sequences) * kManyKeys;
+  m.max_units = (static_cast<int64_t>(b.rows) * group / kManyRows + b.sequences) * c.kv_heads;
+  const size_t codes = static_cast<size_t>(m.tot_pad) * c.kv_heads * c.head_dim * sizeof(__half);
+  size_t at = up256(std::max(static_cast<size_t>(num_sms) * 2 * kManyRows * (c.head_dim + 2) * sizeof(float),
+                             few_workspace(c, b, group, num_sms)));
+  m.k16 = at, at = up256(at + codes);
+  m.v16 = at, at = up256(at + codes);
+  // one tile more: a unit without keys still reads the scales of one granule
+  m.scales = at, at = up256(at + (static_cast<size_t>(m.tot_pad) * c.kv_heads + kManyKeys) / 16 * sizeof(float2));
+  m.seq_off = at, at = up256(at + (static_cast<size_t>(b.sequences) + 1) * sizeof(int));
+  m.units = at, at = up256(at + static_cast<size_t>(m.max_units) * sizeof(int4));
+  m.cum = at, at = up256(at + (static_cast<size_t>(m.max_units) + 1) * sizeof(int64_t));
+  m.cta_unit = at, at = up256(at + static_cast<size_t>(num_sms) * sizeof(int));
+  m.count = at, at = up256(at + sizeof(int));
+  m.bytes = at;
+  return m;
+}
+
+bool tile_map(CUtensorMap* map, const __half* base, int64_t rows, int64_t cols, int box_rows) {
+  static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  if (!enc) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int HD>
+cudaError_t many_launch(const Kvq8AttnParams& a, const ManyLayout& w, uint8_t* ws, int num_sms, int* err, cudaStream_t st) {
+  constexpr int PL = sizeof(T) == 4 ? 2 : 1;
+  using Sh = ManyShape<HD, PL>;
+  static bool ready = false;
+  cudaError_t e = allow_smem(kvq8_many_kernel<HD, PL>, Sh::kSmem, &ready);
+  if (e != cudaSuccess) return e;
+  Kvq8ManyParams p;
+  p.a = a;
+  p.a.partial = reinterpret_cast<float*>(ws);
+  p.tot_pad = static_cast<int>(w.tot_pad);
+  p.max_units = static_cast<int>(w.max_units);
+  p.k16 = reinterpret_cast<__half*>(ws + w.k16);
+  p.v16 = reinterpret_cast<__half*>(ws + w.v16);
+  p.scales = reinterpret_cast<float2*>(ws + w.scales);
+  p.seq_off = reinterpret_cast<int*>(ws + w.seq_off);
+  p.units = reinterpret_cast<int4*>(ws + w.units);
+  p.cum = reinterpret_cast<int64_t*>(ws + w.cum);
+  p.cta_unit = reinterpret_cast<int*>(ws + w.cta_unit);
+  p.count = reinterpret_cast<int*>(ws + w.count);
+  p.ctas = num_sms;
+  p.err = err;
+  const int kvh = a.c.kv_heads;
+  CUtensorMap kmap, vmap;
+  if (!tile_map(&kmap, p.k16, static_cast<int64_t>(kvh) * w.tot_pad, HD, kManyKeys) ||
+      !tile_map(&vmap, p.v16, static_cast<int64_t>(kvh) * HD, w.tot_pad, HD))
+    return cudaErrorInvalidValue;
+  const dim3 tiles(static_cast<unsigned>(w.tot_pad / kManyKeys + 1), static_cast<unsigned>(kvh));
+  kvq8_gather_kernel<HD><<<tiles, kGatherThreads, 0, st>>>(p);
+  kvq8_many_kernel<HD, PL><<<num_sms, kManyThreads, Sh::kSmem, st>>>(kmap, vmap, p);
+  kvq8_many_merge<HD, PL><<<dim3(static_cast<unsigned>(w.max_units), kManyRows / 8), 256, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
 // -------------------------------------------------------------- host side
 
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -420,7 +507,15 @@ int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, cons
   KIB_ARG(elem_size(type), "kvq8_attention: type must be F32(0) or F16(1)");
   KIB_ARG(heads > 0 && heads <= 4096 && heads % static_cast<uint64_t>(c.kv_heads) == 0,
           "kvq8_attention: heads must be a multiple of kv_heads, at most 4096");
-  *bytes = few_workspace(c, b, static_cast<int>(heads) / c.kv_heads, ctx->num_sms);
+  KIB_ARG(static_cast<uint64_t>(b.rows) * heads < (1ull << 31), "kvq8_attention: rows times heads out of range");
+  const int group = static_cast<int>(heads) / c.kv_heads;
+  *bytes = few_workspace(c, b, group, ctx->num_sms);
+  if (any_many(b, group)) {
+    const ManyLayout m = many_layout(c, b, static_cast<int64_t>(batch->total_length), group, ctx->num_sms);
+    KIB_ARG(m.tot_pad * c.kv_heads < (1ll << 31) && m.max_units < (1ll << 27),
+            "kvq8_attention: total_length or rows too large for one call");
+    *bytes = m.bytes;
+  }
   return KIB_OK;
 }
 
@@ -447,13 +542,24 @@ int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8
   p.group = p.heads / p.c.kv_heads;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.partial = static_cast<float*>(workspace);
-  p.few_limit = 0x7fffffff;
-  cudaError_t e;
-#define CALL(T, HD)                                                                            \
-  e = few_wide(p.b, p.group) ? few_launch<T, HD, 2>(p, ctx->num_sms, op_stream(ctx, stream))   \
-                             : few_launch<T, HD, 1>(p, ctx->num_sms, op_stream(ctx, stream))
-  KVQ8_DISPATCH(type, p.c.head_dim, CALL);
+  const cudaStream_t st = op_stream(ctx, stream);
+  const bool many = any_many(p.b, p.group);
+  // one sequence of many rows needs one path; a mixed batch takes both, each its own sequences
+  p.few_limit = many ? (p.b.sequences == 1 ? 0 : kFewLimit) : 0x7fffffff;
+  cudaError_t e = cudaSuccess;
+  if (p.few_limit > 0) {
+#define CALL(T, HD)                                                                \
+  e = few_wide(p.b, p.group) ? few_launch<T, HD, 2>(p, ctx->num_sms, st)           \
+                             : few_launch<T, HD, 1>(p, ctx->num_sms, st)
+    KVQ8_DISPATCH(type, p.c.head_dim, CALL);
 #undef CALL
+  }
+  if (many && e == cudaSuccess) {
+    const ManyLayout m = many_layout(p.c, p.b, static_cast<int64_t>(batch->total_length), p.group, ctx->num_sms);
+#define CALL(T, HD) e = many_launch<T, HD>(p, m, static_cast<uint8_t*>(workspace), ctx->num_sms, ctx->d_err, st)
+    KVQ8_DISPATCH(type, p.c.head_dim, CALL);
+#undef CALL
+  }
   if (e != cudaSuccess) return check_cuda(ctx, e, "kvq8_attention");
   return finish(ctx, stream, "kvq8_attention");
 }
