@@ -240,7 +240,7 @@ bool any_many(const Kvq8Batch& b, int group) { return static_cast<int64_t>(b.max
 
 // The workspace of the many-row path, in this order behind the records.
 struct ManyLayout {
-  size_t partial, k16, v16, scales, seq_off, units, cum, cta_unit, count, bytes;
+  size_t k16, v16, scales, seq_off, units, cum, cta_unit, split, count, bytes;
   int64_t tot_pad, max_units;
 };
 size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -261,7 +261,8 @@ ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_len
   m.units = at, at = up256(at + static_cast<size_t>(m.max_units) * sizeof(int4));
   m.cum = at, at = up256(at + (static_cast<size_t>(m.max_units) + 1) * sizeof(int64_t));
   m.cta_unit = at, at = up256(at + static_cast<size_t>(num_sms) * sizeof(int));
-  m.count = at, at = up256(at + sizeof(int));
+  m.split = at, at = up256(at + static_cast<size_t>(num_sms) * sizeof(int4));
+  m.count = at, at = up256(at + 2 * sizeof(int));
   m.bytes = at;
   return m;
 }
@@ -304,6 +305,7 @@ cudaError_t many_launch(const Kvq8AttnParams& a, const ManyLayout& w, uint8_t* w
   p.units = reinterpret_cast<int4*>(ws + w.units);
   p.cum = reinterpret_cast<int64_t*>(ws + w.cum);
   p.cta_unit = reinterpret_cast<int*>(ws + w.cta_unit);
+  p.split = reinterpret_cast<int4*>(ws + w.split);
   p.count = reinterpret_cast<int*>(ws + w.count);
   p.ctas = num_sms;
   p.err = err;
@@ -315,8 +317,9 @@ cudaError_t many_launch(const Kvq8AttnParams& a, const ManyLayout& w, uint8_t* w
   const dim3 tiles(static_cast<unsigned>(w.tot_pad / kManyKeys + 1), static_cast<unsigned>(kvh));
   kvq8_gather_kernel<HD><<<tiles, kGatherThreads, 0, st>>>(p);
   kvq8_many_kernel<HD, PL><<<num_sms, kManyThreads, Sh::kSmem, st>>>(kmap, vmap, p);
-  kvq8_many_merge<HD, PL><<<dim3(static_cast<unsigned>(w.max_units), kManyRows / 8), 256, 0, st>>>(p);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kvq8_many_merge<HD, PL>, dim3(static_cast<unsigned>(num_sms), kManyRows / 8), dim3(256), 0, st, p);
 }
 
 // -------------------------------------------------------------- host side

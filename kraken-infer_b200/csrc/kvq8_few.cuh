@@ -501,7 +501,12 @@ __global__ void __launch_bounds__(HD) kvq8_merge_kernel(const __grid_constant__ 
   const FewSeq fs = few_seq<NT>(p, seq);
   const Kvq8Seq sq = kvq8_seq(p.b, seq);
   const int64_t row = static_cast<int64_t>(rg) * RG + r;
-  if (rg >= fs.groups || row >= static_cast<int64_t>(sq.n) * p.group) return;
+  // every CTA waits before it leaves: a grid that ends early would let the
+  // stream's next kernel run beside the one before this
+  if (rg >= fs.groups || row >= static_cast<int64_t>(sq.n) * p.group) {
+    pdl_wait();
+    return;
+  }
   int64_t before = 0, total = 0;
   for (int s = tid; s < p.b.sequences; s += HD) {
     const FewSeq f = few_seq<NT>(p, s);
@@ -529,12 +534,12 @@ __global__ void __launch_bounds__(HD) kvq8_merge_kernel(const __grid_constant__ 
     return static_cast<int>(i);
   };
   const int c0 = owner(lo), n = owner(hi - 1) - c0 + 1;
+  pdl_wait();
   if (n == 1) return;
   // a CTA's first run is its record 0: the unit's, but where the unit begins inside the CTA
   constexpr int64_t REC = few_partial_floats<HD, NT>();
   const float* rec0 = p.partial + static_cast<int64_t>(c0) * 2 * REC;
   const float* rec_first = rec0 + (total * c0 / ctas < lo ? REC : 0);
-  pdl_wait();
   float top = -INFINITY;
   for (int i = tid; i < n; i += HD) {
     const float m = (i ? rec0 + 2 * REC * i : rec_first)[RG * HD + 2 * r];

@@ -42,6 +42,13 @@ constexpr int kManyKeys = 128;   // keys of a granule
 constexpr int kManySoft = 256;   // softmax threads
 constexpr int kManyThreads = kManySoft + 64;
 
+// A unit costs about as much as this many granules besides its own (q in, the
+// pipeline filled and drained, O out), so runs are cut by granules plus this:
+// without it the CTA at the start of a prompt, where a unit sees one to three
+// tiles of keys, takes 26 units where others take 3 (prompts of up to 3001
+// tokens).
+constexpr int kManyUnitCost = 4;
+
 struct Kvq8ManyParams {
   Kvq8AttnParams a;
   int tot_pad;      // padded keys that the workspace holds
@@ -51,9 +58,10 @@ struct Kvq8ManyParams {
   float2* scales;   // [kv_heads][tot_pad / 16]: k and v scale; v < 0: an absent page
   int* seq_off;     // [sequences + 1] first padded key
   int4* units;      // [max_units] sequence, row tile, head, granules
-  int64_t* cum;     // [max_units + 1] running granules; cum[count[0]] is the total
-  int* cta_unit;    // [ctas] unit of a CTA's first granule
-  int* count;       // [1] units
+  int64_t* cum;     // [max_units + 1] running cost; cum[count[0]] is the total
+  int* cta_unit;    // [ctas] unit at which a CTA begins
+  int4* split;      // [ctas] units that cross CTAs: unit, first CTA, CTAs, whether its first record is a CTA's second
+  int* count;       // [2] units, split units
   int ctas;
   int* err;
 };
@@ -142,7 +150,7 @@ __global__ void __launch_bounds__(kGatherThreads) kvq8_gather_kernel(const __gri
       units += all;
     }
     units = min(units, p.max_units);
-    if (tid == 0) s_off[S] = units, p.count[0] = units;
+    if (tid == 0) s_off[S] = units, p.count[0] = units, p.count[1] = 0;
     __syncthreads();
     int64_t total = 0;
     for (int u0 = 0; u0 < units; u0 += kGatherThreads) {
@@ -164,7 +172,7 @@ __global__ void __launch_bounds__(kGatherThreads) kvq8_gather_kernel(const __gri
         const int end = min(min(m.span, room), q.length - q.n + static_cast<int>(last / p.a.group) + 1);
         const int g = max(1, (end + kManyKeys - 1) / kManyKeys);
         p.units[u] = make_int4(lo, tile, h, g);
-        v = g;
+        v = g + kManyUnitCost;
       }
       int64_t all;
       const int64_t x = total + many_scan(v, s_scan, &all);
@@ -178,6 +186,15 @@ __global__ void __launch_bounds__(kGatherThreads) kvq8_gather_kernel(const __gri
       const int64_t c0 = p.cum[u], c1 = p.cum[u + 1];
       for (int64_t i = (c0 * ctas + total - 1) / total; i < ctas && total * i / ctas < c1; ++i)
         if (total * i / ctas >= c0) p.cta_unit[i] = u;
+      // CTA i holds [total * i / ctas, total * (i + 1) / ctas): the one of position x
+      auto owner = [&](int64_t x) {
+        int64_t i = x * ctas / total;
+        while (total * (i + 1) / ctas <= x) ++i;
+        while (total * i / ctas > x) --i;
+        return static_cast<int>(i);
+      };
+      const int a = owner(c0 + kManyUnitCost), n = owner(c1 - 1) - a + 1;
+      if (n > 1) p.split[atomicAdd(p.count + 1, 1)] = make_int4(u, a, n, total * a / ctas < c0 ? 1 : 0);
     }
     return;
   }
@@ -326,7 +343,7 @@ KIB_DEV bool soft_any(bool x) {
 }
 
 struct ManyShared {
-  uint64_t full[8], empty[8], s_full[2], p_full[2], o_done, q_full;
+  uint64_t full[8], empty[8], s_full[2], p_full[2], o_done[2], q_full;
   float qs[kManyRows];        // what takes a row's scores back from its power of two, times scale_log2
   float x[2][2][kManyRows];   // row maxima of the two halves, by tile parity
   float red[8];
@@ -360,7 +377,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   uint8_t* s_st = many_raw + Sh::kQ;
   ManyShared& sh = *reinterpret_cast<ManyShared*>(s_st + Sh::kStages * Sh::kStage);
   uint64_t *full = sh.full, *empty = sh.empty, *s_full = sh.s_full, *p_full = sh.p_full;
-  uint64_t &o_done = sh.o_done, &q_full = sh.q_full;
+  // like the S buffers, the products' barriers alternate: at the end of a run two of them may still be running
+  uint64_t *o_done = sh.o_done, &q_full = sh.q_full;
   float* s_qs = sh.qs;
   float* s_red = sh.red;
   if (smem_u32(many_raw) & 1023u) {
@@ -377,8 +395,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < Sh::kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-    for (int b = 0; b < 2; ++b) mbar_init(&s_full[b], 1), mbar_init(&p_full[b], 8);
-    mbar_init(&o_done, 1);
+    for (int b = 0; b < 2; ++b) mbar_init(&s_full[b], 1), mbar_init(&p_full[b], 8), mbar_init(&o_done[b], 1);
     mbar_init(&q_full, 8);
     fence_mbar_init();
   }
@@ -394,15 +411,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   // every role walks the same runs: granules [g0, g1) of a unit
   struct Run {
-    int seq, tile, head, granules, g0, g1;
+    int seq, tile, head, g0, g1;
     bool whole;
-    int64_t begin;
+    int64_t begin, next;
   };
   auto run_at = [&](int unit, int64_t at) {
     const int4 u = p.units[unit];
-    Run r{u.x, u.y, u.z, u.w, 0, 0, false, at};
-    r.g0 = static_cast<int>(at - p.cum[unit]);
-    r.g1 = static_cast<int>(min(static_cast<int64_t>(u.w), r.g0 + (stop - at)));
+    const int64_t c0 = p.cum[unit] + kManyUnitCost, c1 = c0 + u.w;
+    Run r{u.x, u.y, u.z, 0, 0, false, at, min(c1, stop)};
+    r.g0 = static_cast<int>(max(at - c0, static_cast<int64_t>(0)));
+    r.g1 = static_cast<int>(max(r.next - c0, static_cast<int64_t>(0)));
     r.whole = r.g0 == 0 && r.g1 == u.w;
     return r;
   };
@@ -437,13 +455,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       int unit = unit0;
       for (int64_t at = first; at < stop && ok; ++unit) {
         const Run r = run_at(unit, at);
+        at = r.next;
+        if (r.g0 == r.g1) continue;
         const int off = p.seq_off[r.seq];
         for (int j = r.g0; j < r.g1 && ok; ++j) {
           load(&kmap, true, r.head, off + j * kManyKeys);
           if (j > r.g0) load(&vmap, false, r.head, off + (j - 1) * kManyKeys);
         }
         if (ok) load(&vmap, false, r.head, off + (r.g1 - 1) * kManyKeys);
-        at += r.g1 - r.g0;
       }
     }
   } else if (warp == 9) {
@@ -494,12 +513,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
           umma_commit(&empty[s]);
         }
-        umma_commit(&o_done);
+        umma_commit(&o_done[jj & 1]);
       };
       int unit = unit0;
-      for (int64_t at = first; at < stop && ok; ++unit, ++piece) {
+      for (int64_t at = first; at < stop && ok; ++unit) {
         const Run r = run_at(unit, at);
-        ok = tc_wait(&q_full, piece & 1, p.err);
+        at = r.next;
+        if (r.g0 == r.g1) continue;
+        ok = tc_wait(&q_full, piece++ & 1, p.err);
         tc_fence_after();
         const int n = r.g1 - r.g0;
         for (int j = 0; j < n && ok; ++j) {
@@ -508,7 +529,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         if (ok) outputs(jg + n - 1, n == 1);
         jg += n;
-        at += n;
       }
     }
   } else if (warp < 8) {
@@ -519,7 +539,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     int unit = unit0;
     for (int64_t at = first; at < stop; ++unit) {
       const Run r = run_at(unit, at);
-      at += r.g1 - r.g0;
+      at = r.next;
+      if (r.g0 == r.g1) continue;
       const Kvq8Seq sq = kvq8_seq(p.a.b, r.seq);
       const ManySeq ms = many_seq(p.a, r.seq);
       const int off = p.seq_off[r.seq];
@@ -532,7 +553,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const float2* scales = p.scales + (static_cast<int64_t>(r.head) * p.tot_pad + off) / 16;
 
       // q rows to shared memory as halves, in the swizzled layout of the MMA
-#pragma unroll 2
+#pragma unroll 4
       for (int i = warp; i < kManyRows; i += 8) {
         constexpr int V = HD / 32;
         float x[V];
@@ -640,7 +661,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           l *= f;
           if (j > 0) {
             // S(j) was issued after the product before last, so only the last one may still run
-            ok = warp_ok(ok && tc_wait(&o_done, (jj - 1) & 1, p.err));
+            ok = warp_ok(ok && tc_wait(&o_done[(jj - 1) & 1], ((jj - 1) >> 1) & 1, p.err));
             tc_fence_after();
             if (ok) {
 #pragma unroll 1
@@ -691,7 +712,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       jg += n;
 
       // the unit's or the run's end: O / l, or a record
-      ok = warp_ok(ok && tc_wait(&o_done, (jg - 1) & 1, p.err));
+      ok = warp_ok(ok && tc_wait(&o_done[(jg - 1) & 1], ((jg - 1) >> 1) & 1, p.err));
       tc_fence_after();
       float* s_l = reinterpret_cast<float*>(s_q);  // q has been read by every product of the run
       s_l[half * kManyRows + row] = l;
@@ -736,37 +757,31 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 }
 
 // Joins the records of the units that cross CTAs, in CTA order: a CTA per
-// unit and 8 rows, a warp per row.
+// such unit and 8 rows, a warp per row.
 template <int HD, int PL>
 __global__ void __launch_bounds__(256) kvq8_many_merge(const __grid_constant__ Kvq8ManyParams p) {
   using T = typename std::conditional<PL == 2, float, __half>::type;
   constexpr int64_t REC = ManyShape<HD, PL>::kPartial;
-  const int unit = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 8 + warp;
-  const int units = p.count[0];
-  if (unit >= units) return;
-  const int4 u = p.units[unit];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 8 + warp;
+  pdl_wait();
+  if (static_cast<int>(blockIdx.x) >= p.count[1]) return;
+  const int4 sp = p.split[blockIdx.x], u = p.units[sp.x];
   const Kvq8Seq sq = kvq8_seq(p.a.b, u.x);
-  const int64_t rr = static_cast<int64_t>(u.y) * kManyRows + row;
-  if (rr >= static_cast<int64_t>(sq.n) * p.a.group) return;
-  const int64_t total = p.cum[units], ctas = few_ctas(total, p.ctas), lo = p.cum[unit], hi = lo + u.w;
-  auto owner = [&](int64_t x) {
-    int64_t i = x * ctas / total;
-    while (total * (i + 1) / ctas <= x) ++i;
-    while (total * i / ctas > x) --i;
-    return static_cast<int>(i);
-  };
-  const int c0 = owner(lo), n = owner(hi - 1) - c0 + 1;
-  if (n == 1) return;
-  const float* rec0 = p.a.partial + static_cast<int64_t>(c0) * 2 * REC;
-  const float* rec_first = rec0 + (total * c0 / ctas < lo ? REC : 0);
+  const int rr = u.y * kManyRows + row, n = sp.z;
+  if (rr >= sq.n * p.a.group) return;
+  const float* rec0 = p.a.partial + static_cast<int64_t>(sp.y) * 2 * REC;
+  const float* rec_first = rec0 + (sp.w ? REC : 0);
   float top = -INFINITY;
-  for (int i = 0; i < n; ++i) top = fmaxf(top, (i ? rec0 + 2 * REC * i : rec_first)[kManyRows * HD + 2 * row]);
+  for (int i = lane; i < n; i += 32) top = fmaxf(top, (i ? rec0 + 2 * REC * i : rec_first)[kManyRows * HD + 2 * row]);
+  top = warp_max(top);
   constexpr int V = HD / 32;
   float acc[V] = {}, sum = 0.0f;
+#pragma unroll 4
   for (int i = 0; i < n; ++i) {
     const float* rec = i ? rec0 + 2 * REC * i : rec_first;
-    const float m = rec[kManyRows * HD + 2 * row], f = m == -INFINITY ? 0.0f : ex2(m - top);
-    sum += f * rec[kManyRows * HD + 2 * row + 1];
+    const float2 ml = *reinterpret_cast<const float2*>(rec + kManyRows * HD + 2 * row);
+    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+    sum += f * ml.y;
     float x[V];
     load_vec<float, V>(rec + row * HD + lane * V, x);
 #pragma unroll
@@ -775,7 +790,7 @@ __global__ void __launch_bounds__(256) kvq8_many_merge(const __grid_constant__ K
   const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] *= inv;
-  store_vec<T, V>(static_cast<T*>(p.a.out) + (sq.first + rr / p.a.group) * p.a.out_stride +
+  store_vec<T, V>(static_cast<T*>(p.a.out) + static_cast<int64_t>(sq.first + rr / p.a.group) * p.a.out_stride +
                       (static_cast<int64_t>(u.z) * p.a.group + rr % p.a.group) * HD + lane * V,
                   acc);
 }
