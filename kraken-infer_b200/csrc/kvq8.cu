@@ -211,27 +211,82 @@ cudaError_t allow_smem(void (*kernel)(KArgs...), size_t bytes, bool* done) {
   return e;
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return enc;
+}
+
+// [rows][cols] halves in boxes of box_rows x 64, 128-byte swizzle.
+bool tile_map(CUtensorMap* map, const __half* base, int64_t rows, int64_t cols, int box_rows) {
+  const auto enc = map_encoder();
+  if (!enc) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The cache's codes [page][head][token][d] in boxes of 16 tokens x 128 (64)
+// dimensions, swizzled by the box's width.
+bool codes_map(CUtensorMap* map, const int8_t* base, const Kvq8Cache& c) {
+  const auto enc = map_encoder();
+  if (!enc) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_tokens),
+                              static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.pages)};
+  // a stride over one element is never taken, but has to be a legal one
+  auto stride = [](int64_t s, bool one) { return static_cast<cuuint64_t>(one && s == 0 ? 16 : s); };
+  const cuuint64_t strides[3] = {stride(c.token_stride, false), stride(c.head_stride, c.kv_heads == 1),
+                                 stride(c.page_stride, c.pages == 1)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(std::min(c.head_dim, 128)), 16, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, c.head_dim >= 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int HD, int NT>
 cudaError_t few_launch(const Kvq8AttnParams& p, int num_sms, cudaStream_t st) {
   static bool ready = false;
   cudaError_t e = allow_smem(kvq8_few_kernel<T, HD, NT>, few_smem<T, HD, NT>(), &ready);
   if (e != cudaSuccess) return e;
-  const int ctas = std::min(num_sms * few_ctas_per_sm<HD>(), kMergeMaxCtas);
-  kvq8_few_kernel<T, HD, NT><<<ctas, kFewWarps * 32, few_smem<T, HD, NT>(), st>>>(p);
+  const int ctas = std::min(num_sms, kMergeMaxCtas);
+  CUtensorMap kmap, vmap;
+  if (!codes_map(&kmap, p.c.k, p.c) || !codes_map(&vmap, p.c.v, p.c)) return cudaErrorInvalidValue;
+  kvq8_few_kernel<T, HD, NT><<<ctas, few_warps<HD, NT>() * 32, few_smem<T, HD, NT>(), st>>>(kmap, vmap, p);
   const int64_t rows = std::min<int64_t>(static_cast<int64_t>(p.b.max_rows) * p.group, p.few_limit);
   const int groups = static_cast<int>((rows + 8 * NT - 1) / (8 * NT));
   const dim3 grid(static_cast<unsigned>(p.b.sequences) * p.c.kv_heads * groups, static_cast<unsigned>(std::min<int64_t>(rows, 8 * NT)));
   return launch_pdl(kvq8_merge_kernel<T, HD, NT>, grid, dim3(HD), 0, st, p, ctas, groups);
 }
 
-// Units of 8 rows while they hold all of a sequence's rows, else of 16: the
-// cache is read once per unit.
-bool few_wide(const Kvq8Batch& b, int group) { return static_cast<int64_t>(b.max_rows) * group > 8; }
+// Eighths of a unit's rows: the fewest that hold all of a sequence's rows, as
+// the cache is read once per unit; the most there are beyond that.
+int few_nt(const Kvq8Cache& c, const Kvq8Batch& b, int group) {
+  return static_cast<int>(std::min<int64_t>((static_cast<int64_t>(b.max_rows) * group + 7) / 8, few_max_nt(c.head_dim)));
+}
+template <typename T, int HD>
+cudaError_t few_launch_nt(const Kvq8AttnParams& p, int num_sms, cudaStream_t st) {
+  const int nt = few_nt(p.c, p.b, p.group);
+  if (nt == 1) return few_launch<T, HD, 1>(p, num_sms, st);
+  if constexpr (few_max_nt(HD) > 2) {
+    if (nt == 3) return few_launch<T, HD, 3>(p, num_sms, st);
+  }
+  return few_launch<T, HD, 2>(p, num_sms, st);
+}
 
 size_t few_workspace(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_sms) {
-  const size_t rows = few_wide(b, group) ? 16 : 8;
-  const size_t ctas = std::min(num_sms * (c.head_dim == 256 ? 1 : c.head_dim == 128 ? 2 : 3), kMergeMaxCtas);
-  return ctas * 2 * rows * static_cast<size_t>(c.head_dim + 2) * sizeof(float);
+  return static_cast<size_t>(std::min(num_sms, kMergeMaxCtas)) * 2 * 8 * few_nt(c, b, group) *
+         static_cast<size_t>(c.head_dim + 2) * sizeof(float);
 }
 
 // Rows (times the group) up to which a sequence is the few-row kernel's.
@@ -265,25 +320,6 @@ ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_len
   m.count = at, at = up256(at + 2 * sizeof(int));
   m.bytes = at;
   return m;
-}
-
-bool tile_map(CUtensorMap* map, const __half* base, int64_t rows, int64_t cols, int box_rows) {
-  static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  }();
-  if (!enc) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
-  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t estr[2] = {1, 1};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half*>(base), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int HD>
@@ -545,15 +581,14 @@ int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8
   p.group = p.heads / p.c.kv_heads;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.partial = static_cast<float*>(workspace);
+  p.err = ctx->d_err;
   const cudaStream_t st = op_stream(ctx, stream);
   const bool many = any_many(p.b, p.group);
   // one sequence of many rows needs one path; a mixed batch takes both, each its own sequences
   p.few_limit = many ? (p.b.sequences == 1 ? 0 : kFewLimit) : 0x7fffffff;
   cudaError_t e = cudaSuccess;
   if (p.few_limit > 0) {
-#define CALL(T, HD)                                                                \
-  e = few_wide(p.b, p.group) ? few_launch<T, HD, 2>(p, ctx->num_sms, st)           \
-                             : few_launch<T, HD, 1>(p, ctx->num_sms, st)
+#define CALL(T, HD) e = few_launch_nt<T, HD>(p, ctx->num_sms, st)
     KVQ8_DISPATCH(type, p.c.head_dim, CALL);
 #undef CALL
   }

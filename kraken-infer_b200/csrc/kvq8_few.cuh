@@ -15,26 +15,44 @@
 // of the grid's CTAs takes an equal run of them, whatever the lengths are, so
 // the kernel needs no host knowledge of the lengths.  A unit that crosses
 // CTAs leaves partial (m, l, O) records, which kvq8_merge_kernel joins in
-// order: the result depends on no timing.  Within a CTA, eight warps take
+// order: the result depends on no timing.  Within a CTA, the warps take
 // 16-key tiles in turn, each with its own m, l and O, and join in shared
 // memory at the end of the unit's run.
 //
-// Bound by HBM: 2 bytes per key, head and dimension.  K rows are loaded so
-// that a lane's 16 bytes are the A fragments of four mma k-steps (the
-// dimensions of a dot product may be taken in any order, and q is laid out
-// the same way); V rows so that two byte permutes transpose 4 keys x 2
-// dimensions into a fragment.  No shared memory and no barrier between the
-// loads and the tensor cores: a warp has the next K rows in flight while it
-// works on V, and V rows while it works on K.
+// Bound by HBM: 2 bytes per key, head and dimension, and next by the
+// instructions that unpack them.  Every warp has a ring of tiles of its own in
+// shared memory that one of its lanes refills by tensor-map TMA over the
+// cache's own layout (any strides): a K or V piece is asked for as soon as its
+// predecessor has been read, so no register and no other warp waits for a
+// load; the pages and scales of the warp's next 32 tiles sit in its lanes.
+// (One producer warp serving all others, a lane each, kept up with 4.4 TB/s
+// only: its TMA instructions issue one lane after another.)  The 128-byte
+// swizzle keeps both fragment reads free of bank conflicts: a lane's 16 bytes
+// of a K row are the A fragments of four mma k-steps (the dimensions of a dot
+// product may be taken in any order, and q is laid out the same way); of V,
+// two byte permutes transpose 4 keys x 2 dimensions into a fragment.
 #pragma once
 
+#include "gemm_tc.cuh"
 #include "kvq8.cuh"
 
 namespace kib {
 
 constexpr int kFewGranule = 128;
-constexpr int kFewWarps = 8;
 constexpr int kFewMaxSeqs = 4096;
+
+// Warps of a CTA (one CTA per SM), by what the accumulators (head_dim / 16 x
+// NT x 4 registers a lane) leave.
+template <int HD, int NT>
+constexpr int few_warps() { return HD / 16 * NT * 4 > 96 ? 8 : 12; }
+// Tiles (16 rows of K and of V) in a warp's ring, within 192 KB for all warps.
+template <int HD, int NT>
+constexpr int few_ring() {
+  constexpr int n = 196608 / (few_warps<HD, NT>() * 32 * HD);
+  return n < 4 ? n : 4;
+}
+// Groups of 8 rows a unit may have.
+__host__ __device__ constexpr int few_max_nt(int hd) { return hd == 256 ? 2 : 3; }
 
 struct Kvq8AttnParams {
   Kvq8Cache c;
@@ -46,6 +64,7 @@ struct Kvq8AttnParams {
   float scale_log2;  // softmax scale times log2(e)
   float* partial;    // [ctas][2][rows of a unit][head_dim + 2]
   int few_limit;     // sequences of at most this many rows * group are this kernel's
+  int* err;
 };
 
 KIB_DEV float ex2(float x) {
@@ -83,6 +102,21 @@ KIB_DEV uint4 ldg_stream(const int8_t* p) {
   return v;
 }
 
+KIB_DEV void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// store_vec where a lane may hold a single value.
+template <typename T, int V>
+KIB_DEV void store_any(T* p, const float (&x)[V]) {
+  if constexpr (V * sizeof(T) >= 4) store_vec<T, V>(p, x);
+  else p[0] = from_f32<T>(x[0]);
+}
+
 // Granules of one unit of a sequence, and its units per KV head.
 struct FewSeq {
   int granules, groups;
@@ -104,102 +138,177 @@ KIB_DEV int64_t few_ctas(int64_t total, int64_t grid) { return total < grid ? to
 
 template <int HD, int NT>
 constexpr int few_partial_floats() { return 8 * NT * (HD + 2); }
-template <int HD>
-constexpr int few_ctas_per_sm() { return HD == 256 ? 1 : (HD == 128 ? 2 : 3); }
 template <typename T, int HD, int NT>
 constexpr size_t few_smem() {
-  constexpr int planes = sizeof(T) == 4 ? 2 : 1;
-  return static_cast<size_t>(8 * NT) * planes * (HD * 2 + 16) + static_cast<size_t>(kFewWarps) * 8 * NT * (HD + 4) * 4;
+  constexpr int planes = sizeof(T) == 4 ? 2 : 1, warps = few_warps<HD, NT>();
+  constexpr size_t ring = static_cast<size_t>(warps) * few_ring<HD, NT>() * 32 * HD;
+  constexpr size_t join = static_cast<size_t>(warps) * 8 * NT * (HD + 4) * 4;
+  return (ring > join ? ring : join) + static_cast<size_t>(8 * NT) * planes * (HD * 2 + 16);
 }
 
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(kFewWarps * 32, few_ctas_per_sm<HD>())
-    kvq8_few_kernel(const __grid_constant__ Kvq8AttnParams p) {
+__global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
+    kvq8_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                    const __grid_constant__ Kvq8AttnParams p) {
   constexpr int RG = 8 * NT;                      // rows of a unit
   constexpr int PL = sizeof(T) == 4 ? 2 : 1;      // half planes of q and p
   constexpr int QB = HD * 2 + 16;                 // bytes of a q row: conflict-free 16-byte reads
   constexpr int OF = HD + 4;                      // floats of an O row in shared memory
-  constexpr int KL = HD / 64, VL = HD / 128 > 0 ? HD / 128 : 1;
-  extern __shared__ __align__(16) uint8_t few_raw[];
-  uint8_t* s_q = few_raw;                                           // [PL][RG][QB]
-  float* s_o = reinterpret_cast<float*>(few_raw + PL * RG * QB);    // [warps][RG][OF]
-  __shared__ int64_t s_cum[kFewMaxSeqs + 1];
-  __shared__ int64_t s_warp[kFewWarps];
-  __shared__ float s_qs[RG], s_m[kFewWarps][RG], s_l[kFewWarps][RG];
+  constexpr int W = few_warps<HD, NT>(), D = few_ring<HD, NT>(), PIECE = 16 * HD;
+  constexpr size_t RING = static_cast<size_t>(W) * D * 2 * PIECE, JOIN = static_cast<size_t>(W) * RG * OF * 4;
+  extern __shared__ __align__(1024) uint8_t few_raw[];
+  float* s_o = reinterpret_cast<float*>(few_raw);                   // [W][RG][OF], in the ring's place once it is empty
+  uint8_t* s_q = few_raw + (RING > JOIN ? RING : JOIN);             // [PL][RG][QB]
+  __shared__ uint64_t s_bar[W][D][2];                               // K and V of a ring slot have arrived
+  __shared__ int64_t s_warp[W], s_at;
+  __shared__ int s_seq;
+  __shared__ float s_qs[RG], s_m[W][RG], s_l[W][RG];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int S = p.b.sequences, kvh = p.c.kv_heads;
+  if (lane < 2 * D) mbar_init(&s_bar[warp][lane >> 1][lane & 1], 1);
+  fence_mbar_init();
+  if (tid == 0) tma_prefetch_desc(&kmap), tma_prefetch_desc(&vmap);
 
-  // running granule totals of the sequences
-  int64_t base = 0;
-  for (int s0 = 0; s0 < S; s0 += kFewWarps * 32) {
-    const int s = s0 + tid;
-    int64_t v = 0;
-    if (s < S) {
-      const FewSeq f = few_seq<NT>(p, s);
-      v = static_cast<int64_t>(f.granules) * f.groups * kvh;
-    }
+  // granules of all sequences; then the sequence in which this CTA's run begins
+  constexpr int TH = W * 32;
+  auto seq_cost = [&](int s) -> int64_t {
+    if (s >= S) return 0;
+    const FewSeq f = few_seq<NT>(p, s);
+    return static_cast<int64_t>(f.granules) * f.groups * kvh;
+  };
+  auto scan = [&](int64_t v, int64_t* all) {
     int64_t inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t n = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += n;
     }
+    __syncthreads();
     if (lane == 31) s_warp[warp] = inc;
     __syncthreads();
-    int64_t before = base;
-    for (int w = 0; w < kFewWarps; ++w) {
+    int64_t before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
       if (w < warp) before += s_warp[w];
-      base += s_warp[w];
+      sum += s_warp[w];
     }
-    if (s < S) s_cum[s] = before + inc - v;
-    __syncthreads();
+    *all = sum;
+    return before + inc - v;
+  };
+  const int64_t cost0 = seq_cost(tid);
+  int64_t all0;
+  const int64_t x0 = scan(cost0, &all0);
+  int64_t total = all0;
+  for (int s0 = TH; s0 < S; s0 += TH) {
+    int64_t all;
+    scan(seq_cost(s0 + tid), &all);
+    total += all;
   }
-  if (tid == 0) s_cum[S] = base;
-  __syncthreads();
-  const int64_t total = base;
   const int64_t ctas = few_ctas(total, gridDim.x);
   if (blockIdx.x >= ctas) return;
   int64_t at = total * blockIdx.x / ctas;
-  const int64_t stop = total * (blockIdx.x + 1) / ctas;
-  const int64_t first = at;
-  int seq;
-  {
-    int lo = 0, hi = S;  // the last sequence that begins at or before `at`
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_cum[mid] <= at) lo = mid;
-      else hi = mid;
-    }
-    seq = lo;
+  const int64_t stop = total * (blockIdx.x + 1) / ctas, first = at;
+  if (x0 <= at && at < x0 + cost0) s_seq = tid, s_at = x0;
+  int64_t base = all0;
+  for (int s0 = TH; s0 < S && base <= at; s0 += TH) {
+    int64_t all;
+    const int64_t v = seq_cost(s0 + tid), x = base + scan(v, &all);
+    if (x <= at && at < x + v) s_seq = s0 + tid, s_at = x;
+    base += all;
   }
+  __syncthreads();
+  int seq = s_seq;
+  int64_t seq_at = s_at;  // granules before the sequence
 
-  while (at < stop) {
-    while (s_cum[seq + 1] <= at) ++seq;
-    const Kvq8Seq sq = kvq8_seq(p.b, seq);
-    const FewSeq fs = few_seq<NT>(p, seq);
-    const int64_t rel = at - s_cum[seq];
-    const int unit = static_cast<int>(rel / fs.granules), gran0 = static_cast<int>(rel % fs.granules);
-    const int head = unit % kvh, rg = unit / kvh;
+  // the run of granules [gran0, gran1) of a unit that begins at `at`
+  struct Run {
+    Kvq8Seq sq;
+    int head, row0, live, key0, key1;
+    bool whole;
+  };
+  auto next_run = [&]() {
+    Run r;
+    r.sq = kvq8_seq(p.b, seq);
+    FewSeq fs = few_seq<NT>(p, seq);
+    while (at >= seq_at + static_cast<int64_t>(fs.granules) * fs.groups * kvh) {
+      seq_at += static_cast<int64_t>(fs.granules) * fs.groups * kvh;
+      ++seq;
+      r.sq = kvq8_seq(p.b, seq);
+      fs = few_seq<NT>(p, seq);
+    }
+    const int64_t rel = at - seq_at;
+    const int unit = static_cast<int>(rel / fs.granules), gran0 = static_cast<int>(rel - static_cast<int64_t>(unit) * fs.granules);
     const int gran1 = static_cast<int>(min(static_cast<int64_t>(fs.granules), gran0 + (stop - at)));
-    const int64_t begin = at;
+    r.head = unit % kvh;
+    r.row0 = unit / kvh * RG;
+    r.live = min(RG, r.sq.n * p.group - r.row0);
+    r.key0 = gran0 * kFewGranule;
+    const int span = max(0, min(r.sq.length, p.b.max_length));
+    r.key1 = min(min(span, gran1 * kFewGranule), r.sq.length - r.sq.n + (r.row0 + r.live - 1) / p.group + 1);
+    r.whole = gran0 == 0 && gran1 == fs.granules;
     at += gran1 - gran0;
-    const int64_t nrows = static_cast<int64_t>(sq.n) * p.group;
-    const int row0 = rg * RG, live = static_cast<int>(min(static_cast<int64_t>(RG), nrows - row0));
-    const int start = sq.length - sq.n;  // position of the first row
-    const int span = max(0, min(sq.length, p.b.max_length));
-    const int key0 = gran0 * kFewGranule;
-    const int key1 = min(min(span, gran1 * kFewGranule), start + (row0 + live - 1) / p.group + 1);
+    return r;
+  };
+
+  uint32_t slot_i = 0, slot = 0, phase = 0;  // ring slots: of the next tile to ask for, and to work on
+  bool ok = true;
+  uint8_t* ring = few_raw + static_cast<size_t>(warp) * D * 2 * PIECE;
+  while (at < stop) {
+    const int64_t begin = at;
+    const Run r = next_run();
+    const Kvq8Seq sq = r.sq;
+    const int head = r.head, row0 = r.row0, live = r.live, key1 = r.key1, start = sq.length - sq.n;
     const int all_see = start + row0 / p.group + 1;  // keys below it are seen by every row
 
+    // this warp's tiles: keys key0 + 16 (warp + W t); lane t % 32 holds tile t's page and scales
+    const int first_key = r.key0 + 16 * warp;
+    const int tiles = key1 > first_key ? (key1 - first_key - 1) / (16 * W) + 1 : 0;
+    auto lane_page = [&](int t0) {
+      const int t = t0 + lane;
+      return t < tiles ? kvq8_page(p.c, p.b, seq, (first_key + 16 * W * t) >> p.c.page_shift) : -1;
+    };
+    auto lane_scale = [&](const float* s, int page) { return page >= 0 ? __ldg(s + static_cast<int64_t>(page) * kvh + head) : 0.0f; };
+    int page_l = lane_page(0), page_n = lane_page(32), page_nn = -1;  // of this batch of 32 tiles, and the next
+    int ti = 0, batch = 0;       // the next tile to ask for; the first tile of the batch in the lanes
+    int page_i = -1, row_i = 0;  // the tile whose K was asked for last: its V follows
+    auto piece = [&](const CUtensorMap* map, int half) {
+      if (lane == 0) {
+        uint64_t* bar = &s_bar[warp][slot_i][half];
+        uint8_t* dst = ring + (slot_i * 2 + half) * PIECE;
+        mbar_arrive_expect_tx(bar, PIECE);
+#pragma unroll
+        for (int i = 0; i < (HD + 127) / 128; ++i) tma_load_4d(dst + 2048 * i, map, 128 * i, row_i, head, page_i, bar);
+      }
+    };
+    auto ask_k = [&]() {
+      const int lim = min(tiles, batch + 64);
+      page_i = -1;
+      for (; ti < lim; ++ti) {
+        page_i = __shfl_sync(0xffffffffu, ti < batch + 32 ? page_l : page_n, ti & 31);
+        if (page_i >= 0) break;
+      }
+      if (page_i < 0) return;
+      row_i = (first_key + 16 * W * ti) & (p.c.page_tokens - 1);
+      piece(&kmap, 0);
+      ++ti;
+    };
+    auto ask_v = [&]() {
+      if (page_i < 0) return;
+      piece(&vmap, 1);
+      slot_i = slot_i + 1 == D ? 0 : slot_i + 1;
+    };
+#pragma unroll 1
+    for (int i = 0; i < D; ++i) ask_k(), ask_v();
+    float ks_l = lane_scale(p.c.k_scale, page_l), vs_l = lane_scale(p.c.v_scale, page_l), ks_n = 0.0f, vs_n = 0.0f;
+
     // q rows to shared memory, as halves (fp32 rows scaled to about 2^13 by a power of two first)
-    __syncthreads();
-    for (int r = warp; r < RG; r += kFewWarps) {
+    for (int rr = warp; rr < RG; rr += W) {
       constexpr int V = HD / 32;
       float x[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) x[e] = 0.0f;
-      if (r < live) {
-        const int row = row0 + r;
+      if (rr < live) {
+        const int row = row0 + rr;
         load_vec<T, V>(static_cast<const T*>(p.q) + static_cast<int64_t>(sq.first + row / p.group) * p.q_stride +
                            (static_cast<int64_t>(head) * p.group + row % p.group) * HD + lane * V,
                        x);
@@ -225,13 +334,16 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_ctas_per_sm<HD>())
         hi[e] = __float2half_rn(x[e]);
         lo[e] = __float2half_rn(x[e] - __half2float(hi[e]));
       }
-      uint8_t* dst = s_q + r * QB + lane * V * 2;
+      // 16 dimensions of chunk 2 c + i of a 128-dimension slab go to place 4 i + c: lane c's k-steps
+      const int d = lane * V, ch = d % 128 / 16;
+      const int place = HD >= 128 ? d / 128 * 128 + ((ch & 1) * 4 + (ch >> 1)) * 16 + d % 16 : d;
+      uint8_t* dst = s_q + rr * QB + place * 2;
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
         *reinterpret_cast<__half2*>(dst + 2 * e) = __halves2half2(hi[e], hi[e + 1]);
         if constexpr (PL == 2) *reinterpret_cast<__half2*>(dst + RG * QB + 2 * e) = __halves2half2(lo[e], lo[e + 1]);
       }
-      if (lane == 0) s_qs[r] = back * p.scale_log2;
+      if (lane == 0) s_qs[rr] = back * p.scale_log2;
     }
     __syncthreads();
 
@@ -249,57 +361,46 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_ctas_per_sm<HD>())
       for (int e = 0; e < 2; ++e) m[j][e] = -INFINITY, l[j][e] = 0.0f, qs[j][e] = s_qs[8 * j + 2 * c + e];
     int vexp = 20;  // exponent field of the power of two that p is relative to
 
-    uint4 kr[KL][2], vr[VL][4];
-    float ks = 0.0f, vs = 0.0f, ks_n = 0.0f, vs_n = 0.0f;
-    const int kstep = kFewWarps * 16;
-    int key = key0 + warp * 16;
-    auto page_at = [&](int k) { return k < key1 ? kvq8_page(p.c, p.b, seq, k >> p.c.page_shift) : -1; };
-    auto tile = [&](const int8_t* codes, int page, int k) {
-      return codes + page * p.c.page_stride + head * p.c.head_stride + (k & (p.c.page_tokens - 1)) * p.c.token_stride;
-    };
-    auto load_k = [&](int page, int k) {
-      if (page < 0) return;
-      const int8_t* t = tile(p.c.k, page, k) + 16 * c;
+    auto wait_piece = [&](int half) { ok = ok && mbar_wait_bounded(&s_bar[warp][slot][half], phase, p.err); };
+#pragma unroll 1
+    for (int t = 0; t < tiles; ++t) {
+      if (t == batch + 32) {
+        batch = t;
+        page_l = page_n, page_n = page_nn;
+        ks_l = ks_n, vs_l = vs_n;
+      }
+      // the batch after the next: its pages early in this one, the next one's scales later
+      if (t == batch + 4) page_nn = lane_page(batch + 64);
+      if (t == batch + 8) ks_n = lane_scale(p.c.k_scale, page_n), vs_n = lane_scale(p.c.v_scale, page_n);
+      if (__shfl_sync(0xffffffffu, page_l, t & 31) < 0) continue;
+      if (ti <= t) {  // nothing was asked for: more than a batch of absent pages lay between
+#pragma unroll 1
+        for (int i = 0; i < D; ++i) ask_k(), ask_v();
+      }
+      const int key = first_key + 16 * W * t;
+      const float ks = __shfl_sync(0xffffffffu, ks_l, t & 31), vs = __shfl_sync(0xffffffffu, vs_l, t & 31);
+      wait_piece(0);
+
+      // S^T = K Q^T; two accumulators a plane keep the chains of dependent products short
+      float sc[NT][4];
+      {
+        float sp[2 * PL][NT][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+        for (int a = 0; a < 2 * PL; ++a)
 #pragma unroll
-        for (int i = 0; i < KL; ++i) kr[i][h] = ldg_stream(t + (g + 8 * h) * p.c.token_stride + 64 * i);
-      const int64_t at_s = static_cast<int64_t>(page) * kvh + head;
-      ks_n = __ldg(p.c.k_scale + at_s);
-      vs_n = __ldg(p.c.v_scale + at_s);
-    };
-    int page = page_at(key), page_n = page_at(key + kstep);
-    load_k(page, key);
-    for (; key < key1; key += kstep) {
-      const int page_nn = page_at(key + 2 * kstep);
-      ks = ks_n, vs = vs_n;
-      if (page >= 0) {
-        const int8_t* t = tile(p.c.v, page, key);
-        if constexpr (HD >= 128) {
+          for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int i = 0; i < VL; ++i)
+            for (int e = 0; e < 4; ++e) sp[a][j][e] = 0.0f;
+        const uint8_t* kt = ring + slot * 2 * PIECE;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              vr[i][e] = ldg_stream(t + (2 * c + (e & 1) + 8 * (e >> 1)) * p.c.token_stride + 128 * i + 16 * g);
-        } else {
-          // 64 dimensions: 8 bytes a lane and key
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint2 x = __ldg(reinterpret_cast<const uint2*>(t + (2 * c + (e & 1) + 8 * (e >> 1)) * p.c.token_stride + 8 * g));
-            vr[0][e].x = x.x, vr[0][e].y = x.y;
-          }
-        }
-        float sc[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[j][e] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < KL; ++i) {
-          const uint32_t w0[4] = {kr[i][0].x ^ 0x80808080u, kr[i][0].y ^ 0x80808080u, kr[i][0].z ^ 0x80808080u,
-                                  kr[i][0].w ^ 0x80808080u};
-          const uint32_t w1[4] = {kr[i][1].x ^ 0x80808080u, kr[i][1].y ^ 0x80808080u, kr[i][1].z ^ 0x80808080u,
-                                  kr[i][1].w ^ 0x80808080u};
+        for (int i = 0; i < HD / 64; ++i) {
+          // rows g and g + 8 share their swizzle
+          const uint8_t* at_k = HD >= 128 ? kt + 2048 * (i >> 1) + 128 * g + (((2 * c + (i & 1)) ^ g) << 4)
+                                          : kt + 64 * g + ((c ^ (g >> 1)) << 4);
+          const uint4 k0 = *reinterpret_cast<const uint4*>(at_k);
+          const uint4 k1 = *reinterpret_cast<const uint4*>(at_k + (HD >= 128 ? 1024 : 512));
+          const uint32_t w0[4] = {k0.x ^ 0x80808080u, k0.y ^ 0x80808080u, k0.z ^ 0x80808080u, k0.w ^ 0x80808080u};
+          const uint32_t w1[4] = {k1.x ^ 0x80808080u, k1.y ^ 0x80808080u, k1.z ^ 0x80808080u, k1.w ^ 0x80808080u};
           uint4 qf[PL][NT][2];
 #pragma unroll
           for (int pl = 0; pl < PL; ++pl)
@@ -318,108 +419,126 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_ctas_per_sm<HD>())
 #pragma unroll
               for (int j = 0; j < NT; ++j) {
                 const uint4 qv = qf[pl][j][u >> 1];
-                mma_16816(sc[j], a0, a1, a2, a3, u & 1 ? qv.z : qv.x, u & 1 ? qv.w : qv.y);
+                mma_16816(sp[2 * pl + (u & 1)][j], a0, a1, a2, a3, u & 1 ? qv.z : qv.x, u & 1 ? qv.w : qv.y);
               }
           }
         }
-        load_k(page_n, key + kstep);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[j][e] = sp[0][j][e] + sp[1][j][e];
+            if constexpr (PL == 2) sc[j][e] += sp[2 * PL - 2][j][e] + sp[2 * PL - 1][j][e];
+          }
+      }
+      __syncwarp();
+      ask_k();
 
-        // softmax over the tile's keys g and g + 8
-        const bool edge = key + 16 > all_see || key + 16 > key1;
-        const int ve = min(max(static_cast<int>(__float_as_uint(vs) >> 23), 20), 254);
-        const float kmul = ks;
-        float mn[NT][2];
-        bool grow = ve > vexp;
+      // softmax over the tile's keys g and g + 8
+      const bool edge = key + 16 > all_see || key + 16 > key1;
+      const int ve = min(max(static_cast<int>(__float_as_uint(vs) >> 23), 20), 254);
+      float mn[NT][2];
+      bool grow = ve > vexp;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float mul = ks * qs[j][e];
+          float a = sc[j][e] * mul, b = sc[j][e + 2] * mul;
+          if (edge) {
+            const int r = 8 * j + 2 * c + e;
+            const int end = r < live ? min(key1, start + (row0 + r) / p.group + 1) : 0;
+            if (key + g >= end) a = -INFINITY;
+            if (key + g + 8 >= end) b = -INFINITY;
+          }
+          sc[j][e] = a, sc[j][e + 2] = b;
+          float t2 = fmaxf(a, b);
+          t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, 4));
+          t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, 8));
+          t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, 16));
+          mn[j][e] = fmaxf(m[j][e], t2);
+          grow = grow || mn[j][e] > m[j][e];
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+        const int vn = max(ve, vexp);
+        const float vf = __uint_as_float(static_cast<uint32_t>(max(127 + vexp - vn, 0)) << 23);
+        vexp = vn;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float mul = kmul * qs[j][e];
-            float a = sc[j][e] * mul, b = sc[j][e + 2] * mul;
-            if (edge) {
-              const int r = 8 * j + 2 * c + e;
-              const int end = r < live ? min(key1, start + (row0 + r) / p.group + 1) : 0;
-              if (key + g >= end) a = -INFINITY;
-              if (key + g + 8 >= end) b = -INFINITY;
-            }
-            sc[j][e] = a, sc[j][e + 2] = b;
-            float t2 = fmaxf(a, b);
-            t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, 4));
-            t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, 8));
-            t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, 16));
-            mn[j][e] = fmaxf(m[j][e], t2);
-            grow = grow || mn[j][e] > m[j][e];
+            const float f = m[j][e] == -INFINITY ? 0.0f : ex2(m[j][e] - mn[j][e]);
+            m[j][e] = mn[j][e];
+            l[j][e] *= f;
+            const float fo = f * vf;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) o[i][j][e] *= fo, o[i][j][e + 2] *= fo;
           }
-        if (__any_sync(0xffffffffu, grow)) {
-          const int vn = max(ve, vexp);
-          const float vf = __uint_as_float(static_cast<uint32_t>(max(127 + vexp - vn, 0)) << 23);
-          vexp = vn;
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float f = m[j][e] == -INFINITY ? 0.0f : ex2(m[j][e] - mn[j][e]);
-              m[j][e] = mn[j][e];
-              l[j][e] *= f;
-              const float fo = f * vf;
-#pragma unroll
-              for (int i = 0; i < HD / 16; ++i) o[i][j][e] *= fo, o[i][j][e + 2] *= fo;
-            }
-        }
-        // 2^14 * v_scale / 2^(vexp - 126)
-        const float vmul = vs * __uint_as_float(static_cast<uint32_t>(min(127 + 140 - vexp, 254)) << 23);
-        uint32_t pb[PL][NT][2];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          float w[4];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float mm = fmaxf(m[j][e], -1e30f);
-            const float a = ex2(sc[j][e] - mm), b = ex2(sc[j][e + 2] - mm);
-            l[j][e] += a + b;
-            w[e] = a * vmul;
-            w[e + 2] = b * vmul;
-          }
-          const uint32_t h0 = pack_half2(w[0], w[1]), h1 = pack_half2(w[2], w[3]);
-          pb[0][j][0] = transpose_8x8(h0);
-          pb[0][j][1] = transpose_8x8(h1);
-          if constexpr (PL == 2) {
-            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-            const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-            pb[PL - 1][j][0] = transpose_8x8(pack_half2(w[0] - f0.x, w[1] - f0.y));
-            pb[PL - 1][j][1] = transpose_8x8(pack_half2(w[2] - f1.x, w[3] - f1.y));
-          }
-        }
-        // O^T += V^T P^T
-        constexpr int WORDS = HD >= 128 ? 4 : 2;
-#pragma unroll
-        for (int i = 0; i < VL; ++i)
-#pragma unroll
-          for (int u = 0; u < WORDS; ++u) {
-            const uint32_t x0 = u == 0 ? vr[i][0].x : u == 1 ? vr[i][0].y : u == 2 ? vr[i][0].z : vr[i][0].w;
-            const uint32_t x1 = u == 0 ? vr[i][1].x : u == 1 ? vr[i][1].y : u == 2 ? vr[i][1].z : vr[i][1].w;
-            const uint32_t x2 = u == 0 ? vr[i][2].x : u == 1 ? vr[i][2].y : u == 2 ? vr[i][2].z : vr[i][2].w;
-            const uint32_t x3 = u == 0 ? vr[i][3].x : u == 1 ? vr[i][3].y : u == 2 ? vr[i][3].z : vr[i][3].w;
-            const uint32_t lo01 = prmt(x0, x1, 0x5140u) ^ 0x80808080u, hi01 = prmt(x0, x1, 0x7362u) ^ 0x80808080u;
-            const uint32_t lo23 = prmt(x2, x3, 0x5140u) ^ 0x80808080u, hi23 = prmt(x2, x3, 0x7362u) ^ 0x80808080u;
-            const uint32_t a0 = codes_to_half2(lo01, 0x4140u), a1 = codes_to_half2(lo01, 0x4342u);
-            const uint32_t a2 = codes_to_half2(lo23, 0x4140u), a3 = codes_to_half2(lo23, 0x4342u);
-            const uint32_t c0 = codes_to_half2(hi01, 0x4140u), c1 = codes_to_half2(hi01, 0x4342u);
-            const uint32_t c2 = codes_to_half2(hi23, 0x4140u), c3 = codes_to_half2(hi23, 0x4342u);
-            const int mt = (i * WORDS + u) * 2;
-#pragma unroll
-            for (int pl = 0; pl < PL; ++pl)
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                mma_16816(o[mt][j], a0, a1, a2, a3, pb[pl][j][0], pb[pl][j][1]);
-                mma_16816(o[mt + 1][j], c0, c1, c2, c3, pb[pl][j][0], pb[pl][j][1]);
-              }
-          }
-      } else {
-        load_k(page_n, key + kstep);
       }
-      page = page_n;
-      page_n = page_nn;
+      // 2^14 * v_scale / 2^(vexp - 126)
+      const float vmul = vs * __uint_as_float(static_cast<uint32_t>(min(127 + 140 - vexp, 254)) << 23);
+      uint32_t pb[PL][NT][2];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float mm = fmaxf(m[j][e], -1e30f);
+          const float a = ex2(sc[j][e] - mm), b = ex2(sc[j][e + 2] - mm);
+          l[j][e] += a + b;
+          w[e] = a * vmul;
+          w[e + 2] = b * vmul;
+        }
+        const uint32_t h0 = pack_half2(w[0], w[1]), h1 = pack_half2(w[2], w[3]);
+        pb[0][j][0] = transpose_8x8(h0);
+        pb[0][j][1] = transpose_8x8(h1);
+        if constexpr (PL == 2) {
+          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+          const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+          pb[PL - 1][j][0] = transpose_8x8(pack_half2(w[0] - f0.x, w[1] - f0.y));
+          pb[PL - 1][j][1] = transpose_8x8(pack_half2(w[2] - f1.x, w[3] - f1.y));
+        }
+      }
+
+      // O^T += V^T P^T
+      wait_piece(1);
+      const uint8_t* vt = ring + (slot * 2 + 1) * PIECE;
+      constexpr int WORDS = HD >= 128 ? 4 : 2, VL = HD >= 128 ? HD / 128 : 1;
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        uint32_t x[4][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = 2 * c + (e & 1) + 8 * (e >> 1);
+          if constexpr (WORDS == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(vt + 2048 * i + 128 * row + ((g ^ (row & 7)) << 4));
+            x[e][0] = v.x, x[e][1] = v.y, x[e][2] = v.z, x[e][3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(vt + 64 * row + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
+            x[e][0] = v.x, x[e][1] = v.y;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < WORDS; ++u) {
+          const uint32_t lo01 = prmt(x[0][u], x[1][u], 0x5140u) ^ 0x80808080u, hi01 = prmt(x[0][u], x[1][u], 0x7362u) ^ 0x80808080u;
+          const uint32_t lo23 = prmt(x[2][u], x[3][u], 0x5140u) ^ 0x80808080u, hi23 = prmt(x[2][u], x[3][u], 0x7362u) ^ 0x80808080u;
+          const uint32_t a0 = codes_to_half2(lo01, 0x4140u), a1 = codes_to_half2(lo01, 0x4342u);
+          const uint32_t a2 = codes_to_half2(lo23, 0x4140u), a3 = codes_to_half2(lo23, 0x4342u);
+          const uint32_t c0 = codes_to_half2(hi01, 0x4140u), c1 = codes_to_half2(hi01, 0x4342u);
+          const uint32_t c2 = codes_to_half2(hi23, 0x4140u), c3 = codes_to_half2(hi23, 0x4342u);
+          const int mt = (i * WORDS + u) * 2;
+#pragma unroll
+          for (int pl = 0; pl < PL; ++pl)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              mma_16816(o[mt][j], a0, a1, a2, a3, pb[pl][j][0], pb[pl][j][1]);
+              mma_16816(o[mt + 1][j], c0, c1, c2, c3, pb[pl][j][0], pb[pl][j][1]);
+            }
+        }
+      }
+      __syncwarp();
+      ask_v();
+      if (++slot == D) slot = 0, phase ^= 1;
     }
 
     // join the warps: common maximum, then sums in warp order
@@ -434,54 +553,63 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_ctas_per_sm<HD>())
         if (g == 0) s_m[warp][8 * j + 2 * c + e] = m[j][e], s_l[warp][8 * j + 2 * c + e] = t2;
       }
     const float back = __uint_as_float(static_cast<uint32_t>(max(vexp - 13, 1)) << 23);  // 2^(vexp - 126 - 14)
+    __syncthreads();  // every ring is empty
     float* mine = s_o + warp * RG * OF;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i)
+      for (int e = 0; e < 2; ++e) {
+        if (8 * j + 2 * c + e >= live || m[j][e] == -INFINITY) continue;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int i = 0; i < HD / 16; ++i)
           *reinterpret_cast<float2*>(mine + (8 * j + 2 * c + e) * OF + (i * 8 + g) * 2) =
               make_float2(o[i][j][e] * back, o[i][j][e + 2] * back);
+      }
     __syncthreads();
-    const bool whole = gran0 == 0 && gran1 == fs.granules;
+    const bool whole = r.whole;
     float* rec = nullptr;
     if (!whole) rec = p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (begin == first ? 0 : 1)) * few_partial_floats<HD, NT>();
-    for (int r = warp; r < live; r += kFewWarps) {
-      float top = s_m[0][r];
+    // a warp per row and part of the head, so that more warps work on few rows
+    constexpr int PARTS = NT == 1 ? 2 : 1, V = HD / 32 / PARTS;
+    for (int rp = warp; rp < live * PARTS; rp += W) {
+      const int rr = rp / PARTS, d0 = (rp % PARTS) * (HD / PARTS) + lane * V;
+      float top = s_m[0][rr];
 #pragma unroll
-      for (int w = 1; w < kFewWarps; ++w) top = fmaxf(top, s_m[w][r]);
-      float f[kFewWarps], sum = 0.0f;
+      for (int w = 1; w < W; ++w) top = fmaxf(top, s_m[w][rr]);
+      float sum = 0.0f, x[V];
 #pragma unroll
-      for (int w = 0; w < kFewWarps; ++w) {
-        f[w] = s_m[w][r] == -INFINITY ? 0.0f : ex2(s_m[w][r] - top);
-        sum += f[w] * s_l[w][r];
+      for (int e = 0; e < V; ++e) x[e] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (s_m[w][rr] == -INFINITY) continue;  // no tile for this warp
+        const float f = ex2(s_m[w][rr] - top);
+        sum += f * s_l[w][rr];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int d = d0 + e;
+          // where dimension d lies: lane g and fragment i of the reads above
+          constexpr int PER = HD >= 128 ? 16 : 8, SLAB = HD >= 128 ? 128 : 64;
+          const int in = d % SLAB;
+          const int idx = (((d / SLAB) * (PER / 2) + (in % PER) / 2) * 8 + in / PER) * 2 + (d & 1);
+          x[e] += f * s_o[(w * RG + rr) * OF + idx];
+        }
       }
-      const float inv = whole ? (sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum)) : 1.0f;
-      const int row = row0 + r;
-      constexpr int V = HD / 32;
-      float x[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int d = lane * V + e;
-        // where dimension d lies: lane g and fragment i of the loads above
-        constexpr int PER = HD >= 128 ? 16 : 8, SLAB = HD >= 128 ? 128 : 64;
-        const int in = d % SLAB;
-        const int idx = (((d / SLAB) * (PER / 2) + (in % PER) / 2) * 8 + in / PER) * 2 + (d & 1);
-        float acc = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) acc += f[w] * s_o[(w * RG + r) * OF + idx];
-        x[e] = acc * inv;
-      }
+      const int row = row0 + rr;
       if (whole) {
-        store_vec<T, V>(static_cast<T*>(p.out) + static_cast<int64_t>(sq.first + row / p.group) * p.out_stride +
-                            (static_cast<int64_t>(head) * p.group + row % p.group) * HD + lane * V,
+        const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] *= inv;
+        store_any<T, V>(static_cast<T*>(p.out) + static_cast<int64_t>(sq.first + row / p.group) * p.out_stride +
+                            (static_cast<int64_t>(head) * p.group + row % p.group) * HD + d0,
                         x);
       } else {
-        store_vec<float, V>(rec + r * HD + lane * V, x);
-        if (lane == 0) rec[RG * HD + 2 * r] = top, rec[RG * HD + 2 * r + 1] = sum;
+        store_any<float, V>(rec + rr * HD + d0, x);
+        if (lane == 0 && rp % PARTS == 0) rec[RG * HD + 2 * rr] = top, rec[RG * HD + 2 * rr + 1] = sum;
       }
     }
+    // the next run's tiles go where the sums lay; s_m, s_l and q are written again
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
   }
 }
 
