@@ -3,20 +3,23 @@
 //
 // For a unit (sequence, KV head, group of up to 8 NT query rows) the cache's
 // codes pass once through registers:
-//   S^T = K Q^T, s = S * k_scale * scale, running maximum m, p = 2^(s - m),
+//   S^T = K Q^T, s = S * k_scale * scale, reference m, p = 2^(s - m),
 //   O^T += V^T (p * v_scale)^T, l += p;   out = O / l.
-// Codes are integers below 128 in magnitude, exact in half, so only q and p
-// are rounded: half rows use q as given and p as one half; fp32 rows use both
-// as high + low halves (22 bits).  v_scale goes into p, relative to the
-// largest power of two met so far (exact to move) and 2^14 above it, so p
-// keeps its relative accuracy down to 2^-28 of the largest in half.
+// m is a score of the row that no later one exceeds by more than 2^8: only
+// when one does (a vote, no reduction) is the true maximum taken and O
+// rescaled.  Codes are integers below 128 in magnitude, exact in half, so only
+// q and p are rounded: half rows use q as given and p as one half; fp32 rows
+// use both as high + low halves (22 bits).  v_scale goes into p, relative to
+// the largest power of two met so far (exact to move) and 2^7 above it: p
+// stays below 2^15 and keeps its accuracy in half down to 2^-21 of a weight
+// of one (with the low half to 2^-31).
 //
 // Work is cut into granules of 128 keys, laid end to end over all units; each
 // of the grid's CTAs takes an equal run of them, whatever the lengths are, so
 // the kernel needs no host knowledge of the lengths.  A unit that crosses
 // CTAs leaves partial (m, l, O) records, which kvq8_merge_kernel joins in
 // order: the result depends on no timing.  Within a CTA, the warps take
-// 16-key tiles in turn, each with its own m, l and O, and join in shared
+// tiles of 16 to 64 keys in turn, each with its own m, l and O, and join in shared
 // memory at the end of the unit's run.
 //
 // Bound by HBM: 2 bytes per key, head and dimension, and next by the
@@ -44,11 +47,13 @@ constexpr int kFewMaxSeqs = 4096;
 // Warps of a CTA (one CTA per SM), by what the accumulators (head_dim / 16 x
 // NT x 4 registers a lane) leave.
 template <int HD, int NT>
-constexpr int few_warps() { return HD / 16 * NT * 4 > 96 ? 8 : 12; }
-// Tiles (16 rows of K and of V) in a warp's ring, within 192 KB for all warps.
+constexpr int few_warps() { return HD / 16 * NT * 4 >= 96 ? 8 : 12; }
+// A warp's tile: this many blocks of 16 keys, 2 or 4 KB of K and as much of V.
+__host__ __device__ constexpr int few_blocks(int hd) { return hd == 256 ? 1 : 2; }
+// Tiles in a warp's ring, within 192 KB for all warps.
 template <int HD, int NT>
 constexpr int few_ring() {
-  constexpr int n = 196608 / (few_warps<HD, NT>() * 32 * HD);
+  constexpr int n = 196608 / (few_warps<HD, NT>() * 32 * HD * few_blocks(HD));
   return n < 4 ? n : 4;
 }
 // Groups of 8 rows a unit may have.
@@ -141,7 +146,7 @@ constexpr int few_partial_floats() { return 8 * NT * (HD + 2); }
 template <typename T, int HD, int NT>
 constexpr size_t few_smem() {
   constexpr int planes = sizeof(T) == 4 ? 2 : 1, warps = few_warps<HD, NT>();
-  constexpr size_t ring = static_cast<size_t>(warps) * few_ring<HD, NT>() * 32 * HD;
+  constexpr size_t ring = static_cast<size_t>(warps) * few_ring<HD, NT>() * 32 * HD * few_blocks(HD);
   constexpr size_t join = static_cast<size_t>(warps) * 8 * NT * (HD + 4) * 4;
   return (ring > join ? ring : join) + static_cast<size_t>(8 * NT) * planes * (HD * 2 + 16);
 }
@@ -154,7 +159,7 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
   constexpr int PL = sizeof(T) == 4 ? 2 : 1;      // half planes of q and p
   constexpr int QB = HD * 2 + 16;                 // bytes of a q row: conflict-free 16-byte reads
   constexpr int OF = HD + 4;                      // floats of an O row in shared memory
-  constexpr int W = few_warps<HD, NT>(), D = few_ring<HD, NT>(), PIECE = 16 * HD;
+  constexpr int W = few_warps<HD, NT>(), D = few_ring<HD, NT>(), MK = few_blocks(HD), BLOCK = 16 * HD, PIECE = MK * BLOCK;
   constexpr size_t RING = static_cast<size_t>(W) * D * 2 * PIECE, JOIN = static_cast<size_t>(W) * RG * OF * 4;
   extern __shared__ __align__(1024) uint8_t few_raw[];
   float* s_o = reinterpret_cast<float*>(few_raw);                   // [W][RG][OF], in the ring's place once it is empty
@@ -260,41 +265,48 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
     const int head = r.head, row0 = r.row0, live = r.live, key1 = r.key1, start = sq.length - sq.n;
     const int all_see = start + row0 / p.group + 1;  // keys below it are seen by every row
 
-    // this warp's tiles: keys key0 + 16 (warp + W t); lane t % 32 holds tile t's page and scales
-    const int first_key = r.key0 + 16 * warp;
-    const int tiles = key1 > first_key ? (key1 - first_key - 1) / (16 * W) + 1 : 0;
-    auto lane_page = [&](int t0) {
-      const int t = t0 + lane;
-      return t < tiles ? kvq8_page(p.c, p.b, seq, (first_key + 16 * W * t) >> p.c.page_shift) : -1;
+    // this warp's tiles: keys from key0 + 16 MK (warp + W t) on; lane b % 32 holds the page and scales of block b
+    const int first_key = r.key0 + 16 * MK * warp;
+    const int tiles = key1 > first_key ? (key1 - first_key - 1) / (16 * MK * W) + 1 : 0;
+    auto block_key = [&](int b) { return first_key + 16 * MK * W * (b / MK) + 16 * (b % MK); };
+    auto lane_page = [&](int b0) {
+      const int key = block_key(b0 + lane);
+      return key < key1 ? kvq8_page(p.c, p.b, seq, key >> p.c.page_shift) : -1;
     };
     auto lane_scale = [&](const float* s, int page) { return page >= 0 ? __ldg(s + static_cast<int64_t>(page) * kvh + head) : 0.0f; };
-    int page_l = lane_page(0), page_n = lane_page(32), page_nn = -1;  // of this batch of 32 tiles, and the next
-    int ti = 0, batch = 0;       // the next tile to ask for; the first tile of the batch in the lanes
-    int page_i = -1, row_i = 0;  // the tile whose K was asked for last: its V follows
-    auto piece = [&](const CUtensorMap* map, int half) {
+    int page_l = lane_page(0), page_n = lane_page(32), page_nn = -1;  // of this batch of 32 blocks, the next and its next
+    int batch = 0;                // the first block of the batch in the lanes
+    int ti = 0, page_i[MK] = {};  // the next tile to ask for; the pages of the one whose K was asked for last
+    // what is absent or past the run is neither copied nor looked at (its weights are 0, and codes are numbers)
+    auto piece = [&](const CUtensorMap* map, int half, int tile) {
       if (lane == 0) {
         uint64_t* bar = &s_bar[warp][slot_i][half];
         uint8_t* dst = ring + (slot_i * 2 + half) * PIECE;
-        mbar_arrive_expect_tx(bar, PIECE);
+        int bytes = 0;
 #pragma unroll
-        for (int i = 0; i < (HD + 127) / 128; ++i) tma_load_4d(dst + 2048 * i, map, 128 * i, row_i, head, page_i, bar);
+        for (int b = 0; b < MK; ++b) bytes += page_i[b] >= 0 ? BLOCK : 0;
+        mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+        for (int b = 0; b < MK; ++b) {
+          if (page_i[b] < 0) continue;
+          const int row = block_key(tile * MK + b) & (p.c.page_tokens - 1);
+#pragma unroll
+          for (int i = 0; i < (HD + 127) / 128; ++i)
+            tma_load_4d(dst + b * BLOCK + 2048 * i, map, 128 * i, row, head, page_i[b], bar);
+        }
       }
     };
     auto ask_k = [&]() {
-      const int lim = min(tiles, batch + 64);
-      page_i = -1;
-      for (; ti < lim; ++ti) {
-        page_i = __shfl_sync(0xffffffffu, ti < batch + 32 ? page_l : page_n, ti & 31);
-        if (page_i >= 0) break;
-      }
-      if (page_i < 0) return;
-      row_i = (first_key + 16 * W * ti) & (p.c.page_tokens - 1);
-      piece(&kmap, 0);
-      ++ti;
+      if (ti >= tiles) return;
+#pragma unroll
+      for (int b = 0; b < MK; ++b)
+        page_i[b] = __shfl_sync(0xffffffffu, ti * MK < batch + 32 ? page_l : page_n, (ti * MK + b) & 31);
+      piece(&kmap, 0, ti);
     };
     auto ask_v = [&]() {
-      if (page_i < 0) return;
-      piece(&vmap, 1);
+      if (ti >= tiles) return;
+      piece(&vmap, 1, ti);
+      ++ti;
       slot_i = slot_i + 1 == D ? 0 : slot_i + 1;
     };
 #pragma unroll 1
@@ -364,43 +376,43 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
     auto wait_piece = [&](int half) { ok = ok && mbar_wait_bounded(&s_bar[warp][slot][half], phase, p.err); };
 #pragma unroll 1
     for (int t = 0; t < tiles; ++t) {
-      if (t == batch + 32) {
-        batch = t;
+      const int blk = t * MK;
+      if (blk == batch + 32) {
+        batch = blk;
         page_l = page_n, page_n = page_nn;
         ks_l = ks_n, vs_l = vs_n;
       }
       // the batch after the next: its pages early in this one, the next one's scales later
-      if (t == batch + 4) page_nn = lane_page(batch + 64);
-      if (t == batch + 8) ks_n = lane_scale(p.c.k_scale, page_n), vs_n = lane_scale(p.c.v_scale, page_n);
-      if (__shfl_sync(0xffffffffu, page_l, t & 31) < 0) continue;
-      if (ti <= t) {  // nothing was asked for: more than a batch of absent pages lay between
-#pragma unroll 1
-        for (int i = 0; i < D; ++i) ask_k(), ask_v();
+      if (blk == batch + 4) page_nn = lane_page(batch + 64);
+      if (blk == batch + 8) ks_n = lane_scale(p.c.k_scale, page_n), vs_n = lane_scale(p.c.v_scale, page_n);
+      const int key = block_key(blk);
+      float ks[MK], vs[MK];
+      bool edge = key + 16 * MK > all_see || key + 16 * MK > key1;
+      uint32_t gone = 0;  // blocks without a page
+#pragma unroll
+      for (int b = 0; b < MK; ++b) {
+        ks[b] = __shfl_sync(0xffffffffu, ks_l, (blk + b) & 31), vs[b] = __shfl_sync(0xffffffffu, vs_l, (blk + b) & 31);
+        if (__shfl_sync(0xffffffffu, page_l, (blk + b) & 31) < 0) gone |= 1u << b;
       }
-      const int key = first_key + 16 * W * t;
-      const float ks = __shfl_sync(0xffffffffu, ks_l, t & 31), vs = __shfl_sync(0xffffffffu, vs_l, t & 31);
+      edge = edge || gone;
       wait_piece(0);
 
-      // S^T = K Q^T; two accumulators a plane keep the chains of dependent products short
-      float sc[NT][4];
+      // S^T = K Q^T; where one block has few accumulators, more of them keep the chains of dependent products short
+      float sc[MK][NT][4];
+      constexpr int SPLIT = MK * NT == 1 ? 2 * PL : (MK * NT == 2 ? PL : 1);
       {
-        float sp[2 * PL][NT][4];
+        float sp[SPLIT][MK][NT][4];
 #pragma unroll
-        for (int a = 0; a < 2 * PL; ++a)
+        for (int a = 0; a < SPLIT; ++a)
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
+          for (int b = 0; b < MK; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sp[a][j][e] = 0.0f;
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sp[a][b][j][e] = 0.0f;
         const uint8_t* kt = ring + slot * 2 * PIECE;
 #pragma unroll
         for (int i = 0; i < HD / 64; ++i) {
-          // rows g and g + 8 share their swizzle
-          const uint8_t* at_k = HD >= 128 ? kt + 2048 * (i >> 1) + 128 * g + (((2 * c + (i & 1)) ^ g) << 4)
-                                          : kt + 64 * g + ((c ^ (g >> 1)) << 4);
-          const uint4 k0 = *reinterpret_cast<const uint4*>(at_k);
-          const uint4 k1 = *reinterpret_cast<const uint4*>(at_k + (HD >= 128 ? 1024 : 512));
-          const uint32_t w0[4] = {k0.x ^ 0x80808080u, k0.y ^ 0x80808080u, k0.z ^ 0x80808080u, k0.w ^ 0x80808080u};
-          const uint32_t w1[4] = {k1.x ^ 0x80808080u, k1.y ^ 0x80808080u, k1.z ^ 0x80808080u, k1.w ^ 0x80808080u};
           uint4 qf[PL][NT][2];
 #pragma unroll
           for (int pl = 0; pl < PL; ++pl)
@@ -411,53 +423,75 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
               qf[pl][j][1] = src[1];
             }
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const uint32_t a0 = codes_to_half2(w0[u], 0x4140u), a2 = codes_to_half2(w0[u], 0x4342u);
-            const uint32_t a1 = codes_to_half2(w1[u], 0x4140u), a3 = codes_to_half2(w1[u], 0x4342u);
+          for (int b = 0; b < MK; ++b) {
+            // rows g and g + 8 share their swizzle
+            const uint8_t* at_k = kt + b * BLOCK + (HD >= 128 ? 2048 * (i >> 1) + 128 * g + (((2 * c + (i & 1)) ^ g) << 4)
+                                                              : 64 * g + ((c ^ (g >> 1)) << 4));
+            const uint4 k0 = *reinterpret_cast<const uint4*>(at_k);
+            const uint4 k1 = *reinterpret_cast<const uint4*>(at_k + (HD >= 128 ? 1024 : 512));
+            const uint32_t w0[4] = {k0.x ^ 0x80808080u, k0.y ^ 0x80808080u, k0.z ^ 0x80808080u, k0.w ^ 0x80808080u};
+            const uint32_t w1[4] = {k1.x ^ 0x80808080u, k1.y ^ 0x80808080u, k1.z ^ 0x80808080u, k1.w ^ 0x80808080u};
 #pragma unroll
-            for (int pl = 0; pl < PL; ++pl)
+            for (int u = 0; u < 4; ++u) {
+              const uint32_t a0 = codes_to_half2(w0[u], 0x4140u), a2 = codes_to_half2(w0[u], 0x4342u);
+              const uint32_t a1 = codes_to_half2(w1[u], 0x4140u), a3 = codes_to_half2(w1[u], 0x4342u);
 #pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                const uint4 qv = qf[pl][j][u >> 1];
-                mma_16816(sp[2 * pl + (u & 1)][j], a0, a1, a2, a3, u & 1 ? qv.z : qv.x, u & 1 ? qv.w : qv.y);
-              }
+              for (int pl = 0; pl < PL; ++pl)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                  const uint4 qv = qf[pl][j][u >> 1];
+                  constexpr int A = SPLIT;
+                  const int a = A == 1 ? 0 : (A == PL ? pl : 2 * pl + (u & 1));
+                  mma_16816(sp[a][b][j], a0, a1, a2, a3, u & 1 ? qv.z : qv.x, u & 1 ? qv.w : qv.y);
+                }
+            }
           }
         }
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int b = 0; b < MK; ++b)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            sc[j][e] = sp[0][j][e] + sp[1][j][e];
-            if constexpr (PL == 2) sc[j][e] += sp[2 * PL - 2][j][e] + sp[2 * PL - 1][j][e];
-          }
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float x = sp[0][b][j][e];
+#pragma unroll
+              for (int a = 1; a < SPLIT; ++a) x += sp[a][b][j][e];
+              sc[b][j][e] = x * (ks[b] * qs[j][e & 1]);
+            }
       }
       __syncwarp();
       ask_k();
 
-      // softmax over the tile's keys g and g + 8
-      const bool edge = key + 16 > all_see || key + 16 > key1;
-      const int ve = min(max(static_cast<int>(__float_as_uint(vs) >> 23), 20), 254);
-      float mn[NT][2];
+      // keys g and g + 8 of each block against the row's reference
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int rr = 8 * j + 2 * c + e;
+            const int end = rr < live ? min(key1, start + (row0 + rr) / p.group + 1) : 0;
+#pragma unroll
+            for (int b = 0; b < MK; ++b) {
+              const bool no = gone >> b & 1;
+              if (no || key + 16 * b + g >= end) sc[b][j][e] = -INFINITY;
+              if (no || key + 16 * b + g + 8 >= end) sc[b][j][e + 2] = -INFINITY;
+            }
+          }
+      }
+      int ve = 20;
+#pragma unroll
+      for (int b = 0; b < MK; ++b) ve = max(ve, min(static_cast<int>(__float_as_uint(vs[b]) >> 23), 254));
       bool grow = ve > vexp;
+      float top[NT][2];
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float mul = ks * qs[j][e];
-          float a = sc[j][e] * mul, b = sc[j][e + 2] * mul;
-          if (edge) {
-            const int r = 8 * j + 2 * c + e;
-            const int end = r < live ? min(key1, start + (row0 + r) / p.group + 1) : 0;
-            if (key + g >= end) a = -INFINITY;
-            if (key + g + 8 >= end) b = -INFINITY;
-          }
-          sc[j][e] = a, sc[j][e + 2] = b;
-          float t2 = fmaxf(a, b);
-          t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, 4));
-          t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, 8));
-          t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, 16));
-          mn[j][e] = fmaxf(m[j][e], t2);
-          grow = grow || mn[j][e] > m[j][e];
+          float x = fmaxf(sc[0][j][e], sc[0][j][e + 2]);
+#pragma unroll
+          for (int b = 1; b < MK; ++b) x = fmaxf(x, fmaxf(sc[b][j][e], sc[b][j][e + 2]));
+          top[j][e] = x;
+          grow = grow || x > m[j][e] + 8.0f;
         }
       if (__any_sync(0xffffffffu, grow)) {
         const int vn = max(ve, vexp);
@@ -467,73 +501,85 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float f = m[j][e] == -INFINITY ? 0.0f : ex2(m[j][e] - mn[j][e]);
-            m[j][e] = mn[j][e];
+            float x = top[j][e];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float mn = fmaxf(m[j][e], x);
+            const float f = m[j][e] == -INFINITY ? 0.0f : ex2(m[j][e] - mn);
+            m[j][e] = mn;
             l[j][e] *= f;
             const float fo = f * vf;
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) o[i][j][e] *= fo, o[i][j][e + 2] *= fo;
           }
       }
-      // 2^14 * v_scale / 2^(vexp - 126)
-      const float vmul = vs * __uint_as_float(static_cast<uint32_t>(min(127 + 140 - vexp, 254)) << 23);
-      uint32_t pb[PL][NT][2];
+      // 2^7 / 2^(vexp - 126)
+      const float vup = __uint_as_float(static_cast<uint32_t>(min(260 - vexp, 254)) << 23);
+      uint32_t pb[PL][MK][NT][2];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        float w[4];
+      for (int b = 0; b < MK; ++b) {
+        const float vmul = vs[b] * vup;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float mm = fmaxf(m[j][e], -1e30f);
-          const float a = ex2(sc[j][e] - mm), b = ex2(sc[j][e + 2] - mm);
-          l[j][e] += a + b;
-          w[e] = a * vmul;
-          w[e + 2] = b * vmul;
-        }
-        const uint32_t h0 = pack_half2(w[0], w[1]), h1 = pack_half2(w[2], w[3]);
-        pb[0][j][0] = transpose_8x8(h0);
-        pb[0][j][1] = transpose_8x8(h1);
-        if constexpr (PL == 2) {
-          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-          const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-          pb[PL - 1][j][0] = transpose_8x8(pack_half2(w[0] - f0.x, w[1] - f0.y));
-          pb[PL - 1][j][1] = transpose_8x8(pack_half2(w[2] - f1.x, w[3] - f1.y));
+        for (int j = 0; j < NT; ++j) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float mm = fmaxf(m[j][e], -1e30f);
+            const float x = ex2(sc[b][j][e] - mm), y = ex2(sc[b][j][e + 2] - mm);
+            l[j][e] += x + y;
+            w[e] = x * vmul;
+            w[e + 2] = y * vmul;
+          }
+          const uint32_t h0 = pack_half2(w[0], w[1]), h1 = pack_half2(w[2], w[3]);
+          pb[0][b][j][0] = transpose_8x8(h0);
+          pb[0][b][j][1] = transpose_8x8(h1);
+          if constexpr (PL == 2) {
+            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+            const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+            pb[PL - 1][b][j][0] = transpose_8x8(pack_half2(w[0] - f0.x, w[1] - f0.y));
+            pb[PL - 1][b][j][1] = transpose_8x8(pack_half2(w[2] - f1.x, w[3] - f1.y));
+          }
         }
       }
 
       // O^T += V^T P^T
       wait_piece(1);
-      const uint8_t* vt = ring + (slot * 2 + 1) * PIECE;
       constexpr int WORDS = HD >= 128 ? 4 : 2, VL = HD >= 128 ? HD / 128 : 1;
 #pragma unroll
-      for (int i = 0; i < VL; ++i) {
-        uint32_t x[4][4];
+      for (int b = 0; b < MK; ++b) {
+        const uint8_t* vt = ring + (slot * 2 + 1) * PIECE + b * BLOCK;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = 2 * c + (e & 1) + 8 * (e >> 1);
-          if constexpr (WORDS == 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(vt + 2048 * i + 128 * row + ((g ^ (row & 7)) << 4));
-            x[e][0] = v.x, x[e][1] = v.y, x[e][2] = v.z, x[e][3] = v.w;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(vt + 64 * row + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
-            x[e][0] = v.x, x[e][1] = v.y;
-          }
-        }
+        for (int i = 0; i < VL; ++i) {
+          uint32_t x[4][4];
 #pragma unroll
-        for (int u = 0; u < WORDS; ++u) {
-          const uint32_t lo01 = prmt(x[0][u], x[1][u], 0x5140u) ^ 0x80808080u, hi01 = prmt(x[0][u], x[1][u], 0x7362u) ^ 0x80808080u;
-          const uint32_t lo23 = prmt(x[2][u], x[3][u], 0x5140u) ^ 0x80808080u, hi23 = prmt(x[2][u], x[3][u], 0x7362u) ^ 0x80808080u;
-          const uint32_t a0 = codes_to_half2(lo01, 0x4140u), a1 = codes_to_half2(lo01, 0x4342u);
-          const uint32_t a2 = codes_to_half2(lo23, 0x4140u), a3 = codes_to_half2(lo23, 0x4342u);
-          const uint32_t c0 = codes_to_half2(hi01, 0x4140u), c1 = codes_to_half2(hi01, 0x4342u);
-          const uint32_t c2 = codes_to_half2(hi23, 0x4140u), c3 = codes_to_half2(hi23, 0x4342u);
-          const int mt = (i * WORDS + u) * 2;
-#pragma unroll
-          for (int pl = 0; pl < PL; ++pl)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              mma_16816(o[mt][j], a0, a1, a2, a3, pb[pl][j][0], pb[pl][j][1]);
-              mma_16816(o[mt + 1][j], c0, c1, c2, c3, pb[pl][j][0], pb[pl][j][1]);
+          for (int e = 0; e < 4; ++e) {
+            const int row = 2 * c + (e & 1) + 8 * (e >> 1);
+            if constexpr (WORDS == 4) {
+              const uint4 v = *reinterpret_cast<const uint4*>(vt + 2048 * i + 128 * row + ((g ^ (row & 7)) << 4));
+              x[e][0] = v.x, x[e][1] = v.y, x[e][2] = v.z, x[e][3] = v.w;
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2*>(vt + 64 * row + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
+              x[e][0] = v.x, x[e][1] = v.y;
             }
+          }
+#pragma unroll
+          for (int u = 0; u < WORDS; ++u) {
+            const uint32_t lo01 = prmt(x[0][u], x[1][u], 0x5140u) ^ 0x80808080u, hi01 = prmt(x[0][u], x[1][u], 0x7362u) ^ 0x80808080u;
+            const uint32_t lo23 = prmt(x[2][u], x[3][u], 0x5140u) ^ 0x80808080u, hi23 = prmt(x[2][u], x[3][u], 0x7362u) ^ 0x80808080u;
+            const uint32_t a0 = codes_to_half2(lo01, 0x4140u), a1 = codes_to_half2(lo01, 0x4342u);
+            const uint32_t a2 = codes_to_half2(lo23, 0x4140u), a3 = codes_to_half2(lo23, 0x4342u);
+            const uint32_t c0 = codes_to_half2(hi01, 0x4140u), c1 = codes_to_half2(hi01, 0x4342u);
+            const uint32_t c2 = codes_to_half2(hi23, 0x4140u), c3 = codes_to_half2(hi23, 0x4342u);
+            const int mt = (i * WORDS + u) * 2;
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl)
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                mma_16816(o[mt][j], a0, a1, a2, a3, pb[pl][b][j][0], pb[pl][b][j][1]);
+                mma_16816(o[mt + 1][j], c0, c1, c2, c3, pb[pl][b][j][0], pb[pl][b][j][1]);
+              }
+          }
         }
       }
       __syncwarp();
@@ -552,7 +598,7 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
         t2 += __shfl_xor_sync(0xffffffffu, t2, 16);
         if (g == 0) s_m[warp][8 * j + 2 * c + e] = m[j][e], s_l[warp][8 * j + 2 * c + e] = t2;
       }
-    const float back = __uint_as_float(static_cast<uint32_t>(max(vexp - 13, 1)) << 23);  // 2^(vexp - 126 - 14)
+    const float back = __uint_as_float(static_cast<uint32_t>(max(vexp - 6, 1)) << 23);  // 2^(vexp - 126 - 7)
     __syncthreads();  // every ring is empty
     float* mine = s_o + warp * RG * OF;
 #pragma unroll
