@@ -42,6 +42,13 @@
 namespace kib {
 
 constexpr int kFewGranule = 128;
+// A run takes about 4.5 us besides its granules (pages looked up, q in, the
+// first tiles awaited, the warps joined), what an SM's share of the memory's
+// rate moves in three granules of 256 dimensions: runs are cut by granules
+// plus this, so that few CTAs get two.  (32 slots of about 2048: 24.8 us
+// without it, 27.9 with 8; verify of 17 sequences at 128 dimensions: 58.6 us
+// without it, 51.5 with 8.)
+__host__ __device__ constexpr int few_unit_cost(int hd) { return 768 / hd; }
 constexpr int kFewMaxSeqs = 4096;
 
 // Warps of a CTA (one CTA per SM), by what the accumulators (head_dim / 16 x
@@ -124,13 +131,14 @@ KIB_DEV void store_any(T* p, const float (&x)[V]) {
 
 // Granules of one unit of a sequence, and its units per KV head.
 struct FewSeq {
-  int granules, groups;
+  int granules, groups, unit;
+  KIB_DEV int64_t cost() const { return granules + unit; }
 };
-template <int NT>
+template <int HD, int NT>
 KIB_DEV FewSeq few_seq(const Kvq8AttnParams& p, int s) {
   const Kvq8Seq q = kvq8_seq(p.b, s);
   const int64_t rows = static_cast<int64_t>(q.n) * p.group;
-  FewSeq f{0, 0};
+  FewSeq f{0, 0, few_unit_cost(HD)};
   if (q.n > 0 && rows <= p.few_limit) {
     f.groups = static_cast<int>((rows + 8 * NT - 1) / (8 * NT));
     f.granules = max(1, (min(q.length, p.b.max_length) + kFewGranule - 1) / kFewGranule);
@@ -138,7 +146,7 @@ KIB_DEV FewSeq few_seq(const Kvq8AttnParams& p, int s) {
   return f;
 }
 
-// CTAs that share `total` granules: every one of them gets at least one.
+// CTAs that share a cost of `total`: every one of them gets at least one.
 KIB_DEV int64_t few_ctas(int64_t total, int64_t grid) { return total < grid ? total : grid; }
 
 template <int HD, int NT>
@@ -174,12 +182,14 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
   fence_mbar_init();
   if (tid == 0) tma_prefetch_desc(&kmap), tma_prefetch_desc(&vmap);
 
-  // granules of all sequences; then the sequence in which this CTA's run begins
+  pdl_launch_dependents();  // the merge's CTAs may take the SMs that are left and wait there
+
+  // the cost of all sequences; then the sequence in which this CTA's run begins
   constexpr int TH = W * 32;
   auto seq_cost = [&](int s) -> int64_t {
     if (s >= S) return 0;
-    const FewSeq f = few_seq<NT>(p, s);
-    return static_cast<int64_t>(f.granules) * f.groups * kvh;
+    const FewSeq f = few_seq<HD, NT>(p, s);
+    return f.cost() * f.groups * kvh;
   };
   auto scan = [&](int64_t v, int64_t* all) {
     int64_t inc = v;
@@ -223,27 +233,28 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
   }
   __syncthreads();
   int seq = s_seq;
-  int64_t seq_at = s_at;  // granules before the sequence
+  int64_t seq_at = s_at;  // cost before the sequence
 
   // the run of granules [gran0, gran1) of a unit that begins at `at`
   struct Run {
     Kvq8Seq sq;
     int head, row0, live, key0, key1;
-    bool whole;
+    bool whole, empty;
   };
   auto next_run = [&]() {
     Run r;
     r.sq = kvq8_seq(p.b, seq);
-    FewSeq fs = few_seq<NT>(p, seq);
-    while (at >= seq_at + static_cast<int64_t>(fs.granules) * fs.groups * kvh) {
-      seq_at += static_cast<int64_t>(fs.granules) * fs.groups * kvh;
+    FewSeq fs = few_seq<HD, NT>(p, seq);
+    while (at >= seq_at + fs.cost() * fs.groups * kvh) {
+      seq_at += fs.cost() * fs.groups * kvh;
       ++seq;
       r.sq = kvq8_seq(p.b, seq);
-      fs = few_seq<NT>(p, seq);
+      fs = few_seq<HD, NT>(p, seq);
     }
     const int64_t rel = at - seq_at;
-    const int unit = static_cast<int>(rel / fs.granules), gran0 = static_cast<int>(rel - static_cast<int64_t>(unit) * fs.granules);
-    const int gran1 = static_cast<int>(min(static_cast<int64_t>(fs.granules), gran0 + (stop - at)));
+    const int unit = static_cast<int>(rel / fs.cost());
+    const int64_t g0 = rel - unit * fs.cost() - few_unit_cost(HD), g1 = min(static_cast<int64_t>(fs.granules), g0 + (stop - at));
+    const int gran0 = static_cast<int>(max(g0, static_cast<int64_t>(0))), gran1 = static_cast<int>(max(g1, static_cast<int64_t>(0)));
     r.head = unit % kvh;
     r.row0 = unit / kvh * RG;
     r.live = min(RG, r.sq.n * p.group - r.row0);
@@ -251,7 +262,8 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
     const int span = max(0, min(r.sq.length, p.b.max_length));
     r.key1 = min(min(span, gran1 * kFewGranule), r.sq.length - r.sq.n + (r.row0 + r.live - 1) / p.group + 1);
     r.whole = gran0 == 0 && gran1 == fs.granules;
-    at += gran1 - gran0;
+    r.empty = gran0 == gran1;
+    at += g1 - g0;
     return r;
   };
 
@@ -261,6 +273,7 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
   while (at < stop) {
     const int64_t begin = at;
     const Run r = next_run();
+    if (r.empty) continue;
     const Kvq8Seq sq = r.sq;
     const int head = r.head, row0 = r.row0, live = r.live, key1 = r.key1, start = sq.length - sq.n;
     const int all_see = start + row0 / p.group + 1;  // keys below it are seen by every row
@@ -672,7 +685,7 @@ __global__ void __launch_bounds__(HD) kvq8_merge_kernel(const __grid_constant__ 
   const int r = blockIdx.y, kvh = p.c.kv_heads;
   const int head = blockIdx.x % kvh, rg = blockIdx.x / kvh % max_groups, seq = blockIdx.x / kvh / max_groups;
   // the batch's description is not this launch's predecessor's work: read it before the wait
-  const FewSeq fs = few_seq<NT>(p, seq);
+  const FewSeq fs = few_seq<HD, NT>(p, seq);
   const Kvq8Seq sq = kvq8_seq(p.b, seq);
   const int64_t row = static_cast<int64_t>(rg) * RG + r;
   // every CTA waits before it leaves: a grid that ends early would let the
@@ -683,8 +696,8 @@ __global__ void __launch_bounds__(HD) kvq8_merge_kernel(const __grid_constant__ 
   }
   int64_t before = 0, total = 0;
   for (int s = tid; s < p.b.sequences; s += HD) {
-    const FewSeq f = few_seq<NT>(p, s);
-    const int64_t v = static_cast<int64_t>(f.granules) * f.groups * kvh;
+    const FewSeq f = few_seq<HD, NT>(p, s);
+    const int64_t v = f.cost() * f.groups * kvh;
     total += v;
     if (s < seq) before += v;
   }
@@ -698,7 +711,7 @@ __global__ void __launch_bounds__(HD) kvq8_merge_kernel(const __grid_constant__ 
   before = total = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) before += s_sum[0][w], total += s_sum[1][w];
-  const int64_t lo = before + static_cast<int64_t>(rg * kvh + head) * fs.granules, hi = lo + fs.granules;
+  const int64_t lo = before + (rg * kvh + head) * fs.cost(), hi = lo + fs.cost();
   const int64_t ctas = few_ctas(total, grid_ctas);
   // CTA i holds [total * i / ctas, total * (i + 1) / ctas): the one of granule x
   auto owner = [&](int64_t x) {
@@ -707,7 +720,7 @@ __global__ void __launch_bounds__(HD) kvq8_merge_kernel(const __grid_constant__ 
     while (total * i / ctas > x) --i;
     return static_cast<int>(i);
   };
-  const int c0 = owner(lo), n = owner(hi - 1) - c0 + 1;
+  const int c0 = owner(lo + few_unit_cost(HD)), n = owner(hi - 1) - c0 + 1;
   pdl_wait();
   if (n == 1) return;
   // a CTA's first run is its record 0: the unit's, but where the unit begins inside the CTA
