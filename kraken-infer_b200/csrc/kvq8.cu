@@ -21,12 +21,12 @@ struct Kvq8AppendParams {
   Kvq8Batch b;
   const void *q, *k, *v;
   void* q_out;
-  int heads;
-  int64_t q_stride, k_stride, v_stride, q_out_stride;  // elements between rows
-  const float* inv_freq;  // [pairs]
-  int pairs;              // 0: no rotation
+  int heads, q_share;                                   // query heads; of them, those that go with one KV head's CTA
+  int64_t q_stride, k_stride, v_stride, q_out_stride;   // elements between rows
+  const float* inv_freq;                                // [pairs]
+  int pairs;                                            // 0: no rotation
   int sec0, sec1, sec2, sec_total;
-  const int32_t* positions;  // [4][rows], or null: the cache position
+  const int32_t* positions;                             // [4][rows], or null: the cache position
 };
 
 // The reduction of a page's largest value: a finite |x|; NaN and infinities
@@ -42,165 +42,257 @@ KIB_DEV int quantise(float x, float inv) {
   return x == x ? __float2int_rn(y) : 0;
 }
 
-constexpr int kAppendRows = 8;      // rows of a page per warp, held in registers between the two steps
-constexpr int kAppendMaxPairs = 128;
-
-// One CTA per (run, head, sequence): a run is the new rows of one page.
-// blockIdx.y counts K heads, then V heads, then query heads.  A warp holds
-// whole rows (head_dim / 32 values a lane), kAppendRows of them, so rows are
-// read once: the page's largest value is reduced over the CTA, then the same
-// registers are rounded and stored.  Bound by the bytes of the rows.
+// A CTA takes a span of positions, whole pages (64 positions, or a page of
+// 128), of one sequence: blockIdx.y < kv_heads a K head and its share of the
+// query heads, so that the cosines and sines of the span, made once in shared
+// memory, serve them all; then the V heads.  A row is read in 16-byte pieces
+// by LPR lanes (a warp has 32 / LPR rows at a time); K and V rows stay in
+// registers between the reduction of a page's largest value and the rounding,
+// so every row is read once.  Where the rotated pairs lie a whole number of
+// pieces apart, a lane gets its partners by shuffles.  Bound by the bytes of
+// the rows.
 template <typename T, int HD>
-__global__ void kvq8_append_kernel(const __grid_constant__ Kvq8AppendParams p) {
-  constexpr int V = HD / 32;
+struct AppendShape {
+  static constexpr int E = 16 / static_cast<int>(sizeof(T));    // values of a piece
+  static constexpr int LPR = HD / E < 32 ? HD / E : 32;         // lanes of a row
+  static constexpr int NC = HD / (E * LPR);                     // pieces of a lane
+  static constexpr int RPW = 32 / LPR;                          // rows of a warp at a time
+  static constexpr int ROWS = 8 / RPW;                          // times that to cover a warp's part of a page
+};
+constexpr int kAppendSpan = 64;
+
+template <int E>
+KIB_DEV void store_piece_codes(int8_t* p, const int (&c)[E]) {
+  uint32_t w[E / 4];
+#pragma unroll
+  for (int i = 0; i < E / 4; ++i)
+    w[i] = (c[4 * i] & 255) | (c[4 * i + 1] & 255) << 8 | (c[4 * i + 2] & 255) << 16 | (c[4 * i + 3] & 255) << 24;
+  if constexpr (E == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(512) kvq8_append_kernel(const __grid_constant__ Kvq8AppendParams p) {
+  using Sh = AppendShape<T, HD>;
+  constexpr int E = Sh::E, LPR = Sh::LPR, NC = Sh::NC, RPW = Sh::RPW, ROWS = Sh::ROWS;
+  extern __shared__ __align__(16) float2 s_cs[];  // [rows of the span][pairs]
   __shared__ float s_max[16];
-  __shared__ float2 s_cs[16][kAppendMaxPairs];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int rl = lane / LPR, cl = lane % LPR;
   const int seq = blockIdx.z, kvh = p.c.kv_heads;
   const Kvq8Seq s = kvq8_seq(p.b, seq);
-  const int start = s.length - s.n;  // position of the sequence's first new row
-  const int begin = max(start, 0);
-  const int page_index = (begin >> p.c.page_shift) + static_cast<int>(blockIdx.x);
-  const int base = page_index << p.c.page_shift;
-  const int lo = max(begin, base), hi = min(s.length, base + p.c.page_tokens);
+  const int start = s.length - s.n, begin = max(start, 0);  // positions before 0 have no place
+  const int span = max(kAppendSpan, p.c.page_tokens);
+  const int base = (begin / span + static_cast<int>(blockIdx.x)) * span;
+  // (a row past max_rows, the host's bound and that of s_cs, is left out)
+  const int lo = max(begin, base), hi = min(min(s.length, base + span), lo + p.b.max_rows);
   if (lo >= hi) return;
-  int head = blockIdx.y;
-  const int what = head < kvh ? 0 : (head < 2 * kvh ? 1 : 2);  // K, V, Q
-  head -= what * kvh;
-  const bool rotated = p.pairs > 0 && what != 1;
-  const T* in;
-  int64_t stride;
-  if (what == 0) in = static_cast<const T*>(p.k), stride = p.k_stride;
-  else if (what == 1) in = static_cast<const T*>(p.v), stride = p.v_stride;
-  else in = static_cast<const T*>(p.q), stride = p.q_stride;
-  in += static_cast<int64_t>(head) * HD;
+  const bool is_v = static_cast<int>(blockIdx.y) >= kvh;
+  const int head = static_cast<int>(blockIdx.y) - (is_v ? kvh : 0);
+  const int half = is_v ? 0 : p.pairs;
+  // rotated pairs within the first piece of each lane, a whole number of lanes apart
+  const bool quick = half % E == 0 && 2 * half <= LPR * E;
 
-  float x[kAppendRows][V];
-  const int r0 = lo - base + ((warp - (lo - base)) % warps + warps) % warps;  // this warp's rows: r0, r0 + warps, ..
+  // this warp's page and rows
+  const int wpp = warps * p.c.page_tokens / span, page_base = base + warp / wpp * p.c.page_tokens, wi = warp % wpp;
+  auto row_pos = [&](int i) { return page_base + (i * wpp + wi) * RPW + rl; };
+  const T* in = static_cast<const T*>(is_v ? p.v : p.k) + static_cast<int64_t>(head) * HD + cl * E;
+  const int64_t stride = is_v ? p.v_stride : p.k_stride;
+  float x[ROWS][NC][E];
 #pragma unroll
-  for (int i = 0; i < kAppendRows; ++i) {
-    const int r = r0 + i * warps;
-    if (base + r < hi) load_vec<T, V>(in + (s.first + base + r - start) * stride + lane * V, x[i]);
+  for (int i = 0; i < ROWS; ++i) {
+    const int pos = row_pos(i);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[i][n][e] = 0.0f;
+      if (pos >= lo && pos < hi) load_vec<T, E>(in + (s.first + pos - start) * stride + n * LPR * E, x[i][n]);
+    }
   }
-  if (rotated) {
-    const int half = p.pairs, e0 = lane * V;
-#pragma unroll
-    for (int i = 0; i < kAppendRows; ++i) {
-      const int r = r0 + i * warps;
-      if (base + r >= hi) continue;
-      const int row = s.first + base + r - start;
-      for (int j = lane; j < half; j += 32) {
-        int pos = base + r;
-        if (p.positions) {
-          const int sector = p.sec_total ? j % p.sec_total : 0;
-          const int stream = sector < p.sec0 ? 0 : (sector < p.sec0 + p.sec1 ? 1 : (sector < p.sec0 + p.sec1 + p.sec2 ? 2 : 3));
-          pos = p.positions[static_cast<int64_t>(p.sec_total ? stream : 0) * p.b.rows + row];
-        }
-        float sn, cs;
-        sincosf(__fmul_rn(static_cast<float>(pos), p.inv_freq[j]), &sn, &cs);
-        s_cs[warp][j] = make_float2(cs, sn);
+  if (half) {
+    for (int i = threadIdx.x; i < (hi - lo) * half; i += blockDim.x) {
+      const int r = i / half, j = i - r * half;
+      int pos = lo + r;
+      if (p.positions) {
+        const int sector = p.sec_total ? j % p.sec_total : 0;
+        const int stream = sector < p.sec0 ? 0 : (sector < p.sec0 + p.sec1 ? 1 : (sector < p.sec0 + p.sec1 + p.sec2 ? 2 : 3));
+        pos = p.positions[static_cast<int64_t>(p.sec_total ? stream : 0) * p.b.rows + s.first + pos - start];
       }
-      __syncwarp();
-      const T* xr = in + static_cast<int64_t>(row) * stride;
+      float sn, cs;
+      sincosf(__fmul_rn(static_cast<float>(pos), p.inv_freq[j]), &sn, &cs);
+      s_cs[i] = make_float2(cs, sn);
+    }
+    __syncthreads();
+  }
+  // Rotates the pieces v of the row at `row` (its first value) and position
+  // pos; each product is rounded by itself, as the element-wise form does.
+  // Every lane of the warp takes part.
+  auto rotate = [&](float (&v)[NC][E], const T* row, int pos, bool live) {
+    const float2* cs = s_cs + (pos - lo) * half;
+    if (quick) {
+      const int d = cl * E, off = half / E;
+      const bool upper = d >= half, in_pairs = d < 2 * half;
+      float o[E];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int d = e0 + e;
-        if (d < 2 * half) {
+      for (int e = 0; e < E; ++e) o[e] = __shfl_sync(0xffffffffu, v[0][e], in_pairs ? (upper ? lane - off : lane + off) : lane);
+      if (live && in_pairs) {
+        cs += upper ? d - half : d;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float4 f = *reinterpret_cast<const float4*>(cs + e);
+          const float c2[2] = {f.x, f.z}, s2[2] = {f.y, f.w};
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float a = __fmul_rn(v[0][e + u], c2[u]), b = __fmul_rn(o[e + u], s2[u]);
+            v[0][e + u] = upper ? __fadd_rn(a, b) : __fsub_rn(a, b);
+          }
+        }
+      }
+    } else if (live) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int d = n * LPR * E + cl * E + e;
+          if (d >= 2 * half) continue;
           const bool upper = d >= half;
-          const float2 cs = s_cs[warp][upper ? d - half : d];
-          const float o = to_f32<T>(xr[upper ? d - half : d + half]);
-          // each product rounded by itself, as the element-wise form does
-          x[i][e] = upper ? __fadd_rn(__fmul_rn(x[i][e], cs.x), __fmul_rn(o, cs.y))
-                          : __fsub_rn(__fmul_rn(x[i][e], cs.x), __fmul_rn(o, cs.y));
+          const float2 f = cs[upper ? d - half : d];
+          const float o = to_f32<T>(row[upper ? d - half : d + half]);
+          const float a = __fmul_rn(v[n][e], f.x), b = __fmul_rn(o, f.y);
+          v[n][e] = upper ? __fadd_rn(a, b) : __fsub_rn(a, b);
         }
-      }
-      __syncwarp();
     }
-  }
-  if (what == 2) {
-    T* out = static_cast<T*>(p.q_out) + static_cast<int64_t>(head) * HD;
-    // q_out may be q itself: every lane of a row has read its partner's value
-    // before the row is written (the warp is in step after the rotation)
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kAppendRows; ++i) {
-      const int r = r0 + i * warps;
-      if (base + r < hi) store_vec<T, V>(out + (s.first + base + r - start) * p.q_out_stride + lane * V, x[i]);
-    }
-    return;
-  }
-  const int page = kvq8_page(p.c, p.b, seq, page_index);
-  if (page < 0) return;
+  };
   float big = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kAppendRows; ++i) {
-    if (base + r0 + i * warps < hi) {
+  for (int i = 0; i < ROWS; ++i) {
+    const int pos = row_pos(i);
+    const bool live = pos >= lo && pos < hi;
+    if (half) rotate(x[i], in - cl * E + (s.first + pos - start) * stride, pos, live);
+    if (live) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) big = fmaxf(big, finite_abs(x[i][e]));
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int e = 0; e < E; ++e) big = fmaxf(big, finite_abs(x[i][n][e]));
     }
   }
   big = warp_max(big);
   if (lane == 0) s_max[warp] = big;
-  float* scale = (what == 0 ? p.c.k_scale : p.c.v_scale) + static_cast<int64_t>(page) * kvh + head;
-  // a run that begins at the page's first row takes the page over: its old scale is no longer anyone's
-  const float old = lo > base ? *scale : 0.0f;
   __syncthreads();
-  big = s_max[0];
-  for (int w = 1; w < warps; ++w) big = fmaxf(big, s_max[w]);
-  const float now = fmaxf(old, __fmul_rn(big, 1.0f / 127.0f));
-  if (threadIdx.x == 0) *scale = now;
-  const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f;
-  int8_t* codes = (what == 0 ? p.c.k : p.c.v) + page * p.c.page_stride + head * p.c.head_stride + lane * V;
-  if (now != old || now == 0.0f) {
+  const int first = max(lo, page_base), last = min(hi, page_base + p.c.page_tokens);  // the new rows of this warp's page
+  const int page = first < last ? kvq8_page(p.c, p.b, seq, page_base >> p.c.page_shift) : -1;
+  float* scale = (is_v ? p.c.v_scale : p.c.k_scale) + static_cast<int64_t>(max(page, 0)) * kvh + head;
+  // a page whose first position is new is taken over: its old scale is no longer anyone's
+  const float old = page >= 0 && first > page_base ? *scale : 0.0f;
+  if (page >= 0) {
+    for (int w = warp / wpp * wpp, i = 0; i < wpp; ++i) big = fmaxf(big, s_max[w + i]);
+  }
+  __syncthreads();  // every warp of a page has its old scale before one of them writes the new
+  if (page >= 0) {
+    const float now = fmaxf(old, __fmul_rn(big, 1.0f / 127.0f));
+    if (wi == 0 && lane == 0) *scale = now;
+    const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f;
     const float ratio = now > 0.0f ? __fdiv_rn(old, now) : 0.0f;
-    for (int r = warp; r < lo - base; r += warps) {
-      int c[V];
-      load_codes<V>(codes + r * p.c.token_stride, c);
+    const bool again = now != old || now == 0.0f;
+    int8_t* codes = (is_v ? p.c.v : p.c.k) + page * p.c.page_stride + head * p.c.head_stride + cl * E;
 #pragma unroll
-      for (int e = 0; e < V; ++e) c[e] = __float2int_rn(__fmul_rn(static_cast<float>(c[e]), ratio));
-      store_codes<V>(codes + r * p.c.token_stride, c);
+    for (int i = 0; i < ROWS; ++i) {
+      const int pos = row_pos(i);
+      int8_t* at = codes + (pos - page_base) * p.c.token_stride;
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        int c[E];
+        if (pos >= first && pos < last) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) c[e] = quantise(x[i][n][e], inv);
+          store_piece_codes<E>(at + n * LPR * E, c);
+        } else if (pos < first && again) {
+          // codes that the page already holds move to its grown scale
+          load_codes<E>(at + n * LPR * E, c);
+#pragma unroll
+          for (int e = 0; e < E; ++e) c[e] = __float2int_rn(__fmul_rn(static_cast<float>(c[e]), ratio));
+          store_piece_codes<E>(at + n * LPR * E, c);
+        }
+      }
     }
   }
+  if (is_v || !p.q) return;
+
+  // the query heads of this KV head, four items (row, head) a warp in flight
+  const int h0 = head * p.q_share, share = min(p.heads, h0 + p.q_share) - h0;
+  if (share <= 0) return;
+  const bool in_place = p.q == p.q_out;  // then what is not rotated stays where it is
+  const int items = (hi - lo) * share, step = warps * RPW;
+  constexpr int U = 4;
+#pragma unroll 1
+  for (int i0 = warp * RPW; i0 < items; i0 += U * step) {
+    float y[U][NC][E];
+    int row[U], pos[U], h[U];
+    bool live[U];
 #pragma unroll
-  for (int i = 0; i < kAppendRows; ++i) {
-    const int r = r0 + i * warps;
-    if (base + r < hi) {
-      int c[V];
+    for (int u = 0; u < U; ++u) {
+      const int item = i0 + u * step + rl, r = item / share;
+      live[u] = item < items;
+      pos[u] = lo + r;
+      row[u] = s.first + pos[u] - start;
+      h[u] = h0 + item - r * share;
 #pragma unroll
-      for (int e = 0; e < V; ++e) c[e] = quantise(x[i][e], inv);
-      store_codes<V>(codes + r * p.c.token_stride, c);
+      for (int n = 0; n < NC; ++n) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[u][n][e] = 0.0f;
+        const int d = n * LPR * E + cl * E;
+        if (live[u] && !(in_place && d >= 2 * half))
+          load_vec<T, E>(static_cast<const T*>(p.q) + row[u] * p.q_stride + static_cast<int64_t>(h[u]) * HD + d, y[u][n]);
+      }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (half) rotate(y[u], static_cast<const T*>(p.q) + row[u] * p.q_stride + static_cast<int64_t>(h[u]) * HD, pos[u], live[u]);
+    __syncwarp();  // in place: every lane of a row has its partners' values before the row is written
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const int d = n * LPR * E + cl * E;
+        if (live[u] && !(in_place && d >= 2 * half))
+          store_vec<T, E>(static_cast<T*>(p.q_out) + row[u] * p.q_out_stride + static_cast<int64_t>(h[u]) * HD + d, y[u][n]);
+      }
   }
 }
 
 // ------------------------------------------------------------- read pages
 
-// One warp per row of a page and head; out [count][kv_heads][page_tokens][head_dim].
+// A thread per 16 codes; out [count][kv_heads][page_tokens][head_dim].
 template <typename T, int HD>
-__global__ void kvq8_read_kernel(const __grid_constant__ Kvq8Cache c, const int32_t* ids, int64_t total, T* k_out,
-                                 T* v_out) {
-  constexpr int V = HD / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (row >= total) return;
-  const int t = static_cast<int>(row & (c.page_tokens - 1));
+__global__ void __launch_bounds__(256) kvq8_read_kernel(const __grid_constant__ Kvq8Cache c, const int32_t* ids, int64_t total,
+                                                        T* k_out, T* v_out) {
+  constexpr int CH = HD / 16;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = i / CH;
+  const int ch = static_cast<int>(i % CH), t = static_cast<int>(row & (c.page_tokens - 1));
   const int64_t ph = row >> c.page_shift;
-  const int head = static_cast<int>(ph % c.kv_heads), page = ids[ph / c.kv_heads];
-  const bool ok = page >= 0 && page < c.pages;
-  const int8_t* src = blockIdx.y ? c.v : c.k;
-  T* dst = (blockIdx.y ? v_out : k_out) + row * HD + lane * V;
-  float x[V] = {};
-  if (ok) {
-    int code[V];
-    load_codes<V>(src + page * c.page_stride + head * c.head_stride + t * c.token_stride + lane * V, code);
-    const float s = (blockIdx.y ? c.v_scale : c.k_scale)[static_cast<int64_t>(page) * c.kv_heads + head];
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = static_cast<float>(code[e]) * s;
+  const int64_t at = ph / c.kv_heads;
+  const int head = static_cast<int>(ph - at * c.kv_heads), page = ids[at];
+  T* dst = (blockIdx.y ? v_out : k_out) + i * 16;
+  uint4 w = make_uint4(0u, 0u, 0u, 0u);
+  float s = 0.0f;
+  if (page >= 0 && page < c.pages) {
+    w = *reinterpret_cast<const uint4*>((blockIdx.y ? c.v : c.k) + page * c.page_stride + head * c.head_stride +
+                                        t * c.token_stride + 16 * ch);
+    s = (blockIdx.y ? c.v_scale : c.k_scale)[static_cast<int64_t>(page) * c.kv_heads + head];
   }
-  store_vec<T, V>(dst, x);
+  const uint32_t word[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    float x[8];
+#pragma unroll
+    // 0x4b0000bb is 2^23 + bb; bb = code + 128
+    for (int e = 0; e < 8; ++e)
+      x[e] = (__uint_as_float(__byte_perm(word[2 * j + e / 4], 0x4b000000u, 0x7440u + e % 4)) - 8388736.0f) * s;
+    store_vec<T, 8>(dst + 8 * j, x);
+  }
 }
-
-// --------------------------------------------------------------- attention
 
 // Dynamic shared memory above 48 KB has to be asked for, once per kernel.
 template <typename... KArgs>
@@ -504,13 +596,23 @@ int kib_kvq8_append(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_ba
   p.v = v;
   p.q_out = q_out;
   p.heads = q ? static_cast<int>(heads) : 0;
-  // pages that max_rows consecutive positions can reach
-  const unsigned runs = static_cast<unsigned>((p.b.max_rows - 1 + p.c.page_tokens - 1) / p.c.page_tokens + 1);
-  const dim3 grid(runs, static_cast<unsigned>(2 * p.c.kv_heads + p.heads), static_cast<unsigned>(p.b.sequences));
-  const unsigned threads = static_cast<unsigned>(p.c.page_tokens / kAppendRows * 32);
-#define CALL(T, HD) kvq8_append_kernel<T, HD><<<grid, threads, 0, op_stream(ctx, stream)>>>(p)
+  // spans that max_rows consecutive positions can reach
+  const int span = std::max(kAppendSpan, p.c.page_tokens);
+  const unsigned spans = static_cast<unsigned>((static_cast<int64_t>(p.b.max_rows) + span - 2) / span + 1);
+  p.q_share = (p.heads + p.c.kv_heads - 1) / p.c.kv_heads;
+  const dim3 grid(spans, static_cast<unsigned>(2 * p.c.kv_heads), static_cast<unsigned>(p.b.sequences));
+  const unsigned threads = span == 128 ? 512u : 256u;
+  const size_t smem = static_cast<size_t>(std::min(span, p.b.max_rows)) * p.pairs * sizeof(float2);
+  cudaError_t e = cudaSuccess;
+#define CALL(T, HD)                                                                                \
+  do {                                                                                             \
+    static bool ready = false;                                                                     \
+    e = allow_smem(kvq8_append_kernel<T, HD>, static_cast<size_t>(128) * (HD / 2) * sizeof(float2), &ready); \
+    if (e == cudaSuccess) kvq8_append_kernel<T, HD><<<grid, threads, smem, op_stream(ctx, stream)>>>(p);   \
+  } while (0)
   KVQ8_DISPATCH(type, p.c.head_dim, CALL);
 #undef CALL
+  if (e != cudaSuccess) return check_cuda(ctx, e, "kvq8_append");
   return finish(ctx, stream, "kvq8_append");
 }
 
@@ -523,10 +625,10 @@ int kib_kvq8_read_pages(kib_ctx* ctx, const kib_kvq8_cache* cache, const int32_t
   if (count == 0) return KIB_OK;
   KIB_ARG(page_ids && k_out && v_out, "kvq8_read_pages: null pointer");
   KIB_ARG(aligned(k_out, 16) && aligned(v_out, 16), "kvq8_read_pages: outputs must be 16-byte aligned");
-  KIB_ARG(count < (1ull << 31) / (static_cast<uint64_t>(c.kv_heads) * c.page_tokens / 8),
+  KIB_ARG(count < (1ull << 38) / (static_cast<uint64_t>(c.kv_heads) * c.page_tokens * (c.head_dim / 16)),
           "kvq8_read_pages: count out of range");
-  const int64_t total = static_cast<int64_t>(count) * c.kv_heads * c.page_tokens;
-  const dim3 grid(static_cast<unsigned>((total + 7) / 8), 2);
+  const int64_t total = static_cast<int64_t>(count) * c.kv_heads * c.page_tokens * (c.head_dim / 16);
+  const dim3 grid(static_cast<unsigned>((total + 255) / 256), 2);
 #define CALL(T, HD)                                                                                  \
   kvq8_read_kernel<T, HD><<<grid, 256, 0, op_stream(ctx, stream)>>>(c, page_ids, total, static_cast<T*>(k_out), \
                                                                     static_cast<T*>(v_out))

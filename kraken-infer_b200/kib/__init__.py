@@ -313,13 +313,29 @@ def _stream(s):
     return None if s is None else (int(s) or 1)
 
 
+_dtype_names = {}
+
+
+def _dtype(x) -> str:
+    """"float32" for torch.float32 and the like."""
+    name = _dtype_names.get(x.dtype)
+    if name is None:
+        name = _dtype_names[x.dtype] = str(x.dtype).split(".")[-1]
+    return name
+
+
+_ROW_TYPES = {"float32": TYPE_F32, "float16": TYPE_F16}
+
+
 def _row_type(x):
     """(KIB_TYPE, row stride in elements) of a [rows][heads][head_dim] tensor
     whose heads are packed within a row."""
-    code = {"float32": TYPE_F32, "float16": TYPE_F16}.get(str(x.dtype).split(".")[-1])
+    code = _ROW_TYPES.get(_dtype(x))
     if code is None:
         raise TypeError(f"rows must be float32 or float16, not {x.dtype}")
     rows, heads, hd = x.shape
+    if x.is_contiguous():
+        return code, heads * hd
     st = x.stride()
     if st[2] != 1 or (heads > 1 and st[1] != hd):
         raise ValueError("the heads of a row must be contiguous")
@@ -329,7 +345,7 @@ def _row_type(x):
 def _vector(x, name, dtype, size):
     if x is None:
         return None
-    if str(x.dtype).split(".")[-1] != dtype or not x.is_contiguous() or x.numel() != size:
+    if _dtype(x) != dtype or x.numel() != size or not x.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of {size} values")
     return x.data_ptr()
 
@@ -341,7 +357,7 @@ class KvQ8Cache:
 
     def __init__(self, k, v, k_scale, v_scale):
         for x in (k, v):
-            if str(x.dtype) != "torch.int8" or x.dim() != 4 or x.stride(3) != 1:
+            if _dtype(x) != "int8" or x.dim() != 4 or x.stride(3) != 1:
                 raise ValueError("codes must be int8 [pages][kv_heads][page_tokens][head_dim], the last stride 1")
         if k.shape != v.shape or k.stride() != v.stride():
             raise ValueError("k and v must have the same shape and strides")
@@ -360,13 +376,14 @@ class KvQ8Batch:
 
     def __init__(self, block_table, lengths, row_start, rows, max_rows, max_length=0, total_length=0):
         n = lengths.numel()
-        if block_table.dim() != 2 or block_table.shape[0] != n or str(block_table.dtype) != "torch.int32" or (
+        if block_table.dim() != 2 or block_table.shape[0] != n or _dtype(block_table) != "int32" or (
                 block_table.shape[1] > 1 and block_table.stride(1) != 1):
             raise ValueError("block_table must be int32 [sequences][pages], rows contiguous")
         self.tensors = (block_table, lengths, row_start)
         if n > 1 and block_table.stride(0) != block_table.shape[1]:
             raise ValueError("block_table must be contiguous")
         self.rows = rows
+        self.workspace = {}  # bytes that attention needs, by cache shape, type and heads
         self.c = _KvQ8BatchC(block_table.data_ptr(), _vector(lengths, "lengths", "int32", n),
                              _vector(row_start, "row_start", "int32", n + 1), n, block_table.shape[1], rows, max_rows,
                              max_length, total_length)
@@ -472,7 +489,7 @@ class Context:
     def kvq8_read_pages(self, cache: KvQ8Cache, page_ids, k_out, v_out, stream=None):
         """The values of whole pages, [count][kv_heads][page_tokens][head_dim]."""
         want = (page_ids.numel(),) + tuple(cache.shape[1:])
-        kind = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16}.get(str(k_out.dtype), -1)
+        kind = _ROW_TYPES.get(_dtype(k_out), -1)
         for x in (k_out, v_out):
             if tuple(x.shape) != want or not x.is_contiguous() or x.dtype != k_out.dtype:
                 raise ValueError(f"outputs must be contiguous {want} of one type")
@@ -481,10 +498,15 @@ class Context:
 
     def kvq8_attention_workspace(self, cache: KvQ8Cache, batch: KvQ8Batch, q) -> int:
         """Bytes of workspace that kvq8_attention needs for these arguments."""
-        need = c_uint64()
-        self.check(self.lib.kib_kvq8_attention_workspace(self.h, byref(cache.c), byref(batch.c), _row_type(q)[0],
-                                                         q.shape[1], byref(need)))
-        return need.value
+        return self._kvq8_need(cache, batch, _row_type(q)[0], q.shape[1])
+
+    def _kvq8_need(self, cache, batch, kind, heads):
+        key = (cache.shape, kind, heads)
+        if key not in batch.workspace:
+            need = c_uint64()
+            self.check(self.lib.kib_kvq8_attention_workspace(self.h, byref(cache.c), byref(batch.c), kind, heads, byref(need)))
+            batch.workspace[key] = need.value
+        return batch.workspace[key]
 
     def kvq8_attention(self, cache: KvQ8Cache, batch: KvQ8Batch, q, out, scale, workspace=None, stream=None):
         """Causal attention of q [rows][heads][head_dim] over the cache.
@@ -492,10 +514,11 @@ class Context:
         that this context keeps and grows (then calls must not overlap)."""
         kind, qs = _row_type(q)
         okind, os_ = _row_type(out)
-        if okind != kind or q.shape != out.shape or q.shape[0] != batch.rows or q.shape[2] != cache.shape[3]:
+        shape = q.shape
+        if okind != kind or shape != out.shape or shape[0] != batch.rows or shape[2] != cache.shape[3]:
             raise ValueError("q and out must be [rows][heads][head_dim] of one type")
         if workspace is None:
-            need = self.kvq8_attention_workspace(cache, batch, q)
+            need = self._kvq8_need(cache, batch, kind, shape[1])
             if need > self._workspace[1]:
                 old, self._workspace = self._workspace[0], (None, 0)
                 if old:
@@ -506,15 +529,15 @@ class Context:
             where, size = self._workspace
         else:
             where, size = ptr(workspace), workspace.numel() * workspace.element_size()
-        self.check(self.lib.kib_kvq8_attention(self.h, byref(cache.c), byref(batch.c), kind, q.shape[1], ptr(q), qs,
-                                               scale, ptr(out), os_, where, size, _stream(stream)))
+        self.check(self.lib.kib_kvq8_attention(self.h, byref(cache.c), byref(batch.c), kind, shape[1], q.data_ptr(), qs,
+                                               scale, out.data_ptr(), os_, where, size, _stream(stream)))
 
     def sample(self, logits, uniform, token_out, prob_out=None, temperature=None, top_k=None, top_p=None, min_p=None,
                stream=None):
         """A token per row of logits [rows][vocab] (float32, last stride 1);
         the per-row tensors as in kib_sample_f32, None for the default."""
         rows, vocab = logits.shape
-        if str(logits.dtype) != "torch.float32" or (vocab > 1 and logits.stride(1) != 1):
+        if _dtype(logits) != "float32" or (vocab > 1 and logits.stride(1) != 1):
             raise ValueError("logits must be float32 [rows][vocab], the last stride 1")
         self.check(self.lib.kib_sample_f32(self.h, ptr(logits), rows, vocab, logits.stride(0) if rows > 1 else 0,
                                            _vector(uniform, "uniform", "float32", rows),
