@@ -21,7 +21,7 @@ struct Kvq8AppendParams {
   Kvq8Batch b;
   const void *q, *k, *v;
   void* q_out;
-  int heads, q_share;                                   // query heads; of them, those that go with one KV head's CTA
+  int heads, q_parts;                                   // query heads; CTAs that share them
   int64_t q_stride, k_stride, v_stride, q_out_stride;   // elements between rows
   const float* inv_freq;                                // [pairs]
   int pairs;                                            // 0: no rotation
@@ -43,9 +43,8 @@ KIB_DEV int quantise(float x, float inv) {
 }
 
 // A CTA takes a span of positions, whole pages (64 positions, or a page of
-// 128), of one sequence: blockIdx.y < kv_heads a K head and its share of the
-// query heads, so that the cosines and sines of the span, made once in shared
-// memory, serve them all; then the V heads.  A row is read in 16-byte pieces
+// 128), of one sequence and one K head, one V head or kAppendQ query heads,
+// for which the cosines and sines of the span are made once in shared memory.  A row is read in 16-byte pieces
 // by LPR lanes (a warp has 32 / LPR rows at a time); K and V rows stay in
 // registers between the reduction of a page's largest value and the rounding,
 // so every row is read once.  Where the rotated pairs lie a whole number of
@@ -58,8 +57,13 @@ struct AppendShape {
   static constexpr int NC = HD / (E * LPR);                     // pieces of a lane
   static constexpr int RPW = 32 / LPR;                          // rows of a warp at a time
   static constexpr int ROWS = 8 / RPW;                          // times that to cover a warp's part of a page
+  static constexpr int HELD = ROWS * NC * E;                    // values that a thread holds
+  static constexpr int U = HELD >= 64 ? 4 : 2;                  // query rows a lane has in flight
+  // small rows leave registers for four CTAs of 256 threads: such calls are bound by latency
+  static constexpr int MINB = HELD >= 64 ? 1 : 2;               // of 512 threads
 };
 constexpr int kAppendSpan = 64;
+constexpr int kAppendQ = 4;
 
 template <int E>
 KIB_DEV void store_piece_codes(int8_t* p, const int (&c)[E]) {
@@ -72,7 +76,7 @@ KIB_DEV void store_piece_codes(int8_t* p, const int (&c)[E]) {
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(512) kvq8_append_kernel(const __grid_constant__ Kvq8AppendParams p) {
+__global__ void __launch_bounds__(512, AppendShape<T, HD>::MINB) kvq8_append_kernel(const __grid_constant__ Kvq8AppendParams p) {
   using Sh = AppendShape<T, HD>;
   constexpr int E = Sh::E, LPR = Sh::LPR, NC = Sh::NC, RPW = Sh::RPW, ROWS = Sh::ROWS;
   extern __shared__ __align__(16) float2 s_cs[];  // [rows of the span][pairs]
@@ -87,8 +91,9 @@ __global__ void __launch_bounds__(512) kvq8_append_kernel(const __grid_constant_
   // (a row past max_rows, the host's bound and that of s_cs, is left out)
   const int lo = max(begin, base), hi = min(min(s.length, base + span), lo + p.b.max_rows);
   if (lo >= hi) return;
-  const bool is_v = static_cast<int>(blockIdx.y) >= kvh;
-  const int head = static_cast<int>(blockIdx.y) - (is_v ? kvh : 0);
+  const int part = blockIdx.y;  // query heads, K heads, V heads
+  const bool is_q = part < p.q_parts, is_v = part >= p.q_parts + kvh;
+  const int head = part - (is_q ? 0 : p.q_parts + (is_v ? kvh : 0));
   const int half = is_v ? 0 : p.pairs;
   // rotated pairs within the first piece of each lane, a whole number of lanes apart
   const bool quick = half % E == 0 && 2 * half <= LPR * E;
@@ -106,21 +111,30 @@ __global__ void __launch_bounds__(512) kvq8_append_kernel(const __grid_constant_
     for (int n = 0; n < NC; ++n) {
 #pragma unroll
       for (int e = 0; e < E; ++e) x[i][n][e] = 0.0f;
-      if (pos >= lo && pos < hi) load_vec<T, E>(in + (s.first + pos - start) * stride + n * LPR * E, x[i][n]);
+      if (!is_q && pos >= lo && pos < hi) load_vec<T, E>(in + (s.first + pos - start) * stride + n * LPR * E, x[i][n]);
     }
   }
+  // the new rows of this warp's page, and its scale: all warps read it before the barrier that the writer passes
+  const int first = max(lo, page_base), last = min(hi, page_base + p.c.page_tokens);
+  const int page = !is_q && first < last ? kvq8_page(p.c, p.b, seq, page_base >> p.c.page_shift) : -1;
+  float* scale = (is_v ? p.c.v_scale : p.c.k_scale) + static_cast<int64_t>(max(page, 0)) * kvh + (is_q ? 0 : head);
+  // a page whose first position is new is taken over: its old scale is no longer anyone's
+  const float old = page >= 0 && first > page_base ? *scale : 0.0f;
   if (half) {
-    for (int i = threadIdx.x; i < (hi - lo) * half; i += blockDim.x) {
-      const int r = i / half, j = i - r * half;
-      int pos = lo + r;
-      if (p.positions) {
-        const int sector = p.sec_total ? j % p.sec_total : 0;
-        const int stream = sector < p.sec0 ? 0 : (sector < p.sec0 + p.sec1 ? 1 : (sector < p.sec0 + p.sec1 + p.sec2 ? 2 : 3));
-        pos = p.positions[static_cast<int64_t>(p.sec_total ? stream : 0) * p.b.rows + s.first + pos - start];
-      }
+    // a thread keeps its pair and goes down the rows
+    const int rows = static_cast<int>(blockDim.x) / half, j = static_cast<int>(threadIdx.x) % half;
+    int stream = 0;
+    if (p.positions && p.sec_total) {
+      const int sector = j % p.sec_total;
+      stream = sector < p.sec0 ? 0 : (sector < p.sec0 + p.sec1 ? 1 : (sector < p.sec0 + p.sec1 + p.sec2 ? 2 : 3));
+    }
+    const float freq = p.inv_freq[j];
+    const int32_t* given = p.positions ? p.positions + static_cast<int64_t>(stream) * p.b.rows + s.first - start : nullptr;
+    for (int r = static_cast<int>(threadIdx.x) / half; r < hi - lo && static_cast<int>(threadIdx.x) < rows * half; r += rows) {
+      const int pos = given ? given[lo + r] : lo + r;
       float sn, cs;
-      sincosf(__fmul_rn(static_cast<float>(pos), p.inv_freq[j]), &sn, &cs);
-      s_cs[i] = make_float2(cs, sn);
+      sincosf(__fmul_rn(static_cast<float>(pos), freq), &sn, &cs);
+      s_cs[r * half + j] = make_float2(cs, sn);
     }
     __syncthreads();
   }
@@ -163,6 +177,48 @@ __global__ void __launch_bounds__(512) kvq8_append_kernel(const __grid_constant_
         }
     }
   };
+  if (is_q) {
+    // query heads, U items (row, head) a lane in flight
+    const int h0 = head * kAppendQ, share = min(kAppendQ, p.heads - h0);
+    const bool in_place = p.q == p.q_out;  // then what is not rotated stays where it is
+    const int items = (hi - lo) * share, step = warps * RPW;
+    constexpr int U = Sh::U;
+#pragma unroll 1
+    for (int i0 = warp * RPW; i0 < items; i0 += U * step) {
+      float y[U][NC][E];
+      int row[U], pos[U], h[U];
+      bool live[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int item = i0 + u * step + rl, r = item / share;
+        live[u] = item < items;
+        pos[u] = lo + r;
+        row[u] = s.first + pos[u] - start;
+        h[u] = h0 + item - r * share;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) y[u][n][e] = 0.0f;
+          const int d = n * LPR * E + cl * E;
+          if (live[u] && !(in_place && d >= 2 * half))
+            load_vec<T, E>(static_cast<const T*>(p.q) + row[u] * p.q_stride + static_cast<int64_t>(h[u]) * HD + d, y[u][n]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (half) rotate(y[u], static_cast<const T*>(p.q) + row[u] * p.q_stride + static_cast<int64_t>(h[u]) * HD, pos[u], live[u]);
+      __syncwarp();  // in place: every lane of a row has its partners' values before the row is written
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+          const int d = n * LPR * E + cl * E;
+          if (live[u] && !(in_place && d >= 2 * half))
+            store_vec<T, E>(static_cast<T*>(p.q_out) + row[u] * p.q_out_stride + static_cast<int64_t>(h[u]) * HD + d, y[u][n]);
+        }
+    }
+    return;
+  }
   float big = 0.0f;
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
@@ -179,15 +235,9 @@ __global__ void __launch_bounds__(512) kvq8_append_kernel(const __grid_constant_
   big = warp_max(big);
   if (lane == 0) s_max[warp] = big;
   __syncthreads();
-  const int first = max(lo, page_base), last = min(hi, page_base + p.c.page_tokens);  // the new rows of this warp's page
-  const int page = first < last ? kvq8_page(p.c, p.b, seq, page_base >> p.c.page_shift) : -1;
-  float* scale = (is_v ? p.c.v_scale : p.c.k_scale) + static_cast<int64_t>(max(page, 0)) * kvh + head;
-  // a page whose first position is new is taken over: its old scale is no longer anyone's
-  const float old = page >= 0 && first > page_base ? *scale : 0.0f;
   if (page >= 0) {
     for (int w = warp / wpp * wpp, i = 0; i < wpp; ++i) big = fmaxf(big, s_max[w + i]);
   }
-  __syncthreads();  // every warp of a page has its old scale before one of them writes the new
   if (page >= 0) {
     const float now = fmaxf(old, __fmul_rn(big, 1.0f / 127.0f));
     if (wi == 0 && lane == 0) *scale = now;
@@ -215,48 +265,6 @@ __global__ void __launch_bounds__(512) kvq8_append_kernel(const __grid_constant_
         }
       }
     }
-  }
-  if (is_v || !p.q) return;
-
-  // the query heads of this KV head, four items (row, head) a warp in flight
-  const int h0 = head * p.q_share, share = min(p.heads, h0 + p.q_share) - h0;
-  if (share <= 0) return;
-  const bool in_place = p.q == p.q_out;  // then what is not rotated stays where it is
-  const int items = (hi - lo) * share, step = warps * RPW;
-  constexpr int U = 4;
-#pragma unroll 1
-  for (int i0 = warp * RPW; i0 < items; i0 += U * step) {
-    float y[U][NC][E];
-    int row[U], pos[U], h[U];
-    bool live[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int item = i0 + u * step + rl, r = item / share;
-      live[u] = item < items;
-      pos[u] = lo + r;
-      row[u] = s.first + pos[u] - start;
-      h[u] = h0 + item - r * share;
-#pragma unroll
-      for (int n = 0; n < NC; ++n) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) y[u][n][e] = 0.0f;
-        const int d = n * LPR * E + cl * E;
-        if (live[u] && !(in_place && d >= 2 * half))
-          load_vec<T, E>(static_cast<const T*>(p.q) + row[u] * p.q_stride + static_cast<int64_t>(h[u]) * HD + d, y[u][n]);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (half) rotate(y[u], static_cast<const T*>(p.q) + row[u] * p.q_stride + static_cast<int64_t>(h[u]) * HD, pos[u], live[u]);
-    __syncwarp();  // in place: every lane of a row has its partners' values before the row is written
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        const int d = n * LPR * E + cl * E;
-        if (live[u] && !(in_place && d >= 2 * half))
-          store_vec<T, E>(static_cast<T*>(p.q_out) + row[u] * p.q_out_stride + static_cast<int64_t>(h[u]) * HD + d, y[u][n]);
-      }
   }
 }
 
@@ -599,8 +607,8 @@ int kib_kvq8_append(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_ba
   // spans that max_rows consecutive positions can reach
   const int span = std::max(kAppendSpan, p.c.page_tokens);
   const unsigned spans = static_cast<unsigned>((static_cast<int64_t>(p.b.max_rows) + span - 2) / span + 1);
-  p.q_share = (p.heads + p.c.kv_heads - 1) / p.c.kv_heads;
-  const dim3 grid(spans, static_cast<unsigned>(2 * p.c.kv_heads), static_cast<unsigned>(p.b.sequences));
+  p.q_parts = (p.heads + kAppendQ - 1) / kAppendQ;
+  const dim3 grid(spans, static_cast<unsigned>(p.q_parts + 2 * p.c.kv_heads), static_cast<unsigned>(p.b.sequences));
   const unsigned threads = span == 128 ? 512u : 256u;
   const size_t smem = static_cast<size_t>(std::min(span, p.b.max_rows)) * p.pairs * sizeof(float2);
   cudaError_t e = cudaSuccess;
