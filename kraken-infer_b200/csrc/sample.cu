@@ -11,6 +11,7 @@
 // running weight exceeds trunc(u * total of the kept).  NaN logits count as
 // -infinity.
 #include <string>
+#include <type_traits>
 
 #include <cooperative_groups.h>
 
@@ -249,43 +250,56 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(const __grid
 //
 // A cluster of C CTAs takes one row: each CTA keeps its slice of the logits in
 // shared memory, so the row is read from HBM once.  One pass turns the logits
-// into e_i; every later pass runs on those.
-//
-// Cuts are found by histograms of kBins bins over the bits of e, which are
-// ordered like e and near-uniform in log e (16 bins an octave, so a vocabulary
-// spreads over hundreds of bins; atomics on one word run one after another).
-// Counts take one 32-bit shared atomic a logit, masses the non-zero ones of
-// three (14 + 14 + 13 bits: a slice of 2^14 logits cannot overflow a word).
-// The tokens of the bin with the boundary go to a list, on which further
-// histograms narrow the bin to one value of e.  Where a cut falls inside a
-// group of equal e, the group is ordered by its logits (different logits may
-// round to one e), then by index.  The CTAs add up their histograms over
-// distributed shared memory: each adds its non-zero bins to share b / (kBins / C)
-// of CTA r by remote 64-bit atomics (integers: in any order the same), then
-// everyone gathers the shares and scans them redundantly, one cluster barrier
-// a histogram.  Three copies of a share take turns: a copy is cleared behind
-// the barrier after the one it was gathered behind, a barrier before its next
-// use.
+// into e_i and, where a cut is wanted, into a histogram of kBins bins over the
+// bits of e (32 bins an octave: ordered like e, near-uniform in log e, so a
+// vocabulary spreads over hundreds of bins; atomics on one word run one after
+// another).  A bin takes two 32-bit shared atomics a logit, its count and the
+// sum of the 18 low bits that the bin leaves open: both cuts, and the exact
+// mass, follow from them (a slice of 2^14 logits cannot overflow the sum).
+// The tokens of the bin with the boundary go to a list, on which two
+// histograms of nine bits each narrow the bin to one value of e.  Where a cut
+// falls inside a group of equal e, the group is ordered by its logits
+// (different logits may round to one e), then by index.  The CTAs add up their
+// histograms over distributed shared memory: each adds its non-zero bins to
+// share b / (bins / C) of CTA r by remote atomics (integers: in any order the
+// same), then everyone gathers the shares and scans them redundantly, one
+// cluster barrier a histogram.  Three copies of the small histogram's share
+// take turns: a copy is cleared behind the barrier after the one it was
+// gathered behind, a barrier before its next use.
 
 constexpr int kSliceMax = 16384;
 constexpr int kClusterMax = 16;
 constexpr int kClThreads = 512;
-constexpr int kBins = 1024;
-constexpr int kBinShift = 19;  // of the bits of e: 16 bins an octave, 40 octaves
+constexpr int kBins = 1536;     // 32 an octave: from bin 1281 on e < 2^-40, without weight
+constexpr int kBinShift = 18;   // of the bits of e
+constexpr int kWeighty = 1281;
+constexpr int kFine = 512;      // bins of the histograms on the list
 constexpr int kListMax = 2048;
 constexpr uint32_t kOneBits = 0x3f800000u;
 
 struct ClusterShared {
-  uint32_t hist[3][kBins];
-  u64 sums[kBins];  // the cluster's bins, gathered
+  uint32_t cnt[kBins], low[kBins];      // this CTA's histogram
+  uint32_t fcnt[kFine], flow[kFine];    // and the small one
+  u64 table[kSliceMax / 128];
   u64 scan[kClThreads / 32];
   uint16_t list[kListMax];
-  u64 total;
-  u64 before;
+  u64 total, before, here;
   float top;
   int first, bin, index, listed;
   uint32_t kmin, kmax;
 };
+
+// Weight of a value of e from its bits, and of a bin from its count and the
+// (likewise shifted) sum of the bits below `open`: trunc(2^40 e) shifts the
+// significand by an amount that is one for a whole bin.
+KIB_DEV int low_shift(uint32_t bits) { return max(0, 110 - static_cast<int>(bits >> 23)); }
+KIB_DEV u64 bin_mass(uint32_t top_bits, uint32_t count, uint32_t low) {
+  if (!count) return 0;
+  const int shift = static_cast<int>(top_bits >> 23) - 110;
+  const u64 m = (top_bits & 0x7fffffu) | 0x800000u;
+  if (shift >= 0) return (m * count + low) << shift;
+  return shift > -24 ? (m >> -shift) * count + low : 0u;
+}
 
 template <typename T>
 KIB_DEV T* peer(cg::cluster_group& cl, T* p, unsigned rank) {
@@ -317,7 +331,8 @@ KIB_DEV u64 block_scan(u64 v, u64* s, u64* total) {
 __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __grid_constant__ SampleParams p, int slice) {
   extern __shared__ __align__(16) float xs[];  // the slice's logits, then its e; padded with weightless tokens
   float4* x4 = reinterpret_cast<float4*>(xs);
-  u64* shares = reinterpret_cast<u64*>(xs + slice);  // [3][kBins / C]
+  // shares of the histograms: masses and counts by bin, then three copies of the small one's
+  u64* share_mass = reinterpret_cast<u64*>(xs + slice);  // [kBins / C]
   __shared__ ClusterShared sh;
   cg::cluster_group cl = cg::this_cluster();
   const unsigned C = cl.num_blocks(), rank = cl.block_rank();
@@ -331,7 +346,9 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   const float min_p0 = p.min_p ? __ldg(p.min_p + row) : 0.0f;
   const float min_p = min_p0 > 0.0f ? fminf(min_p0, 1.0f) : 0.0f;
   const float u = __ldg(p.uniform + row), inv_t = __fdiv_rn(1.0f, t);
-  const int n4 = slice / 4, per = kBins / static_cast<int>(C);
+  const int n4 = slice / 4, per = kBins / static_cast<int>(C), fper = kFine / static_cast<int>(C);
+  u64* share_fine = share_mass + per;                                     // [3][kFine / C]
+  uint32_t* share_cnt = reinterpret_cast<uint32_t*>(share_fine + 3 * fper);  // [kBins / C]
 
   // the slice, cleaned, and its maximum
   float top = -INFINITY;
@@ -351,12 +368,14 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
       top = fmaxf(top, l);
     }
   }
-  for (int j = tid; j < 3 * per; j += kClThreads) shares[j] = 0;
+  for (int j = tid; j < per; j += kClThreads) share_mass[j] = 0, share_cnt[j] = 0;
+  for (int j = tid; j < 3 * fper; j += kClThreads) share_fine[j] = 0;
   top = warp_max(top);
   float* fs = reinterpret_cast<float*>(sh.scan);
   if (lane == 0) fs[warp] = top;
   if (tid == 0) sh.first = 0x7fffffff;
-  for (int b = tid; b < 3 * kBins; b += kClThreads) (&sh.hist[0][0])[b] = 0;
+  for (int b = tid; b < kBins; b += kClThreads) sh.cnt[b] = sh.low[b] = 0;
+  if (tid < kFine) sh.fcnt[tid] = sh.flow[tid] = 0;
   __syncthreads();
   if (tid == 0) {
     for (int w = 1; w < kClThreads / 32; ++w) top = fmaxf(top, fs[w]);
@@ -386,28 +405,30 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   const RowScale rs{top, inv_t};
   const bool by_k = k > 0 && k < p.vocab, by_p = !(top_p >= 1.0f);
 
+  auto owner_of = [&](int b) { return static_cast<unsigned>(b) * C / kBins; };  // of a bin's share
   auto e_bits = [&](int i) { return __float_as_uint(xs[i]); };
   auto logit_key = [&](int i) { return order_key(i < n ? clean_logit(__ldg(x + i)) : -INFINITY); };
-  auto e_bin = [](uint32_t bits) { return static_cast<int>(min((kOneBits - bits) >> kBinShift, kBins - 1u)); };
-  auto add_mass = [&](int b, u64 w) {
-    const uint32_t w0 = static_cast<uint32_t>(w) & 0x3fffu, w1 = static_cast<uint32_t>(w >> 14) & 0x3fffu,
-                   w2 = static_cast<uint32_t>(w >> 28);
-    if (w0) atomicAdd(&sh.hist[0][b], w0);
-    if (w1) atomicAdd(&sh.hist[1][b], w1);
-    if (w2) atomicAdd(&sh.hist[2][b], w2);
-  };
+  auto e_bin = [](uint32_t bits) { return min(static_cast<int>(kOneBits >> kBinShift) - static_cast<int>(bits >> kBinShift), kBins - 1); };
+  auto bin_bits = [](int bin) { return ((kOneBits >> kBinShift) - static_cast<uint32_t>(bin)) << kBinShift; };  // its smallest
 
-  // logits to weights, with the first histogram on the way
+  // logits to weights: with the histogram on the way, or (no cut to find) the sum of the kept
+  const uint32_t min_bits = __float_as_uint(min_p);
+  u64 kept_mass = 0;
   for (int i = tid; i < n4; i += kClThreads) {
     const float4 l = x4[i];
     const float e[4] = {logit_weight(l.x, rs), logit_weight(l.y, rs), logit_weight(l.z, rs), logit_weight(l.w, rs)};
     x4[i] = make_float4(e[0], e[1], e[2], e[3]);
-    if (by_k) {
+    if (by_k || by_p) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) atomicAdd(&sh.hist[0][e_bin(__float_as_uint(e[j]))], 1u);
-    } else if (by_p) {
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t b = __float_as_uint(e[j]);
+        const int bin = e_bin(b);
+        atomicAdd(&sh.cnt[bin], 1u);
+        atomicAdd(&sh.low[bin], (b & ((1u << kBinShift) - 1)) >> min(low_shift(b), 31));
+      }
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) add_mass(e_bin(__float_as_uint(e[j])), fixed_weight(e[j]));
+      for (int j = 0; j < 4; ++j) kept_mass += __float_as_uint(e[j]) >= min_bits ? fixed_weight(e[j]) : 0;
     }
   }
 
@@ -425,47 +446,49 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     return key > cut.key || (key == cut.key && i0 + i <= cut.last);
   };
 
-  // The cluster's sums of the histogram (of counts or of masses) in sh.sums;
-  // the bin at which they reach want_of(their total), with what lies before it.
-  int turn = 0;
-  auto find_bin = [&](bool masses, u64 before, auto want_of, u64* want, u64* here) -> int {
-    u64* mine_at = shares + turn * per;
-    turn = turn == 2 ? 0 : turn + 1;
-    __syncthreads();
-    for (int b = tid; b < kBins; b += kClThreads) {
-      u64 v = sh.hist[0][b];
-      sh.hist[0][b] = 0;  // for the next histogram
-      if (masses) {
-        v += (static_cast<u64>(sh.hist[1][b]) << 14) + (static_cast<u64>(sh.hist[2][b]) << 28);
-        sh.hist[1][b] = sh.hist[2][b] = 0;
-      }
-      if (v) atomicAdd(peer(cl, mine_at + b % per, static_cast<unsigned>(b / per)), v);
-    }
-    cl.sync();
-    // the copy of the histogram before last has been gathered by everyone
-    for (int j = tid; j < per; j += kClThreads) shares[(turn == 2 ? 0 : turn + 1) * per + j] = 0;
-    constexpr int PER = kBins / kClThreads;
-    u64 v[PER], mine = 0, total = 0;
+  // Of the values that a thread holds, in scan order over the threads: sets
+  // sh.bin, sh.before, sh.here where the running sum (from `before`) reaches want.
+  auto find = [&](const u64* v, auto per_thread, u64 before, u64 acc, u64 want) {
+    constexpr int PER = decltype(per_thread)::value;
+    acc += before;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const int b = tid * PER + e;
-      v[e] = *peer(cl, mine_at + b % per, static_cast<unsigned>(b / per));
-      mine += v[e];
-    }
-    if (tid == 0) sh.bin = kBins - 1, sh.before = before;
-    u64 acc = before + block_scan(mine, sh.scan, &total);
-    *want = want_of(total);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      sh.sums[tid * PER + e] = v[e];
-      if (acc < *want && *want <= acc + v[e]) sh.bin = tid * PER + e, sh.before = acc;
+      if (acc < want && want <= acc + v[e]) sh.bin = tid * PER + e, sh.before = acc, sh.here = v[e];
       acc += v[e];
     }
     __syncthreads();
-    *here = sh.sums[sh.bin];
-    return sh.bin;
   };
-  // The listed tokens, or all that `member` holds of where the list is too short.
+  // The cluster's sums of the small histogram, scanned for `want`; the bin (in
+  // descending order), with what lies before it and in it.
+  int turn = 0;
+  auto find_fine = [&](bool masses, uint32_t top_bits, int open, u64* before, u64* here, u64 want) -> int {
+    u64* mine_at = share_fine + turn * fper;
+    turn = turn == 2 ? 0 : turn + 1;
+    __syncthreads();
+    {
+      const uint32_t count = sh.fcnt[tid];
+      u64 v = count;
+      if (masses) v = bin_mass(top_bits | static_cast<uint32_t>(kFine - 1 - tid) << open, count, sh.flow[tid]);
+      sh.fcnt[tid] = sh.flow[tid] = 0;  // for the next
+      if (v) atomicAdd(peer(cl, mine_at + (tid & (fper - 1)), tid * C / kFine), v);
+    }
+    cl.sync();
+    // the copy before last has been gathered by everyone
+    for (int j = tid; j < fper; j += kClThreads) share_fine[(turn == 2 ? 0 : turn + 1) * fper + j] = 0;
+    const u64 v = *peer(cl, mine_at + (tid & (fper - 1)), tid * C / kFine);
+    if (tid == 0) sh.bin = kFine - 1, sh.before = *before, sh.here = 0;
+    u64 total;
+    const u64 acc = block_scan(v, sh.scan, &total);
+    find(&v, std::integral_constant<int, 1>{}, *before, acc, want);
+    *before = sh.before;
+    *here = sh.here;
+    const int bin = sh.bin;
+    __syncthreads();  // sh.bin is written again
+    return bin;
+  };
+  static_assert(kFine == kClThreads, "one bin of the small histogram a thread");
+  // The tokens with bits of e in [klo, khi] that `member` lets through, listed;
+  // or gone through again and again where the list is too short.
   bool short_list = false;
   auto make_list = [&](uint32_t klo, uint32_t khi, auto member) {
     if (tid == 0) sh.listed = 0;
@@ -483,47 +506,35 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     __syncthreads();
     short_list = sh.listed <= kListMax;
   };
-  auto for_list = [&](auto member, auto what) {
+  auto for_list = [&](uint32_t klo, uint32_t khi, auto member, auto what) {
     if (short_list) {
-      for (int j = tid; j < sh.listed; j += kClThreads) what(sh.list[j]);
+      for (int j = tid; j < sh.listed; j += kClThreads) what(static_cast<int>(sh.list[j]));
     } else {
-      for (int i = tid; i < slice; i += kClThreads)
-        if (member(i)) what(i);
+      for (int i = tid; i < slice; i += kClThreads) {
+        const uint32_t b = e_bits(i);
+        if (b >= klo && b <= khi && member(i)) what(i);
+      }
     }
   };
-  // Narrows [klo, khi] to the value at which the running sum (from `before`,
-  // values in descending order) reaches want.
-  auto narrow = [&](bool masses, auto member, auto value, uint32_t klo, uint32_t khi, u64 want, u64* before, u64* here) -> uint32_t {
-    for (int level = 0; klo < khi && level < 8; ++level) {  // five at most: 2^32 values, 2^10 a level
-      const int shift = max(0, 22 - __clz(khi - klo));
-      for_list(member, [&](int i) {
-        const uint32_t v = value(i);
-        if (v < klo || v > khi) return;
-        const int b = static_cast<int>((khi - v) >> shift);
-        if (masses) add_mass(b, fixed_weight(xs[i]));
-        else atomicAdd(&sh.hist[0][b], 1u);
-      });
-      u64 w;
-      const int bin = find_bin(masses, *before, [&](u64) { return want; }, &w, here);
-      *before = sh.before;
-      const uint32_t h = khi - (static_cast<uint32_t>(bin) << shift), size = 1u << shift;
-      klo = h - klo >= size - 1 ? h - (size - 1) : klo;
-      khi = h;
-      __syncthreads();  // sh.bin is written again
-    }
-    return klo;
+  // The block's sum, then the cluster's, of a value of each thread.
+  auto cluster_sum = [&](u64 v) -> u64 {
+    u64 all;
+    block_scan(v, sh.scan, &all);
+    if (tid == 0) sh.total = all;
+    cl.sync();
+    u64 sum = lane < static_cast<int>(C) ? *peer(cl, &sh.total, lane) : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
   };
 
   // Weights summed in index order: the token (relative to the slice) at which
   // the running sum exceeds aim(total), in the CTA that holds it (-1 in the
   // others); *owner is that CTA's rank.
-  auto locate = [&](auto weight, auto aim_of, unsigned* owner, u64* total) -> int {
+  // `mine`: this thread's part of the CTA's sum.
+  auto locate = [&](u64 mine, auto weight, auto aim_of, unsigned* owner, u64* total) -> int {
     // weight(q, w): the weights of tokens 4 q .. 4 q + 3
-    u64 mine = 0, all = 0, w[4];
-    for (int q = tid; q < n4; q += kClThreads) {
-      weight(q, w);
-      mine += (w[0] + w[1]) + (w[2] + w[3]);
-    }
+    u64 all = 0, w[4];
     block_scan(mine, sh.scan, &all);
     if (tid == 0) sh.total = all;
     cl.sync();
@@ -550,11 +561,11 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) sh.sums[j * W + warp] = v;
+      if (lane == 0) sh.table[j * W + warp] = v;
     }
     if (tid == 0) sh.bin = 0, sh.before = base;
     __syncthreads();
-    const u64 v = tid < rounds * W ? sh.sums[tid] : 0;
+    const u64 v = tid < rounds * W ? sh.table[tid] : 0;
     const u64 acc = base + block_scan(v, sh.scan, &all);
     if (acc <= aim && aim < acc + v) sh.bin = tid, sh.before = acc;
     __syncthreads();
@@ -579,32 +590,38 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     return __shfl_sync(0xffffffffu, at, max(__ffs(past) - 1, 0));
   };
 
-  // Cuts at the running sum `want_of(total)` of the histogram that is ready in shared memory.
-  auto select = [&](bool masses, auto want_of) {
-    u64 want, here;
-    const int bin = find_bin(masses, 0, want_of, &want, &here);
-    u64 before = sh.before;
-    const uint32_t khi = kOneBits - (static_cast<uint32_t>(bin) << kBinShift);
-    const uint32_t klo = bin == kBins - 1 ? 0u : khi - ((1u << kBinShift) - 1);
-    auto member = [&](int i) {
+  // Moves the cut into bin `bin`, of whose tokens (that pass the cut so far,
+  // for masses) `before` already lies ahead, to where the sum reaches want.
+  auto select = [&](bool masses, int bin, u64 before, u64 want) {
+    const uint32_t klo = bin_bits(bin), khi = min(klo + ((1u << kBinShift) - 1), kOneBits);
+    auto member = [&](int i) { return !masses || in_cut(i); };
+    make_list(klo, khi, member);
+    u64 here = 0;
+    const int shift = min(low_shift(klo), 31);
+    for_list(klo, khi, member, [&](int i) {
       const uint32_t b = e_bits(i);
-      return b >= klo && b <= khi && (!masses || in_cut(i));
-    };
-    make_list(klo, khi, [&](int i) { return !masses || in_cut(i); });
-    const uint32_t bits = narrow(masses, member, [&](int i) { return e_bits(i); }, klo, khi, want, &before, &here);
+      const int f = kFine - 1 - static_cast<int>(b >> 9 & 511u);
+      atomicAdd(&sh.fcnt[f], 1u);
+      if (masses) atomicAdd(&sh.flow[f], (b & 511u) >> shift);
+    });
+    const uint32_t mid = klo | static_cast<uint32_t>(kFine - 1 - find_fine(masses, klo, 9, &before, &here, want)) << 9;
+    for_list(klo, khi, member, [&](int i) {
+      const uint32_t b = e_bits(i);
+      if (b >> 9 == mid >> 9) atomicAdd(&sh.fcnt[kFine - 1 - static_cast<int>(b & 511u)], 1u);
+    });
+    const uint32_t bits = mid | static_cast<uint32_t>(kFine - 1 - find_fine(masses, mid, 0, &before, &here, want));
     const u64 w = masses ? max(fixed_weight(__uint_as_float(bits)), 1ull) : 1;
     u64 ties = (want - before + w - 1) / w;
-    // (tokens without weight need no order)
-    const bool partial = fixed_weight(__uint_as_float(bits)) > 0 && (ties < here / w || (masses && cut.partial && bits == cut.bits));
+    const bool partial = ties < here / w || (masses && cut.partial && bits == cut.bits);
     cut.bits = bits;
     cut.partial = partial;
     if (!partial) return;
     // the first `ties` of the tokens with this e: by logit, then by index
-    auto equal = [&](int i) { return e_bits(i) == bits; };
+    auto any = [](int) { return true; };
     if (tid == 0) sh.kmin = 0xffffffffu, sh.kmax = 0;
-    make_list(bits, bits, [](int) { return true; });
+    make_list(bits, bits, any);
     uint32_t lo = 0xffffffffu, hi = 0;
-    for_list(equal, [&](int i) {
+    for_list(bits, bits, any, [&](int i) {
       const uint32_t key = logit_key(i);
       lo = min(lo, key), hi = max(hi, key);
     });
@@ -615,51 +632,127 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     lo = __reduce_min_sync(0xffffffffu, lane < static_cast<int>(C) ? *peer(cl, &sh.kmin, lane) : 0xffffffffu);
     hi = __reduce_max_sync(0xffffffffu, lane < static_cast<int>(C) ? *peer(cl, &sh.kmax, lane) : 0u);
     before = 0;
-    cut.key = narrow(false, equal, logit_key, lo, hi, ties, &before, &here);
+    for (int level = 0; lo < hi && level < 8; ++level) {  // four at most: 2^32 keys, 2^9 a level
+      const int open = max(0, 23 - __clz(hi - lo));
+      for_list(bits, bits, any, [&](int i) {
+        const uint32_t key = logit_key(i);
+        if (key >= lo && key <= hi) atomicAdd(&sh.fcnt[(hi - key) >> open], 1u);
+      });
+      const uint32_t top_key = hi - (static_cast<uint32_t>(find_fine(false, 0u, 0, &before, &here, ties)) << open), size = 1u << open;
+      lo = top_key - lo >= size - 1 ? top_key - (size - 1) : lo;
+      hi = top_key;
+    }
+    cut.key = lo;
     ties -= before;
+    u64 mine = 0;
+    for_list(bits, bits, any, [&](int i) { mine += logit_key(i) == lo; });
     unsigned owner;
     u64 total;
-    const uint32_t key = cut.key;
     const int at = locate(
+        mine,
         [&](int q, u64(&w4)[4]) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w4[j] = equal(4 * q + j) && logit_key(4 * q + j) == key;
+          for (int j = 0; j < 4; ++j) w4[j] = e_bits(4 * q + j) == bits && logit_key(4 * q + j) == lo;
         },
         [&](u64) { return ties - 1; }, &owner, &total);
     if (at >= 0 && tid == 0) sh.index = i0 + at;
     cl.sync();
     cut.last = *peer(cl, &sh.index, owner);
   };
-  if (by_k) select(false, [&](u64) { return static_cast<u64>(k); });
-  if (by_p) {
-    if (by_k) {
-      for (int q = tid; q < n4; q += kClThreads) {
-        const uint4 b = reinterpret_cast<const uint4*>(xs)[q];
-        const uint32_t bits[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (bits[j] >= cut.bits && in_cut(4 * q + j)) add_mass(e_bin(bits[j]), fixed_weight(__uint_as_float(bits[j])));
-      }
-    }
-    select(true, [&](u64 total) {
-      const double limit = static_cast<double>(total) * static_cast<double>(top_p);
-      return limit > 1.0 ? static_cast<u64>(limit) : 1ull;
-    });
-  }
-
-  const uint32_t low = max(cut.bits, __float_as_uint(min_p));
   auto kept = [&](int q, u64(&w)[4]) {
     const uint4 b = reinterpret_cast<const uint4*>(xs)[q];
     const uint32_t bits[4] = {b.x, b.y, b.z, b.w};
+    const uint32_t low = max(cut.bits, min_bits);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       w[j] = 0;
       if (bits[j] >= low && (bits[j] != cut.bits || !cut.partial || in_cut(4 * q + j))) w[j] = fixed_weight(__uint_as_float(bits[j]));
     }
   };
+  if (by_k || by_p) {
+    // the cluster's bins: three to a thread, in the order of the candidates
+    __syncthreads();
+    for (int b = tid; b < kBins; b += kClThreads) {
+      const uint32_t count = sh.cnt[b];
+      if (!count) continue;
+      atomicAdd(peer(cl, share_cnt + b - owner_of(b) * per, owner_of(b)), count);
+      if (by_p && b < kWeighty) atomicAdd(peer(cl, share_mass + b - owner_of(b) * per, owner_of(b)), bin_mass(bin_bits(b), count, sh.low[b]));
+    }
+    cl.sync();
+    constexpr int PER = kBins / kClThreads;
+    u64 mass[PER], sum = 0;
+    int k_bin = kBins;  // bins from it on are cut, but for what stays of its own
+    u64 k_mass = 0;
+    if (by_k) {
+      u64 v[PER];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const int b = tid * PER + e;
+        v[e] = *peer(cl, share_cnt + b - owner_of(b) * per, owner_of(b));
+        sum += v[e];
+      }
+      u64 total;
+      const u64 acc = block_scan(sum, sh.scan, &total);
+      find(v, std::integral_constant<int, PER>{}, 0, acc, static_cast<u64>(k));
+      const int bin = sh.bin;
+      const u64 before = sh.before;
+      __syncthreads();
+      if (bin < kWeighty) {  // else every token with weight is kept
+        k_bin = bin;
+        select(false, bin, before, static_cast<u64>(k));
+        if (by_p) {
+          // what is kept of its bin (the list may be that of a group of equals by now)
+          const uint32_t klo = bin_bits(bin), khi = klo + ((1u << kBinShift) - 1);
+          u64 mine = 0;
+          for (int q = tid; q < n4; q += kClThreads) {
+            const uint4 b = reinterpret_cast<const uint4*>(xs)[q];
+            const uint32_t bits[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (bits[j] >= cut.bits && bits[j] >= klo && bits[j] <= khi && in_cut(4 * q + j)) mine += fixed_weight(__uint_as_float(bits[j]));
+          }
+          k_mass = cluster_sum(mine);
+        }
+      }
+    }
+    if (by_p) {
+      sum = 0;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const int b = tid * PER + e;
+        mass[e] = b < k_bin ? *peer(cl, share_mass + b - owner_of(b) * per, owner_of(b)) : (b == k_bin ? k_mass : 0);
+        sum += mass[e];
+      }
+      u64 total;
+      const u64 acc = block_scan(sum, sh.scan, &total);
+      const double limit = static_cast<double>(total) * static_cast<double>(top_p);
+      const u64 want = limit > 1.0 ? static_cast<u64>(limit) : 1ull;
+      find(mass, std::integral_constant<int, PER>{}, 0, acc, want);
+      const int bin = sh.bin;
+      const u64 before = sh.before;
+      __syncthreads();
+      select(true, bin, before, want);
+    }
+    // this CTA's kept mass: whole bins from its histogram, the cut's own token by token
+    const uint32_t low = max(cut.bits, min_bits);
+    const int edge = e_bin(low);
+    for (int b = tid; b < min(edge, kWeighty); b += kClThreads) kept_mass += bin_mass(bin_bits(b), sh.cnt[b], sh.low[b]);
+    if (edge < kWeighty) {
+      const uint32_t khi = min(bin_bits(edge) + ((1u << kBinShift) - 1), kOneBits);
+      for (int q = tid; q < n4; q += kClThreads) {
+        const uint4 b = reinterpret_cast<const uint4*>(xs)[q];
+        const uint32_t bits[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (bits[j] >= low && bits[j] <= khi && (bits[j] != cut.bits || !cut.partial || in_cut(4 * q + j)))
+            kept_mass += fixed_weight(__uint_as_float(bits[j]));
+      }
+    }
+  }
+
   unsigned owner;
   u64 total;
-  const int token = locate(kept,
+  const int token = locate(kept_mass, kept,
                            [&](u64 all) -> u64 {
                              const double f = static_cast<double>(all) * static_cast<double>(u);
                              return f > 0.0 ? min(static_cast<u64>(f), all - 1) : 0;
@@ -676,7 +769,7 @@ cudaError_t sample_cluster_launch(const SampleParams& p, int num_sms, cudaStream
   static bool ready = false;
   cudaError_t e;
   if (!ready) {
-    e = cudaFuncSetAttribute(sample_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceMax * 4 + 3 * kBins * 8);
+    e = cudaFuncSetAttribute(sample_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceMax * 4 + kBins * 12 + kFine * 24);
     pin_carveout(sample_cluster_kernel);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_cluster_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
@@ -690,7 +783,7 @@ cudaError_t sample_cluster_launch(const SampleParams& p, int num_sms, cudaStream
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * static_cast<unsigned>(c));
   cfg.blockDim = dim3(kClThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(slice) * sizeof(float) + 3 * kBins / c * sizeof(u64);
+  cfg.dynamicSmemBytes = static_cast<size_t>(slice) * sizeof(float) + (kBins * 12 + kFine * 24) / c;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
