@@ -32,7 +32,6 @@ struct SampleParams {
   float* prob;
 };
 
-constexpr int kSampleThreads = 1024;
 typedef unsigned long long u64;
 
 // Order-preserving integer of a logit: NaN as -infinity, -0 as 0.
@@ -60,190 +59,6 @@ KIB_DEV u64 fixed_weight(float e) {
   const uint32_t m = (b & 0x7fffffu) | 0x800000u;
   if (shift >= 0) return static_cast<u64>(m) << shift;
   return shift > -24 ? m >> -shift : 0u;
-}
-
-template <typename T, typename Op>
-KIB_DEV T block_reduce(T v, Op op, T* s) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if (lane == 0) s[warp] = v;
-  __syncthreads();
-  v = s[0];
-  for (int w = 1; w < kSampleThreads / 32; ++w) v = op(v, s[w]);
-  return v;
-}
-
-// The end of a prefix in candidate order: keys above `key`, and the first
-// `ties` tokens (in index order) with exactly that key.
-struct Cut {
-  uint32_t key;
-  int ties;
-};
-
-__global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(const __grid_constant__ SampleParams p) {
-  __shared__ float s_f[32];
-  __shared__ u64 s_u[32];
-  __shared__ int s_i[32];
-  __shared__ unsigned s_count[256];
-  __shared__ u64 s_mass[256];
-  __shared__ uint32_t s_prefix;
-  __shared__ u64 s_before;
-  const int row = blockIdx.x, tid = threadIdx.x, V = p.vocab;
-  const float* x = p.logits + static_cast<int64_t>(row) * p.row_stride;
-  auto maxf = [](float a, float b) { return fmaxf(a, b); };
-  auto mini = [](int a, int b) { return a < b ? a : b; };
-  auto addu = [](u64 a, u64 b) { return a + b; };
-
-  float top = -INFINITY;
-  for (int i = tid; i < V; i += kSampleThreads) top = fmaxf(top, clean_logit(x[i]));
-  top = block_reduce(top, maxf, s_f);
-  if (top == -INFINITY) {  // nothing to choose from
-    if (tid == 0) {
-      p.token[row] = -1;
-      if (p.prob) p.prob[row] = 0.0f;
-    }
-    return;
-  }
-  const float t = p.temperature ? p.temperature[row] : 1.0f;
-  if (!(t > 1e-6f)) {
-    int best = V;
-    for (int i = tid; i < V; i += kSampleThreads)
-      if (clean_logit(x[i]) == top) best = min(best, i);
-    best = block_reduce(best, mini, s_i);
-    if (tid == 0) {
-      p.token[row] = best;
-      if (p.prob) p.prob[row] = 1.0f;
-    }
-    return;
-  }
-  const RowScale rs{top, __fdiv_rn(1.0f, t)};
-  const int k = p.top_k ? p.top_k[row] : 0;
-  const float top_p = p.top_p ? p.top_p[row] : 1.0f;
-  const float min_p = p.min_p && p.min_p[row] > 0.0f ? fminf(p.min_p[row], 1.0f) : 0.0f;
-
-  // radix selection of a cut, eight bits of the key at a time: by_count: the
-  // cut that keeps `want` tokens; otherwise the shortest prefix whose mass
-  // (within `in`) reaches `want`.
-  auto select = [&](bool by_count, u64 want, const Cut& in) -> Cut {
-    uint32_t prefix = 0;
-    u64 before = 0;
-    u64 weight = 1;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      for (int b = tid; b < 256; b += kSampleThreads) s_count[b] = 0, s_mass[b] = 0;
-      __syncthreads();
-      for (int i = tid; i < V; i += kSampleThreads) {
-        const float l = clean_logit(x[i]);
-        const uint32_t key = order_key(l);
-        if (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8))) continue;
-        if (by_count) atomicAdd(&s_count[(key >> shift) & 255], 1u);
-        else if (key >= in.key) atomicAdd(&s_mass[(key >> shift) & 255], fixed_weight(logit_weight(l, rs)));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        u64 acc = before;
-        int b = 255;
-        for (; b > 0; --b) {
-          u64 h = by_count ? s_count[b] : s_mass[b];
-          // ties of the enclosing cut beyond its count carry no mass
-          if (acc + h >= want) break;
-          acc += h;
-        }
-        s_prefix = prefix | (static_cast<uint32_t>(b) << shift);
-        s_before = acc;
-      }
-      __syncthreads();
-      prefix = s_prefix;
-      before = s_before;
-    }
-    if (!by_count) {
-      // every token of one key has one weight
-      const uint32_t b = prefix & 0x80000000u ? prefix & 0x7fffffffu : ~prefix;
-      weight = fixed_weight(logit_weight(__uint_as_float(b), rs));
-    }
-    Cut c;
-    c.key = prefix;
-    const u64 left = want > before ? want - before : 1;
-    const u64 n = weight ? (left + weight - 1) / weight : 1;
-    c.ties = n > 0x7fffffffull ? 0x7fffffff : static_cast<int>(n);
-    if (!by_count && c.key == in.key) c.ties = min(c.ties, in.ties);
-    return c;
-  };
-
-  Cut cut{0u, 0x7fffffff};  // everything
-  if (k > 0 && k < V) cut = select(true, static_cast<u64>(k), cut);
-  if (top_p < 1.0f) {
-    // mass of the prefix so far
-    u64 mass = 0, tied = 0;
-    for (int i = tid; i < V; i += kSampleThreads) {
-      const float l = clean_logit(x[i]);
-      const uint32_t key = order_key(l);
-      if (key > cut.key) mass += fixed_weight(logit_weight(l, rs));
-      else if (key == cut.key) ++tied;
-    }
-    mass = block_reduce(mass, addu, s_u);
-    tied = block_reduce(tied, addu, s_u);
-    if (tied > static_cast<u64>(cut.ties)) tied = static_cast<u64>(cut.ties);
-    const uint32_t b = cut.key & 0x80000000u ? cut.key & 0x7fffffffu : ~cut.key;
-    if (tied) mass += tied * fixed_weight(logit_weight(__uint_as_float(b), rs));
-    double limit = static_cast<double>(mass) * static_cast<double>(top_p);
-    u64 want = limit > 1.0 ? static_cast<u64>(limit) : 1;
-    if (!(limit == limit)) want = 1;
-    cut = select(false, want, cut);
-  }
-
-  // kept weights in index order: thread chunks, then a scan of the chunks
-  const int chunk = (V + kSampleThreads - 1) / kSampleThreads;
-  const int i0 = min(tid * chunk, V), i1 = min(i0 + chunk, V);
-  int tied = 0;
-  for (int i = i0; i < i1; ++i) tied += order_key(clean_logit(x[i])) == cut.key;
-  auto scan = [&](u64 v, u64* total) -> u64 {  // exclusive
-    const int lane = tid & 31, warp = tid >> 5;
-    u64 inc = v;
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 n = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += n;
-    }
-    __syncthreads();
-    if (lane == 31) s_u[warp] = inc;
-    __syncthreads();
-    u64 base = 0, all = 0;
-    for (int w = 0; w < kSampleThreads / 32; ++w) {
-      if (w < warp) base += s_u[w];
-      all += s_u[w];
-    }
-    *total = all;
-    return base + inc - v;
-  };
-  u64 total = 0;
-  const int tie0 = static_cast<int>(min(scan(static_cast<u64>(tied), &total), static_cast<u64>(0x7fffffff)));
-  auto kept = [&](int i, int& tie) -> u64 {
-    const float l = clean_logit(x[i]);
-    const uint32_t key = order_key(l);
-    if (key < cut.key || (key == cut.key && tie++ >= cut.ties)) return 0;
-    const float e = logit_weight(l, rs);
-    return e >= min_p || l == top ? fixed_weight(e) : 0;
-  };
-  u64 mine = 0;
-  int tie = tie0;
-  for (int i = i0; i < i1; ++i) mine += kept(i, tie);
-  u64 run = scan(mine, &total);
-  double aimf = static_cast<double>(total) * static_cast<double>(p.uniform[row]);
-  u64 aim = aimf > 0.0 ? static_cast<u64>(aimf) : 0;
-  if (aim >= total) aim = total - 1;
-  if (run <= aim && aim < run + mine) {
-    tie = tie0;
-    for (int i = i0; i < i1; ++i) {
-      const u64 w = kept(i, tie);
-      run += w;
-      if (run > aim) {
-        p.token[row] = i;
-        if (p.prob) p.prob[row] = static_cast<float>(static_cast<double>(w) / static_cast<double>(total));
-        break;
-      }
-    }
-  }
 }
 
 // ------------------------------------------------------------- by clusters
@@ -306,8 +121,12 @@ KIB_DEV T* peer(cg::cluster_group& cl, T* p, unsigned rank) {
   return cl.map_shared_rank(p, rank);
 }
 
-// Exclusive scan over the block; *total gets the sum.
+// Exclusive scan over the block; *total gets the sum.  Every warp scans the
+// warps' sums for itself: fewer instructions than a loop, and one barrier less
+// than having one warp do it.
+template <int THREADS>
 KIB_DEV u64 block_scan(u64 v, u64* s, u64* total) {
+  constexpr int W = THREADS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 inc = v;
 #pragma unroll
@@ -318,14 +137,15 @@ KIB_DEV u64 block_scan(u64 v, u64* s, u64* total) {
   __syncthreads();
   if (lane == 31) s[warp] = inc;
   __syncthreads();
-  u64 base = 0, all = 0;
+  const u64 w = lane < W ? s[lane] : 0;
+  u64 winc = w;
 #pragma unroll
-  for (int w = 0; w < kClThreads / 32; ++w) {
-    if (w < warp) base += s[w];
-    all += s[w];
+  for (int o = 1; o < W; o <<= 1) {
+    const u64 n = __shfl_up_sync(0xffffffffu, winc, o);
+    if (lane >= o) winc += n;
   }
-  *total = all;
-  return base + inc - v;
+  *total = __shfl_sync(0xffffffffu, winc, W - 1);
+  return __shfl_sync(0xffffffffu, winc - w, warp) + inc - v;
 }
 
 __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __grid_constant__ SampleParams p, int slice) {
@@ -478,7 +298,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     const u64 v = *peer(cl, mine_at + (tid & (fper - 1)), tid * C / kFine);
     if (tid == 0) sh.bin = kFine - 1, sh.before = *before, sh.here = 0;
     u64 total;
-    const u64 acc = block_scan(v, sh.scan, &total);
+    const u64 acc = block_scan<kClThreads>(v, sh.scan, &total);
     find(&v, std::integral_constant<int, 1>{}, *before, acc, want);
     *before = sh.before;
     *here = sh.here;
@@ -519,7 +339,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   // The block's sum, then the cluster's, of a value of each thread.
   auto cluster_sum = [&](u64 v) -> u64 {
     u64 all;
-    block_scan(v, sh.scan, &all);
+    block_scan<kClThreads>(v, sh.scan, &all);
     if (tid == 0) sh.total = all;
     cl.sync();
     u64 sum = lane < static_cast<int>(C) ? *peer(cl, &sh.total, lane) : 0;
@@ -535,7 +355,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   auto locate = [&](u64 mine, auto weight, auto aim_of, unsigned* owner, u64* total) -> int {
     // weight(q, w): the weights of tokens 4 q .. 4 q + 3
     u64 all = 0, w[4];
-    block_scan(mine, sh.scan, &all);
+    block_scan<kClThreads>(mine, sh.scan, &all);
     if (tid == 0) sh.total = all;
     cl.sync();
     const u64 theirs = lane < static_cast<int>(C) ? *peer(cl, &sh.total, lane) : 0;
@@ -566,7 +386,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
     if (tid == 0) sh.bin = 0, sh.before = base;
     __syncthreads();
     const u64 v = tid < rounds * W ? sh.table[tid] : 0;
-    const u64 acc = base + block_scan(v, sh.scan, &all);
+    const u64 acc = base + block_scan<kClThreads>(v, sh.scan, &all);
     if (acc <= aim && aim < acc + v) sh.bin = tid, sh.before = acc;
     __syncthreads();
     const int q = sh.bin / W * kClThreads + sh.bin % W * 32 + lane;
@@ -692,7 +512,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
         sum += v[e];
       }
       u64 total;
-      const u64 acc = block_scan(sum, sh.scan, &total);
+      const u64 acc = block_scan<kClThreads>(sum, sh.scan, &total);
       find(v, std::integral_constant<int, PER>{}, 0, acc, static_cast<u64>(k));
       const int bin = sh.bin;
       const u64 before = sh.before;
@@ -724,7 +544,7 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
         sum += mass[e];
       }
       u64 total;
-      const u64 acc = block_scan(sum, sh.scan, &total);
+      const u64 acc = block_scan<kClThreads>(sum, sh.scan, &total);
       const double limit = static_cast<double>(total) * static_cast<double>(top_p);
       const u64 want = limit > 1.0 ? static_cast<u64>(limit) : 1ull;
       find(mass, std::integral_constant<int, PER>{}, 0, acc, want);
@@ -765,6 +585,416 @@ __global__ void __launch_bounds__(kClThreads, 2) sample_cluster_kernel(const __g
   cl.sync();  // no CTA leaves while another may read its shared memory
 }
 
+// ------------------------------------------------------------------ by rows
+//
+// One CTA takes a row and reads it three times, mostly from L2: its maximum;
+// the histogram, as above; and, in warps' segments of the index order, what is
+// kept.  No cluster barriers and one set of scans a row, so it does the same
+// work in a third of the time where rows fill the GPU, and it takes rows of
+// any length; a single row is faster on a cluster.  The histogram's sums of
+// low bits are folded into 64-bit masses every 2^14 logits, before they can
+// overflow.
+
+// (two CTAs of 512 threads an SM took 376 us for 256 rows of 248320, one of 1024 330 us)
+constexpr int kRowThreads = 1024;
+constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kRowList = 4096;
+
+struct RowShared {
+  uint32_t cnt[kBins], low[kBins];
+  u64 mass[kBins];
+  uint32_t count[kBins];
+  uint32_t fcnt[kFine], flow[kFine];
+  u64 scan[kRowWarps];
+  uint32_t list[kRowList], list_bits[kRowList];
+  u64 segment[kRowWarps];
+  u64 before, here;
+  float top[kRowWarps];
+  int first, bin, listed, index;
+  uint32_t kmin, kmax;
+};
+
+__global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid_constant__ SampleParams p) {
+  extern __shared__ __align__(16) uint8_t row_raw[];
+  RowShared& sh = *reinterpret_cast<RowShared*>(row_raw);
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.vocab, Q = (V + 3) / 4;
+  const float* x = p.logits + static_cast<int64_t>(row) * p.row_stride;
+  const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  const float t = p.temperature ? __ldg(p.temperature + row) : 1.0f;
+  const int k = p.top_k ? __ldg(p.top_k + row) : 0;
+  const float top_p = p.top_p ? __ldg(p.top_p + row) : 1.0f;
+  const float min_p0 = p.min_p ? __ldg(p.min_p + row) : 0.0f;
+  const float min_p = min_p0 > 0.0f ? fminf(min_p0, 1.0f) : 0.0f;
+  const float u = __ldg(p.uniform + row), inv_t = __fdiv_rn(1.0f, t);
+  auto load = [&](int q) -> float4 {
+    float4 l;
+    if (wide && 4 * q + 3 < V) {
+      l = __ldg(reinterpret_cast<const float4*>(x) + q);
+    } else {
+      l.x = 4 * q < V ? __ldg(x + 4 * q) : -INFINITY;
+      l.y = 4 * q + 1 < V ? __ldg(x + 4 * q + 1) : -INFINITY;
+      l.z = 4 * q + 2 < V ? __ldg(x + 4 * q + 2) : -INFINITY;
+      l.w = 4 * q + 3 < V ? __ldg(x + 4 * q + 3) : -INFINITY;
+    }
+    return make_float4(clean_logit(l.x), clean_logit(l.y), clean_logit(l.z), clean_logit(l.w));
+  };
+
+  // four quads, `step` apart, all asked for before the first is used
+  auto load_four = [&](int q, int step, int end, float4 (&l)[4]) {
+    if (wide && q + 3 * step < min(end, V / 4)) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) l[w] = __ldg(reinterpret_cast<const float4*>(x) + q + w * step);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) l[w] = make_float4(clean_logit(l[w].x), clean_logit(l[w].y), clean_logit(l[w].z), clean_logit(l[w].w));
+    } else {
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        l[w] = q + w * step < end ? load(q + w * step) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    }
+  };
+
+  float top = -INFINITY;
+  for (int q = tid; q < Q; q += 4 * kRowThreads) {
+    float4 l[4];
+    load_four(q, kRowThreads, Q, l);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(fmaxf(top, fmaxf(l[w].x, l[w].y)), fmaxf(l[w].z, l[w].w));
+  }
+  top = warp_max(top);
+  if (lane == 0) sh.top[warp] = top;
+  if (tid == 0) sh.first = 0x7fffffff, sh.index = 0;
+  for (int b = tid; b < kBins; b += kRowThreads) sh.cnt[b] = sh.low[b] = sh.count[b] = 0, sh.mass[b] = 0;
+  if (tid < kFine) sh.fcnt[tid] = sh.flow[tid] = 0;
+  __syncthreads();
+  top = warp_max(lane < kRowWarps ? sh.top[lane] : -INFINITY);
+
+  if (top == -INFINITY || !(t > 1e-6f)) {
+    int best = 0x7fffffff;
+    if (top > -INFINITY)
+      for (int q = tid; q < Q; q += kRowThreads) {
+        const float4 l = load(q);
+        const int at = l.x == top ? 0 : (l.y == top ? 1 : (l.z == top ? 2 : (l.w == top ? 3 : 4)));
+        if (at < 4) best = min(best, 4 * q + at);
+      }
+    best = __reduce_min_sync(0xffffffffu, best);
+    if (lane == 0 && best != 0x7fffffff) atomicMin(&sh.first, best);
+    __syncthreads();
+    if (tid == 0) {
+      p.token[row] = sh.first == 0x7fffffff ? -1 : sh.first;
+      if (p.prob) p.prob[row] = sh.first == 0x7fffffff ? 0.0f : 1.0f;
+    }
+    return;
+  }
+  const RowScale rs{top, inv_t};
+  const bool by_k = k > 0 && k < V, by_p = !(top_p >= 1.0f);
+  const uint32_t min_bits = __float_as_uint(min_p);
+  auto bits_at = [&](int i) { return __float_as_uint(logit_weight(clean_logit(__ldg(x + i)), rs)); };
+  auto logit_key = [&](int i) { return order_key(clean_logit(__ldg(x + i))); };
+  auto e_bin = [](uint32_t bits) { return min(static_cast<int>(kOneBits >> kBinShift) - static_cast<int>(bits >> kBinShift), kBins - 1); };
+  auto bin_bits = [](int bin) { return ((kOneBits >> kBinShift) - static_cast<uint32_t>(bin)) << kBinShift; };
+  // what of (l - top) / T a token with these bits of e has at least (at most): spares the exponential of the others
+  auto z_of = [&](float l) { return __fmul_rn(l == rs.top ? 0.0f : __fsub_rn(l, rs.top), rs.inv_t); };
+  auto z_floor = [](uint32_t bits) { return bits ? logf(__uint_as_float(bits)) - 1e-4f : -INFINITY; };
+
+  struct {
+    uint32_t bits, key;
+    int last;
+    bool partial;
+  } cut = {0u, 0u, 0x7fffffff, false};
+  auto in_cut = [&](int i, uint32_t b) {
+    if (b != cut.bits || !cut.partial) return b >= cut.bits;
+    const uint32_t key = logit_key(i);
+    return key > cut.key || (key == cut.key && i <= cut.last);
+  };
+  auto find = [&](const u64* v, auto per_thread, u64 acc, u64 want) {
+    constexpr int PER = decltype(per_thread)::value;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      if (acc < want && want <= acc + v[e]) sh.bin = tid * PER + e, sh.before = acc, sh.here = v[e];
+      acc += v[e];
+    }
+    __syncthreads();
+  };
+  auto find_fine = [&](bool masses, uint32_t top_bits, int open, u64* before, u64* here, u64 want) -> int {
+    __syncthreads();
+    u64 v = 0;
+    if (tid < kFine) {
+      const uint32_t count = sh.fcnt[tid];
+      v = masses ? bin_mass(top_bits | static_cast<uint32_t>(kFine - 1 - tid) << open, count, sh.flow[tid]) : count;
+      sh.fcnt[tid] = sh.flow[tid] = 0;
+    }
+    if (tid == 0) sh.bin = kFine - 1, sh.before = *before, sh.here = 0;
+    u64 total;
+    const u64 acc = *before + block_scan<kRowThreads>(v, sh.scan, &total);
+    find(&v, std::integral_constant<int, 1>{}, acc, want);
+    *before = sh.before;
+    *here = sh.here;
+    const int bin = sh.bin;
+    __syncthreads();
+    return bin;
+  };
+  // The tokens with bits of e in [klo, khi]: listed, or gone through where there are too many.
+  auto for_range = [&](uint32_t klo, uint32_t khi, auto what) {
+    const float zl = z_floor(klo), zh = khi >= kOneBits ? INFINITY : logf(__uint_as_float(max(khi, 1u))) + 1e-4f;
+    for (int q0 = tid; q0 < Q; q0 += 4 * kRowThreads) {
+      float4 l4[4];
+      load_four(q0, kRowThreads, Q, l4);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float l[4] = {l4[w].x, l4[w].y, l4[w].z, l4[w].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float z = z_of(l[j]);
+          if (!(z >= zl && z <= zh)) continue;
+          const int i = 4 * (q0 + w * kRowThreads) + j;
+          const uint32_t b = __float_as_uint(logit_weight(l[j], rs));
+          if (b >= klo && b <= khi && i < V) what(i, b);
+        }
+      }
+    }
+  };
+  bool short_list = false;
+  auto make_list = [&](uint32_t klo, uint32_t khi) {
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    for_range(klo, khi, [&](int i, uint32_t b) {
+      const int at = atomicAdd(&sh.listed, 1);
+      if (at < kRowList) sh.list[at] = static_cast<uint32_t>(i), sh.list_bits[at] = b;
+    });
+    __syncthreads();
+    short_list = sh.listed <= kRowList;
+  };
+  auto for_list = [&](uint32_t klo, uint32_t khi, auto what) {
+    if (short_list) {
+      for (int j = tid; j < sh.listed; j += kRowThreads)
+        if (sh.list_bits[j] >= klo && sh.list_bits[j] <= khi) what(static_cast<int>(sh.list[j]), sh.list_bits[j]);
+    } else {
+      for_range(klo, khi, what);
+    }
+  };
+  // Index at which the running sum, in index order, of weight(i, bits of e)
+  // over the tokens with bits of at least `floor` exceeds aim_of(total): the
+  // warps' segments first, then the block goes through the one that holds it.
+  auto locate = [&](uint32_t floor, auto weight, auto aim_of, u64* total) -> int {
+    const float zl = z_floor(floor);
+    const int s0 = static_cast<int>(static_cast<int64_t>(Q) * warp / kRowWarps), s1 = static_cast<int>(static_cast<int64_t>(Q) * (warp + 1) / kRowWarps);
+    auto four = [&](int q, const float4& l4, u64 (&w)[4]) {
+      const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = 0;
+        if (!(z_of(l[j]) >= zl) || 4 * q + j >= V) continue;
+        const uint32_t b = __float_as_uint(logit_weight(l[j], rs));
+        if (b >= floor) w[j] = weight(4 * q + j, b);
+      }
+    };
+    u64 sum = 0, w[4];
+    for (int q = s0 + lane; q < s1; q += 128) {
+      float4 l4[4];
+      load_four(q, 32, s1, l4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        four(q + 32 * r, l4[r], w);
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
+    if (lane == 0) sh.segment[warp] = sum;
+    __syncthreads();
+    u64 base = 0, all = 0;
+    int seg = kRowWarps - 1;
+    for (int s = 0; s < kRowWarps; ++s) all += sh.segment[s];
+    *total = all;
+    const u64 aim = aim_of(all);
+    for (int s = 0; s < kRowWarps; ++s) {
+      if (aim < base + sh.segment[s]) {
+        seg = s;
+        break;
+      }
+      base += sh.segment[s];
+    }
+    const int q0 = static_cast<int>(static_cast<int64_t>(Q) * seg / kRowWarps), q1 = static_cast<int>(static_cast<int64_t>(Q) * (seg + 1) / kRowWarps);
+    for (int qb = q0; qb < q1; qb += kRowThreads) {
+      const int q = qb + tid;
+      w[0] = w[1] = w[2] = w[3] = 0;
+      if (q < q1) four(q, load(q), w);
+      const u64 own = (w[0] + w[1]) + (w[2] + w[3]);
+      u64 block;
+      u64 run = base + block_scan<kRowThreads>(own, sh.scan, &block);
+      if (run <= aim && aim < run + own) {
+        int at = 4 * q;
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          run += w[j];
+          at += run <= aim;
+        }
+        sh.index = at;
+      }
+      base += block;
+      if (base > aim) break;
+    }
+    __syncthreads();
+    return sh.index;
+  };
+  auto select = [&](bool masses, int bin, u64 before, u64 want) {
+    const uint32_t klo = bin_bits(bin), khi = min(klo + ((1u << kBinShift) - 1), kOneBits);
+    make_list(klo, khi);
+    u64 here = 0;
+    const int shift = min(low_shift(klo), 31);
+    for_list(klo, khi, [&](int i, uint32_t b) {
+      if (masses && !in_cut(i, b)) return;
+      const int f = kFine - 1 - static_cast<int>(b >> 9 & 511u);
+      atomicAdd(&sh.fcnt[f], 1u);
+      // rows of more than 2^23 tokens are refused, so 9 bits of each cannot overflow
+      if (masses) atomicAdd(&sh.flow[f], (b & 511u) >> shift);
+    });
+    const uint32_t mid = klo | static_cast<uint32_t>(kFine - 1 - find_fine(masses, klo, 9, &before, &here, want)) << 9;
+    for_list(mid, mid + 511u, [&](int i, uint32_t b) {
+      if (!masses || in_cut(i, b)) atomicAdd(&sh.fcnt[kFine - 1 - static_cast<int>(b & 511u)], 1u);
+    });
+    const uint32_t bits = mid | static_cast<uint32_t>(kFine - 1 - find_fine(masses, mid, 0, &before, &here, want));
+    const u64 w = masses ? max(fixed_weight(__uint_as_float(bits)), 1ull) : 1;
+    u64 ties = (want - before + w - 1) / w;
+    const bool partial = ties < here / w || (masses && cut.partial && bits == cut.bits);
+    cut.bits = bits;
+    cut.partial = partial;
+    if (!partial) return;
+    // the first `ties` of the tokens with this e: by logit, then by index
+    if (tid == 0) sh.kmin = 0xffffffffu, sh.kmax = 0;
+    __syncthreads();
+    uint32_t lo = 0xffffffffu, hi = 0;
+    for_list(bits, bits, [&](int i, uint32_t) {
+      const uint32_t key = logit_key(i);
+      lo = min(lo, key), hi = max(hi, key);
+    });
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) atomicMin(&sh.kmin, lo), atomicMax(&sh.kmax, hi);
+    __syncthreads();
+    lo = sh.kmin, hi = sh.kmax;
+    before = 0;
+    for (int level = 0; lo < hi && level < 8; ++level) {  // four at most: 2^32 keys, 2^9 a level
+      const int open = max(0, 23 - __clz(hi - lo));
+      for_list(bits, bits, [&](int i, uint32_t) {
+        const uint32_t key = logit_key(i);
+        if (key >= lo && key <= hi) atomicAdd(&sh.fcnt[(hi - key) >> open], 1u);
+      });
+      const uint32_t top_key = hi - (static_cast<uint32_t>(find_fine(false, 0u, 0, &before, &here, ties)) << open), size = 1u << open;
+      lo = top_key - lo >= size - 1 ? top_key - (size - 1) : lo;
+      hi = top_key;
+    }
+    cut.key = lo;
+    ties -= before;
+    u64 total;
+    cut.last = locate(bits, [&](int i, uint32_t b) -> u64 { return b == bits && logit_key(i) == lo; }, [&](u64) { return ties - 1; }, &total);
+    __syncthreads();  // sh.index is written again
+  };
+
+  if (by_k || by_p) {
+    for (int q0 = 0; q0 < Q; q0 += 4 * kRowThreads) {  // 2^14 logits between two folds
+      float4 l4[4];
+      load_four(q0 + tid, kRowThreads, Q, l4);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if (q0 + tid + w * kRowThreads >= Q) continue;
+        const float l[4] = {l4[w].x, l4[w].y, l4[w].z, l4[w].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t b = __float_as_uint(logit_weight(l[j], rs));
+          const int bin = e_bin(b);
+          atomicAdd(&sh.cnt[bin], 1u);
+          atomicAdd(&sh.low[bin], (b & ((1u << kBinShift) - 1)) >> min(low_shift(b), 31));
+        }
+      }
+      __syncthreads();
+      for (int b = tid; b < kBins; b += kRowThreads) {
+        const uint32_t count = sh.cnt[b];
+        if (!count) continue;
+        sh.count[b] += count;
+        if (b < kWeighty) sh.mass[b] += bin_mass(bin_bits(b), count, sh.low[b]);
+        sh.cnt[b] = sh.low[b] = 0;
+      }
+      __syncthreads();
+    }
+    constexpr int PER = (kBins + kRowThreads - 1) / kRowThreads;
+    u64 v[PER], sum = 0, total;
+    int k_bin = kBins;
+    u64 k_mass = 0;
+    if (by_k) {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const int b = tid * PER + e;
+        v[e] = b < kBins ? sh.count[b] : 0;
+        sum += v[e];
+      }
+      const u64 acc = block_scan<kRowThreads>(sum, sh.scan, &total);
+      find(v, std::integral_constant<int, PER>{}, acc, static_cast<u64>(k));
+      const int bin = sh.bin;
+      const u64 before = sh.before;
+      __syncthreads();
+      if (bin < kWeighty) {  // else every token with weight is kept
+        k_bin = bin;
+        select(false, bin, before, static_cast<u64>(k));
+        if (by_p) {
+          const uint32_t klo = bin_bits(bin), khi = min(klo + ((1u << kBinShift) - 1), kOneBits);
+          u64 mine = 0;
+          for_list(klo, khi, [&](int i, uint32_t b) { mine += in_cut(i, b) ? fixed_weight(__uint_as_float(b)) : 0; });
+          block_scan<kRowThreads>(mine, sh.scan, &k_mass);
+        }
+      }
+    }
+    if (by_p) {
+      sum = 0;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const int b = tid * PER + e;
+        v[e] = b < min(k_bin, kBins) ? sh.mass[b] : (b == k_bin ? k_mass : 0);
+        sum += v[e];
+      }
+      const u64 acc = block_scan<kRowThreads>(sum, sh.scan, &total);
+      const double limit = static_cast<double>(total) * static_cast<double>(top_p);
+      const u64 want = limit > 1.0 ? static_cast<u64>(limit) : 1ull;
+      find(v, std::integral_constant<int, PER>{}, acc, want);
+      const int bin = sh.bin;
+      const u64 before = sh.before;
+      __syncthreads();
+      select(true, bin, before, want);
+    }
+  }
+  u64 total;
+  const uint32_t floor = max(cut.bits, min_bits);
+  const int token = locate(floor,
+                           [&](int i, uint32_t b) -> u64 {
+                             return b != cut.bits || !cut.partial || in_cut(i, b) ? fixed_weight(__uint_as_float(b)) : 0;
+                           },
+                           [&](u64 all) -> u64 {
+                             const double f = static_cast<double>(all) * static_cast<double>(u);
+                             return f > 0.0 ? min(static_cast<u64>(f), all - 1) : 0;
+                           },
+                           &total);
+  if (tid == 0) {
+    p.token[row] = token;
+    if (p.prob) p.prob[row] = static_cast<float>(static_cast<double>(fixed_weight(__uint_as_float(bits_at(token)))) / static_cast<double>(total));
+  }
+}
+
+// The fewest CTAs that hold a row in shared memory.
+int cluster_of(int vocab) {
+  int c = 1;
+  while (c * kSliceMax < vocab) c *= 2;
+  return c;
+}
+// A row whose logits one CTA holds is always fastest there.  Longer ones take
+// clusters while those of about five rounds cover the GPU: measured at 248320
+// tokens 64 rows 157 us by clusters and 178 by rows, 96 rows 232 and 190, 256
+// rows 587 and 330; at 100000 tokens 64 rows 61 and 100, 256 rows 216 and 150.
+bool by_rows(const SampleParams& p, int num_sms) {
+  const int c = cluster_of(p.vocab);
+  return c > kClusterMax || (c > 1 && static_cast<int64_t>(p.rows) * c > 8ll * num_sms);
+}
+
 cudaError_t sample_cluster_launch(const SampleParams& p, int num_sms, cudaStream_t st) {
   static bool ready = false;
   cudaError_t e;
@@ -775,9 +1005,8 @@ cudaError_t sample_cluster_launch(const SampleParams& p, int num_sms, cudaStream
     if (e != cudaSuccess) return e;
     ready = true;
   }
-  // the fewest CTAs that hold a row; for few rows more of them, down to slices of 2048
-  int c = 1;
-  while (c * kSliceMax < p.vocab) c *= 2;
+  // for few rows more CTAs than hold one, down to slices of 2048
+  int c = cluster_of(p.vocab);
   while (c < kClusterMax && static_cast<int64_t>(p.rows) * c * 2 <= num_sms && p.vocab / (2 * c) >= 2048) c *= 2;
   const int slice = ((p.vocab + c - 1) / c + 127) / 128 * 128;
   cudaLaunchConfig_t cfg = {};
@@ -821,12 +1050,17 @@ extern "C" int kib_sample_f32(kib_ctx* ctx, const float* logits, uint64_t rows, 
   p.token = token_out;
   p.prob = prob_out;
   const cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-  if (vocab <= static_cast<uint64_t>(kClusterMax) * kSliceMax) {
-    const cudaError_t e = sample_cluster_launch(p, ctx->num_sms, st);
-    if (e != cudaSuccess) return check_cuda(ctx, e, "sample");
+  cudaError_t e;
+  if (!by_rows(p, ctx->num_sms)) {
+    e = sample_cluster_launch(p, ctx->num_sms, st);
   } else {
-    sample_row_kernel<<<static_cast<unsigned>(rows), kSampleThreads, 0, st>>>(p);
+    static bool ready = false;
+    e = ready ? cudaSuccess
+              : cudaFuncSetAttribute(sample_row_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(RowShared)));
+    ready = e == cudaSuccess;
+    if (ready) sample_row_kernel<<<static_cast<unsigned>(rows), kRowThreads, sizeof(RowShared), st>>>(p);
   }
+  if (e != cudaSuccess) return check_cuda(ctx, e, "sample");
   if (!stream) return finish_op(ctx, "sample");
   return check_cuda(ctx, cudaGetLastError(), "sample");
 }

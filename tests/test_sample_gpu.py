@@ -131,6 +131,41 @@ def test_sample_random_settings(ctx, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab,rows,stride", [(300001, 9, 0), (262145, 3, 262150), (262144, 75, 0), (40000, 400, 0), (99999, 150, 100003)])
+def test_sample_long_rows_and_large_batches(ctx, vocab, rows, stride):
+    """The path of rows too long or too many for clusters, next to its limits."""
+    r = np.random.default_rng(vocab)
+    x = (r.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    x[0] = 1.25                      # all equal
+    x[1, ::3] = -np.inf
+    x[2, 5] = np.nan
+    pick = lambda *a: r.choice(np.float32(a), rows)  # noqa: E731
+    u = r.random(rows).astype(np.float32)
+    for args in (dict(t=pick(0.5, 1, 1.7), k=pick(0, 1, 50, 20000), p=pick(0.01, 0.9, 0.99, 1), m=pick(0, 0.05)),
+                 dict(t=pick(1), k=pick(0), p=pick(1), m=pick(0))):
+        clean = np.where(np.isnan(x), -np.inf, x).astype(np.float32)
+        assert np.array_equal(sample(ctx, x, u, **args, stride=stride)[0], by_torch(clean, u, **args))
+    tok, prob = sample(ctx, x, u, t=np.zeros(rows), stride=stride)
+    assert np.array_equal(tok, np.nanargmax(x, 1)) and (prob == 1).all()
+    dead = np.full((rows, vocab), -np.inf, np.float32)
+    assert (sample(ctx, dead, u)[0] == -1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [270000])
+def test_sample_long_rows_of_equals(ctx, vocab):
+    r = np.random.default_rng(8)
+    x = r.choice(np.array([-1.0, -0.0, 0.0, 0.5], np.float32), (6, vocab))
+    # logits that differ and round to one weight: the order is theirs, then the index's
+    x[5] = np.nextafter(np.float32(1e-3), np.float32(1), dtype=np.float32) * r.choice(np.float32([1, 1 - 2.0 ** -23, 1 - 2.0 ** -22]), vocab)
+    u, one, none = r.random(6).astype(np.float32), np.ones(6), np.zeros(6)
+    for k, p in ((r.integers(1, vocab, 6), one), (none, r.uniform(0.05, 0.99, 6)), (r.integers(1, vocab, 6), r.uniform(0.05, 0.99, 6))):
+        assert np.array_equal(sample(ctx, x, u, one, k, p, none)[0], by_torch(x, u, one, k, p, none))
+        assert np.array_equal(sample(ctx, x[:, :9000].copy(), u, one, k % 9000 + 1, p, none)[0],
+                              by_torch(x[:, :9000].copy(), u, one, k % 9000 + 1, p, none))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("stride", [0, 1003, 1024])
 def test_sample_defaults_and_strides(ctx, stride):
     r = np.random.default_rng(2)
