@@ -329,6 +329,18 @@ KIB_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
 }
 KIB_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// One lane of a converged warp, the same each time.  The whole warp walks the
+// producing and the issuing loop, so the descriptors stay in uniform registers.
+KIB_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // Barrier of the softmax threads that also tells whether any of them said yes.
 KIB_DEV bool soft_any(bool x) {
   uint32_t r;
@@ -386,7 +398,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     if (threadIdx.x == 0) atomicCAS(p.err, 0, 3);
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
   const int64_t total = p.cum[p.count[0]];
   const int64_t ctas = few_ctas(total, p.ctas);
@@ -427,9 +439,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   };
 
   if (warp == 8) {
-    if (lane == 0) {
-      tma_prefetch_desc(&kmap);
-      tma_prefetch_desc(&vmap);
+    {
+      if (elect_one()) tma_prefetch_desc(&kmap), tma_prefetch_desc(&vmap);
       uint32_t it = 0;
       bool ok = true;
       auto load = [&](const CUtensorMap* map, bool is_k, int head, int key) {
@@ -438,10 +449,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll 1
         for (int i = 0; i < Sh::kPer && ok; ++i, ++it) {
           const int s = static_cast<int>(it % Sh::kStages);
-          ok = tc_wait(&empty[s], ((it / Sh::kStages) & 1) ^ 1, p.err);
+          ok = warp_ok(tc_wait(&empty[s], ((it / Sh::kStages) & 1) ^ 1, p.err));
           if (!ok) break;
-          mbar_arrive_expect_tx(&full[s], Sh::kStage);
           uint8_t* dst = s_st + s * Sh::kStage;
+          if (!elect_one()) continue;
+          mbar_arrive_expect_tx(&full[s], Sh::kStage);
           if (is_k) {
 #pragma unroll
             for (int b = 0; b < Sh::kStage / kBox; ++b)
@@ -467,61 +479,66 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       }
     }
   } else if (warp == 9) {
-    if (lane == 0) {
+    {
       constexpr uint32_t idesc_s = umma_idesc_f16(kManyKeys), idesc_o = umma_idesc_f16(HD);
       uint32_t it = 0, jg = 0, piece = 0;
       bool ok = true;
-      const uint32_t q0 = smem_u32(s_q), st0 = smem_u32(s_st);
+      // a descriptor's start address counts 16 bytes, so steps within the operands are additions
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), st_desc = umma_desc_sw128(smem_u32(s_st));
       auto scores = [&](uint32_t jj) {
         const uint32_t d = tmem + 256 + 128 * (jj & 1);
 #pragma unroll 1
         for (int i = 0; i < Sh::kPer && ok; ++i, ++it) {
           const int s = static_cast<int>(it % Sh::kStages);
-          ok = tc_wait(&full[s], (it / Sh::kStages) & 1, p.err);
+          ok = warp_ok(tc_wait(&full[s], (it / Sh::kStages) & 1, p.err));
           if (!ok) break;
           tc_fence_after();
           constexpr int STEPS = HD / 16 / Sh::kPer;
+          const uint64_t b0 = st_desc + static_cast<uint64_t>(s * (Sh::kStage / 16)), a0 = q_desc + static_cast<uint64_t>(i * (STEPS / 4) * 1024);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < STEPS; ++k) {
-            const uint32_t b = st0 + s * Sh::kStage + (k / 4) * 16384 + 32 * (k % 4);
-            const uint32_t a = q0 + (i * (STEPS / 4) + k / 4) * 16384 + 32 * (k % 4);
+            for (int k = 0; k < STEPS; ++k)
 #pragma unroll
-            for (int pl = 0; pl < PL; ++pl)
-              umma_f16(d, umma_desc_sw128(a + pl * kManyRows * HD * 2), umma_desc_sw128(b), idesc_s, (i | k | pl) != 0 ? 1u : 0u);
+              for (int pl = 0; pl < PL; ++pl)
+                umma_f16(d, a0 + (k / 4) * 1024 + 2 * (k % 4) + pl * (kManyRows * HD * 2 / 16), b0 + (k / 4) * 1024 + 2 * (k % 4),
+                         idesc_s, (k | pl) != 0 ? 1u : (i != 0 ? 1u : 0u));
+            umma_commit(&empty[s]);
+            if (i + 1 == Sh::kPer) umma_commit(&s_full[jj & 1]);
           }
-          umma_commit(&empty[s]);
+          __syncwarp();
         }
-        umma_commit(&s_full[jj & 1]);
       };
       auto outputs = [&](uint32_t jj, bool begin) {
-        ok = ok && tc_wait(&p_full[jj & 1], (jj >> 1) & 1, p.err);
+        ok = warp_ok(ok && tc_wait(&p_full[jj & 1], (jj >> 1) & 1, p.err));
         tc_fence_after();
         const uint32_t a = tmem + 256 + 128 * (jj & 1);
 #pragma unroll 1
         for (int i = 0; i < Sh::kPer && ok; ++i, ++it) {
           const int s = static_cast<int>(it % Sh::kStages);
-          ok = tc_wait(&full[s], (it / Sh::kStages) & 1, p.err);
+          ok = warp_ok(tc_wait(&full[s], (it / Sh::kStages) & 1, p.err));
           if (!ok) break;
           tc_fence_after();
           constexpr int STEPS = kManyKeys / 16 / Sh::kPer;
+          const uint64_t b0 = st_desc + static_cast<uint64_t>(s * (Sh::kStage / 16));
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < STEPS; ++k) {
-            const uint32_t b = st0 + s * Sh::kStage + (k / 4) * (HD * 128) + 32 * (k % 4);
+            for (int k = 0; k < STEPS; ++k)
 #pragma unroll
-            for (int pl = 0; pl < PL; ++pl)
-              umma_f16_ts(tmem, a + 64 * pl + 8 * (i * STEPS + k), umma_desc_sw128(b), idesc_o,
-                          begin && (i | k | pl) == 0 ? 0u : 1u);
+              for (int pl = 0; pl < PL; ++pl)
+                umma_f16_ts(tmem, a + 64 * pl + 8 * (i * STEPS + k), b0 + (k / 4) * (HD * 8) + 2 * (k % 4), idesc_o,
+                            (k | pl) != 0 ? 1u : (begin && i == 0 ? 0u : 1u));
+            umma_commit(&empty[s]);
+            if (i + 1 == Sh::kPer) umma_commit(&o_done[jj & 1]);
           }
-          umma_commit(&empty[s]);
+          __syncwarp();
         }
-        umma_commit(&o_done[jj & 1]);
       };
       int unit = unit0;
       for (int64_t at = first; at < stop && ok; ++unit) {
         const Run r = run_at(unit, at);
         at = r.next;
         if (r.g0 == r.g1) continue;
-        ok = tc_wait(&q_full, piece++ & 1, p.err);
+        ok = warp_ok(tc_wait(&q_full, piece++ & 1, p.err));
         tc_fence_after();
         const int n = r.g1 - r.g0;
         for (int j = 0; j < n && ok; ++j) {
@@ -566,6 +583,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                              (static_cast<int64_t>(r.head) * p.a.group + rr % p.a.group) * HD + lane * V,
                          x);
         }
+        // a negative softmax scale goes into q's sign
+        if (p.a.scale_log2 < 0.0f) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) x[e] = -x[e];
+        }
         float back = 1.0f;
         if constexpr (PL == 2) {
           float big = 0.0f;
@@ -595,7 +617,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           reinterpret_cast<uint32_t*>(dst)[e] = hi[e];
           if constexpr (PL == 2) reinterpret_cast<uint32_t*>(dst + kManyRows * HD * 2)[e] = lo[e];
         }
-        if (lane == 0) s_qs[i] = back * p.a.scale_log2;
+        if (lane == 0) s_qs[i] = back * fabsf(p.a.scale_log2);
       }
       // the run's largest v_scale
       float vmax = 0.0f;
@@ -639,20 +661,25 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         tc_fence_after();
         uint32_t s[64];
         if (ok) tmem_ld(tmem + lanes + 256 + 128 * buf + 64 * half, s);
-        // scores s * kc, with what is masked at -infinity (then already multiplied, kc = 1)
+        // what is masked goes to -infinity; kc is not negative, so a group's largest score is that of its largest s
         if (key + 64 > all_see || absent) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            const float x = __uint_as_float(s[i]) * kc[i >> 4];
-            s[i] = __float_as_uint(key + i >= end || sc[i >> 4].y < 0.0f ? -INFINITY : x);
-          }
+          for (int i = 0; i < 64; ++i)
+            if (key + i >= end || sc[i >> 4].y < 0.0f) s[i] = 0xff800000u;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) kc[g] = 1.0f;
+          for (int g = 0; g < 4; ++g) kc[g] = fmaxf(kc[g], 1e-38f);  // 0 times -infinity would be NaN
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]) * kc[i >> 4]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        for (int g = 0; g < 4; ++g) {
+          float a = __uint_as_float(s[16 * g]), b = __uint_as_float(s[16 * g + 1]);
+#pragma unroll
+          for (int i = 2; i < 16; i += 4) {
+            a = fmaxf(fmaxf(a, __uint_as_float(s[16 * g + i])), i + 2 < 16 ? __uint_as_float(s[16 * g + i + 2]) : a);
+            b = fmaxf(fmaxf(b, __uint_as_float(s[16 * g + i + 1])), i + 3 < 16 ? __uint_as_float(s[16 * g + i + 3]) : b);
+          }
+          top = fmaxf(top, fmaxf(a, b) * kc[g]);
+        }
         sh.x[buf][half][row] = top;
         // m follows only a growth of more than 2^8: p stays below 2^8, its half below 2^15
         if (soft_any(top > m + 8.0f)) {
@@ -679,7 +706,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
         }
         const float mm = fmaxf(m, -1e30f);
-        float lp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        // two scores an instruction: s * kc - m, and p * v_scale
+        float2 lp[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        const float2 nm = make_float2(-mm, -mm);
         const uint32_t pdst = tmem + lanes + 256 + 128 * buf + 32 * half;
 #pragma unroll
         for (int c0 = 0; c0 < 64; c0 += 32) {
@@ -687,14 +716,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             const int g = (c0 + i) >> 4;
-            const float a = ex2(fmaf(__uint_as_float(s[c0 + i]), kc[g], -mm));
-            const float b = ex2(fmaf(__uint_as_float(s[c0 + i + 1]), kc[g], -mm));
-            lp[(i >> 1) & 3] += a + b;
-            const float wa = a * vc[g], wb = b * vc[g];
-            ph[i >> 1] = pack_half2(wa, wb);
+            float2 e = __ffma2_rn(make_float2(__uint_as_float(s[c0 + i]), __uint_as_float(s[c0 + i + 1])), make_float2(kc[g], kc[g]), nm);
+            e = make_float2(ex2(e.x), ex2(e.y));
+            lp[(i >> 1) & 1] = __fadd2_rn(lp[(i >> 1) & 1], e);
+            const float2 w = __fmul2_rn(e, make_float2(vc[g], vc[g]));
+            ph[i >> 1] = pack_half2(w.x, w.y);
             if constexpr (PL == 2) {
               const float2 f2 = __half22float2(*reinterpret_cast<const __half2*>(&ph[i >> 1]));
-              pl[i >> 1] = pack_half2(wa - f2.x, wb - f2.y);
+              pl[i >> 1] = pack_half2(w.x - f2.x, w.y - f2.y);
             }
           }
           if (ok) {
@@ -702,7 +731,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             if constexpr (PL == 2) tmem_st16(pdst + 64 + c0 / 2, pl);
           }
         }
-        l += (lp[0] + lp[1]) + (lp[2] + lp[3]);
+        l += (lp[0].x + lp[0].y) + (lp[1].x + lp[1].y);
         if (ok) tmem_st_wait();
         tc_fence_before();
         __syncwarp();
