@@ -45,9 +45,11 @@ constexpr int kManyThreads = kManySoft + 64;
 // A unit costs about as much as this many granules besides its own (q in, the
 // pipeline filled and drained, O out), so runs are cut by granules plus this:
 // without it the CTA at the start of a prompt, where a unit sees one to three
-// tiles of keys, takes 26 units where others take 3 (prompts of up to 3001
-// tokens).
-constexpr int kManyUnitCost = 4;
+// tiles of keys, takes 26 units where others take 3.  Five prompts of up to
+// 3001 tokens, head_dim 256, 8 query heads, halves / fp32: 321 / 507 us with a
+// cost of 1, 261 / 412 with 2, 208 / 325 with 4, 178 / 273 with 6, 197 / 320
+// with 16 (head_dim 128: 6 is best too).
+constexpr int kManyUnitCost = 6;
 
 struct Kvq8ManyParams {
   Kvq8AttnParams a;
@@ -570,54 +572,64 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       auto row_end = [&](int i) { return i < live ? min(span, start + (row0 + i) / p.a.group + 1) : 0; };
       const float2* scales = p.scales + (static_cast<int64_t>(r.head) * p.tot_pad + off) / 16;
 
-      // q rows to shared memory as halves, in the swizzled layout of the MMA
-#pragma unroll 4
-      for (int i = warp; i < kManyRows; i += 8) {
-        constexpr int V = HD / 32;
-        float x[V];
+      // q rows to shared memory as halves, in the swizzled layout of the MMA;
+      // eight of a warp's rows asked for before the first is used (one after
+      // the other their latencies add up to 15 us a unit)
+      constexpr int V = HD / 32;
+#pragma unroll 1
+      for (int i0 = warp; i0 < kManyRows; i0 += 64) {
+        float xs[8][V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = 0.0f;
-        if (i < live) {
-          const int rr = row0 + i;
+        for (int e = 0; e < 8; ++e) {
+          const int rr = row0 + min(i0 + 8 * e, live - 1);
           load_vec<T, V>(static_cast<const T*>(p.a.q) + static_cast<int64_t>(sq.first + rr / p.a.group) * p.a.q_stride +
                              (static_cast<int64_t>(r.head) * p.a.group + rr % p.a.group) * HD + lane * V,
-                         x);
+                         xs[e]);
         }
-        // a negative softmax scale goes into q's sign
-        if (p.a.scale_log2 < 0.0f) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) x[e] = -x[e];
-        }
-        float back = 1.0f;
-        if constexpr (PL == 2) {
-          float big = 0.0f;
+        for (int i8 = 0; i8 < 8; ++i8) {
+          const int i = i0 + 8 * i8;
+          float (&x)[V] = xs[i8];
+          if (i >= live) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) big = fmaxf(big, fabsf(x[e]));
-          big = warp_max(big);
-          const int ex = static_cast<int>(__float_as_uint(big) >> 23);
-          if (ex > 20 && ex < 255) {
-            const int k = min(max(140 - ex, -100), 100);
-            const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
-            back = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[e] *= up;
+            for (int e = 0; e < V; ++e) x[e] = 0.0f;
           }
-        }
-        uint32_t hi[V / 2], lo[V / 2];
+          // a negative softmax scale goes into q's sign
+          if (p.a.scale_log2 < 0.0f) {
 #pragma unroll
-        for (int e = 0; e < V; e += 2) {
-          hi[e / 2] = pack_half2(x[e], x[e + 1]);
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[e / 2]));
-          lo[e / 2] = pack_half2(x[e] - f.x, x[e + 1] - f.y);
-        }
-        const int byte = lane * V * 2, slab = byte / 128, ch = (byte % 128) / 16;
-        uint8_t* dst = s_q + slab * 16384 + i * 128 + ((ch ^ (i & 7)) * 16) + byte % 16;
+            for (int e = 0; e < V; ++e) x[e] = -x[e];
+          }
+          float back = 1.0f;
+          if constexpr (PL == 2) {
+            float big = 0.0f;
 #pragma unroll
-        for (int e = 0; e < V / 2; ++e) {
-          reinterpret_cast<uint32_t*>(dst)[e] = hi[e];
-          if constexpr (PL == 2) reinterpret_cast<uint32_t*>(dst + kManyRows * HD * 2)[e] = lo[e];
+            for (int e = 0; e < V; ++e) big = fmaxf(big, fabsf(x[e]));
+            big = warp_max(big);
+            const int ex = static_cast<int>(__float_as_uint(big) >> 23);
+            if (ex > 20 && ex < 255) {
+              const int k = min(max(140 - ex, -100), 100);
+              const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+              back = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+#pragma unroll
+              for (int e = 0; e < V; ++e) x[e] *= up;
+            }
+          }
+          uint32_t hi[V / 2], lo[V / 2];
+#pragma unroll
+          for (int e = 0; e < V; e += 2) {
+            hi[e / 2] = pack_half2(x[e], x[e + 1]);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[e / 2]));
+            lo[e / 2] = pack_half2(x[e] - f.x, x[e + 1] - f.y);
+          }
+          const int byte = lane * V * 2, slab = byte / 128, ch = (byte % 128) / 16;
+          uint8_t* dst = s_q + slab * 16384 + i * 128 + ((ch ^ (i & 7)) * 16) + byte % 16;
+#pragma unroll
+          for (int e = 0; e < V / 2; ++e) {
+            reinterpret_cast<uint32_t*>(dst)[e] = hi[e];
+            if constexpr (PL == 2) reinterpret_cast<uint32_t*>(dst + kManyRows * HD * 2)[e] = lo[e];
+          }
+          if (lane == 0) s_qs[i] = back * fabsf(p.a.scale_log2);
         }
-        if (lane == 0) s_qs[i] = back * fabsf(p.a.scale_log2);
       }
       // the run's largest v_scale
       float vmax = 0.0f;
