@@ -102,14 +102,5 @@ KIB_DEV void load_codes(const int8_t* p, int (&c)[V]) {
 #pragma unroll
   for (int i = 0; i < V; ++i) c[i] = raw[i];
 }
-template <int V>
-KIB_DEV void store_codes(int8_t* p, const int (&c)[V]) {
-  alignas(8) int8_t raw[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) raw[i] = static_cast<int8_t>(c[i]);
-  if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(raw);
-  else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(raw);
-  else *reinterpret_cast<uint16_t*>(p) = *reinterpret_cast<const uint16_t*>(raw);
-}
 
 }  // namespace kib

@@ -123,7 +123,6 @@ __global__ void __launch_bounds__(kGatherThreads) kvq8_gather_kernel(const __gri
   __shared__ int s_scan32[kGatherThreads / 32];
   const int tid = threadIdx.x, S = p.a.b.sequences, kvh = p.a.c.kv_heads, head = blockIdx.y;
   const bool plan = blockIdx.x + 1 == gridDim.x;
-  pdl_launch_dependents();
   if (plan && head) return;
 
   // first padded keys; in the planning CTA then first units

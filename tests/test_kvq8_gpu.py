@@ -508,3 +508,61 @@ def test_wrapper_checks_shapes_and_types():
     with pytest.raises(ValueError):
         kib._row_type(torch.zeros(2, 3, 128)[:, :, ::2])
     assert kib._row_type(torch.zeros(5, 10, 64)[:, 2:6]) == (kib.TYPE_F32, 640)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,hd,heads,kv", [("f32", 256, 8, 2), ("f16", 256, 8, 2), ("f16", 64, 6, 6), ("f32", 128, 16, 1)])
+@pytest.mark.parametrize("length,rows", [(900, 900), (700, 129), (65, 65), (128, 64), (129, 1)])
+def test_attention_one_sequence(ctx, dtype, hd, heads, kv, length, rows):
+    # a prompt, a late chunk, row tiles that end with one row, a single row with many heads on one
+    check_attend(ctx, Case([length], [rows], heads, kv, hd, 32, dtype, seed=length + rows + hd))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows", [[1, 7, 8, 9, 2, 3], [15, 16, 17, 1, 2], [63, 64, 65, 1]])
+def test_attention_where_sequences_change_sides(ctx, dtype, rows):
+    """Rows times heads around the multiples of eight that a unit takes and
+    around the bound between the two kernels, in one batch."""
+    lengths = [n + 37 * i for i, n in enumerate(rows)]
+    for heads, kv, hd in ((8, 1, 64), (4, 1, 128), (3, 3, 256)):
+        check_attend(ctx, Case(lengths, rows, heads, kv, hd, 16, dtype, seed=rows[0] + hd))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 5, 40])
+def test_attention_long_absent_stretches(ctx, rows):
+    # 130 of a sequence's pages in a row absent: at its start, in its middle, up to its end
+    c = Case([2500, 2500, 2500, 300], [rows] * 4, 4, 2, 64, 16, seed=31)
+    c.table[0, :130] = -1
+    c.table[1, 15:145] = 1 << 30
+    c.table[2, 26:] = -5
+    c.batch.tensors[0].copy_(torch.from_numpy(c.table))
+    check_attend(ctx, c)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [[1], [1, 3], [1, 40]])
+def test_attention_many_sequences(ctx, rows):
+    n = 700
+    new = [rows[i % len(rows)] if i % 5 else 0 for i in range(n)]
+    lengths = [max(x, (i * 37) % 90) for i, x in enumerate(new)]
+    check_attend(ctx, Case(lengths, new, 4, 2, 64, 16, seed=len(rows) + rows[-1]))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 70])
+def test_a_cache_whose_offsets_pass_32_bits(ctx, rows):
+    """Pages 2^30 bytes apart: the last of nine lies 8 GB behind the first."""
+    c = Case([100, 80], [rows, rows], 8, 2, 128, 32, seed=33)
+    hold, dev = [], []
+    for x in c.codes:
+        big = torch.empty((c.pages - 1 << 30) + x[0].size, dtype=torch.int8, device="cuda")
+        view = torch.as_strided(big, x.shape, (1 << 30, x.shape[2] * x.shape[3], x.shape[3], 1))
+        view.copy_(torch.from_numpy(x))
+        hold.append(big)
+        dev.append(view)
+    c.dev[:2] = dev
+    c.cache = kib.KvQ8Cache(*c.dev)
+    check_attend(ctx, c)
+    check_append(ctx, c)
