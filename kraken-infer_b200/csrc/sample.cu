@@ -626,6 +626,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid
   const float min_p0 = p.min_p ? __ldg(p.min_p + row) : 0.0f;
   const float min_p = min_p0 > 0.0f ? fminf(min_p0, 1.0f) : 0.0f;
   const float u = __ldg(p.uniform + row), inv_t = __fdiv_rn(1.0f, t);
+  // logits below it cannot be among the first k: read as -infinity
+  float least = -INFINITY;
+  auto clean = [&](float l) {
+    l = clean_logit(l);
+    return l < least ? -INFINITY : l;
+  };
   auto load = [&](int q) -> float4 {
     float4 l;
     if (wide && 4 * q + 3 < V) {
@@ -636,7 +642,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid
       l.z = 4 * q + 2 < V ? __ldg(x + 4 * q + 2) : -INFINITY;
       l.w = 4 * q + 3 < V ? __ldg(x + 4 * q + 3) : -INFINITY;
     }
-    return make_float4(clean_logit(l.x), clean_logit(l.y), clean_logit(l.z), clean_logit(l.w));
+    return make_float4(clean(l.x), clean(l.y), clean(l.z), clean(l.w));
   };
 
   // four quads, `step` apart, all asked for before the first is used
@@ -645,7 +651,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid
 #pragma unroll
       for (int w = 0; w < 4; ++w) l[w] = __ldg(reinterpret_cast<const float4*>(x) + q + w * step);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) l[w] = make_float4(clean_logit(l[w].x), clean_logit(l[w].y), clean_logit(l[w].z), clean_logit(l[w].w));
+      for (int w = 0; w < 4; ++w) l[w] = make_float4(clean(l[w].x), clean(l[w].y), clean(l[w].z), clean(l[w].w));
     } else {
 #pragma unroll
       for (int w = 0; w < 4; ++w)
@@ -660,9 +666,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid
 #pragma unroll
     for (int w = 0; w < 4; ++w) top = fmaxf(fmaxf(top, fmaxf(l[w].x, l[w].y)), fmaxf(l[w].z, l[w].w));
   }
+  const float own_top = top;
   top = warp_max(top);
   if (lane == 0) sh.top[warp] = top;
-  if (tid == 0) sh.first = 0x7fffffff, sh.index = 0;
+  if (tid == 0) sh.first = 0x7fffffff, sh.index = 0, sh.listed = 0;
   for (int b = tid; b < kBins; b += kRowThreads) sh.cnt[b] = sh.low[b] = sh.count[b] = 0, sh.mass[b] = 0;
   if (tid < kFine) sh.fcnt[tid] = sh.flow[tid] = 0;
   __syncthreads();
@@ -688,6 +695,19 @@ __global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid
   const RowScale rs{top, inv_t};
   const bool by_k = k > 0 && k < V, by_p = !(top_p >= 1.0f);
   const uint32_t min_bits = __float_as_uint(min_p);
+  // k of the threads' maxima are k tokens, so the k-th token is no less than
+  // the k-th maximum (16 bits of it, found bit by bit): of a long row a few
+  // more than k tokens are left, and all else works on their list
+  if (by_k && k <= kRowThreads) {
+    const uint32_t key = order_key(own_top) >> 16;
+    uint32_t at = 0;
+    for (int bit = 15; bit >= 0; --bit)
+      if (__syncthreads_count(key >= (at | 1u << bit)) >= k) at |= 1u << bit;
+    at <<= 16;
+    least = __uint_as_float(at & 0x80000000u ? at ^ 0x80000000u : ~at);  // below -infinity's: a NaN, which hides nothing
+  }
+  const bool hidden = least > -INFINITY;
+  bool all_listed = false;
   auto bits_at = [&](int i) { return __float_as_uint(logit_weight(clean_logit(__ldg(x + i)), rs)); };
   auto logit_key = [&](int i) { return order_key(clean_logit(__ldg(x + i))); };
   auto e_bin = [](uint32_t bits) { return min(static_cast<int>(kOneBits >> kBinShift) - static_cast<int>(bits >> kBinShift), kBins - 1); };
@@ -755,6 +775,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid
   };
   bool short_list = false;
   auto make_list = [&](uint32_t klo, uint32_t khi) {
+    if (all_listed) return;
     if (tid == 0) sh.listed = 0;
     __syncthreads();
     for_range(klo, khi, [&](int i, uint32_t b) {
@@ -789,7 +810,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid
       }
     };
     u64 sum = 0, w[4];
-    for (int q = s0 + lane; q < s1; q += 128) {
+    __syncthreads();
+    if (all_listed) {
+      if (tid < kRowWarps) sh.segment[tid] = 0;
+      __syncthreads();
+      for (int j = tid; j < sh.listed; j += kRowThreads) {
+        const int i = static_cast<int>(sh.list[j]);
+        const u64 v = sh.list_bits[j] >= floor ? weight(i, sh.list_bits[j]) : 0;
+        if (v) atomicAdd(&sh.segment[(32 * (i / 4 + 1) - 1) / Q], v);  // the segment that holds quad i / 4
+      }
+    }
+    for (int q = all_listed ? s1 : s0 + lane; q < s1; q += 128) {
       float4 l4[4];
       load_four(q, 32, s1, l4);
 #pragma unroll
@@ -800,8 +831,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    __syncthreads();
-    if (lane == 0) sh.segment[warp] = sum;
+    if (lane == 0 && !all_listed) sh.segment[warp] = sum;
     __syncthreads();
     u64 base = 0, all = 0;
     int seg = kRowWarps - 1;
@@ -902,8 +932,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid
         const float l[4] = {l4[w].x, l4[w].y, l4[w].z, l4[w].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          if (hidden && l[j] == -INFINITY) continue;
           const uint32_t b = __float_as_uint(logit_weight(l[j], rs));
           const int bin = e_bin(b);
+          if (hidden) {
+            const int at = atomicAdd(&sh.listed, 1);
+            if (at < kRowList) sh.list[at] = static_cast<uint32_t>(4 * (q0 + tid + w * kRowThreads) + j), sh.list_bits[at] = b;
+          }
           atomicAdd(&sh.cnt[bin], 1u);
           atomicAdd(&sh.low[bin], (b & ((1u << kBinShift) - 1)) >> min(low_shift(b), 31));
         }
@@ -918,6 +953,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) sample_row_kernel(const __grid
       }
       __syncthreads();
     }
+    if (hidden && sh.listed <= kRowList) all_listed = short_list = true;
     constexpr int PER = (kBins + kRowThreads - 1) / kRowThreads;
     u64 v[PER], sum = 0, total;
     int k_bin = kBins;
