@@ -96,7 +96,7 @@ constexpr int kBins = 1536;     // 32 an octave: from bin 1281 on e < 2^-40, wit
 constexpr int kBinShift = 18;   // of the bits of e
 constexpr int kWeighty = 1281;
 constexpr int kFine = 512;      // bins of the histograms on the list
-constexpr int kListMax = 4096;
+constexpr int kListMax = 8192;
 constexpr uint32_t kOneBits = 0x3f800000u;
 
 struct SampleShared {
@@ -191,49 +191,37 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
   const float min_p = min_p0 > 0.0f ? fminf(min_p0, 1.0f) : 0.0f;
   const float u = __ldg(p.uniform + row), inv_t = __fdiv_rn(1.0f, t);
 
-  // logits below it cannot be among the first k: read as -infinity
-  float least = -INFINITY;
-  auto clean = [&](float l) {
-    l = clean_logit(l);
-    return l < least ? -INFINITY : l;
-  };
   auto load = [&](int q) -> float4 {
+    if (wide && 4 * q + 3 < V) return __ldg(reinterpret_cast<const float4*>(x) + q);
     float4 l;
-    if (wide && 4 * q + 3 < V) {
-      l = __ldg(reinterpret_cast<const float4*>(x) + q);
-    } else {
-      l.x = 4 * q < V ? __ldg(x + 4 * q) : -INFINITY;
-      l.y = 4 * q + 1 < V ? __ldg(x + 4 * q + 1) : -INFINITY;
-      l.z = 4 * q + 2 < V ? __ldg(x + 4 * q + 2) : -INFINITY;
-      l.w = 4 * q + 3 < V ? __ldg(x + 4 * q + 3) : -INFINITY;
-    }
-    return make_float4(clean(l.x), clean(l.y), clean(l.z), clean(l.w));
+    l.x = 4 * q < V ? __ldg(x + 4 * q) : -INFINITY;
+    l.y = 4 * q + 1 < V ? __ldg(x + 4 * q + 1) : -INFINITY;
+    l.z = 4 * q + 2 < V ? __ldg(x + 4 * q + 2) : -INFINITY;
+    l.w = 4 * q + 3 < V ? __ldg(x + 4 * q + 3) : -INFINITY;
+    return l;
   };
-  // four quads, `step` apart, all asked for before the first is used; what(token, logit) of each
+  // four quads, `step` apart, all asked for before the first is used; what(first token, logits) of each
   auto for_four = [&](int q, int step, int end, auto what) {
-    float4 l4[4];
+    float4 l[4];
     if (wide && q + 3 * step < min(end, V / 4)) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) l4[w] = __ldg(reinterpret_cast<const float4*>(x) + q + w * step);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) l4[w] = make_float4(clean(l4[w].x), clean(l4[w].y), clean(l4[w].z), clean(l4[w].w));
+      for (int w = 0; w < 4; ++w) l[w] = __ldg(reinterpret_cast<const float4*>(x) + q + w * step);
     } else {
 #pragma unroll
       for (int w = 0; w < 4; ++w)
-        l4[w] = q + w * step < end ? load(q + w * step) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        l[w] = q + w * step < end ? load(q + w * step) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int i = 4 * (q + w * step);
-      what(i, l4[w].x), what(i + 1, l4[w].y), what(i + 2, l4[w].z), what(i + 3, l4[w].w);
-    }
+    for (int w = 0; w < 4; ++w) what(4 * (q + w * step), l[w]);
   };
+  auto max4 = [](float4 l) { return fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w)); };  // (of NaN and a number: the number)
 
   float own_top = -INFINITY;
-  for (int q = qa + tid; q < qb; q += 4 * kThreads) for_four(q, kThreads, qb, [&](int, float l) { own_top = fmaxf(own_top, l); });
+  for (int q = qa + tid; q < qb; q += 4 * kThreads) for_four(q, kThreads, qb, [&](int, float4 l) { own_top = fmaxf(own_top, max4(l)); });
+  own_top += 0.0f;
   float top = warp_max(own_top);
   if (lane == 0) sh.tops[warp] = top;
-  if (tid == 0) sh.first = 0x7fffffff, sh.index = 0, sh.listed = 0;
+  if (tid == 0) sh.first = 0x7fffffff, sh.index = 0, sh.listed = 0, sh.bin = kBins - 1, sh.before = 0;
   for (int b = tid; b < kBins; b += kThreads) sh.cnt[b] = sh.low[b] = sh.count[b] = 0, sh.mass[b] = 0;
   if (tid < kFine) sh.fcnt[tid] = sh.flow[tid] = 0, sh.fine[0][tid] = sh.fine[1][tid] = sh.fine[2][tid] = 0;
   __syncthreads();
@@ -247,11 +235,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
   if (top == -INFINITY || !(t > 1e-6f)) {
     int best = 0x7fffffff;
     if (top > -INFINITY)
-      for (int q = qa + tid; q < qb; q += kThreads) {
-        const float4 l = load(q);
-        const int at = l.x == top ? 0 : (l.y == top ? 1 : (l.z == top ? 2 : (l.w == top ? 3 : 4)));
-        if (at < 4) best = min(best, 4 * q + at);
-      }
+      for (int q = qa + tid; q < qb; q += 4 * kThreads)
+        for_four(q, kThreads, qb, [&](int i, float4 l) {
+          if (max4(l) == top) best = min(best, i + (l.x == top ? 0 : (l.y == top ? 1 : (l.z == top ? 2 : 3))));
+        });
     best = __reduce_min_sync(0xffffffffu, best);
     if (lane == 0 && best != 0x7fffffff) atomicMin(&sh.first, best);
     cl.sync();
@@ -268,15 +255,23 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
   const RowScale rs{top, inv_t};
   const bool by_k = k > 0 && k < V, by_p = !(top_p >= 1.0f);
   const uint32_t min_bits = __float_as_uint(min_p);
+  float least = -INFINITY;  // logits below it are not among the first k
   if (by_k && k <= kThreads) {
     const uint32_t key = order_key(own_top) >> 16;
     uint32_t at = 0;
     for (int bit = 15; bit >= 0; --bit)
       if (__syncthreads_count(key >= (at | 1u << bit)) >= k) at |= 1u << bit;
     at <<= 16;
-    least = __uint_as_float(at & 0x80000000u ? at ^ 0x80000000u : ~at);  // below -infinity's: a NaN, which hides nothing
+    const float l = __uint_as_float(at & 0x80000000u ? at ^ 0x80000000u : ~at);
+    if (l > -INFINITY) least = l;  // (a key below -infinity's is a NaN's)
   }
-  const bool hidden = least > -INFINITY;
+  const bool hides = least > -INFINITY;
+  // e of four logits; without branches (a NaN gives 0)
+  auto weights = [&](float4 l, float (&e)[4]) {
+    const float x4[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = fmaxf(expf(__fmul_rn(x4[j] == rs.top ? 0.0f : __fsub_rn(x4[j], rs.top), rs.inv_t)), 0.0f);
+  };
   auto logit_key = [&](int i) { return order_key(clean_logit(__ldg(x + i))); };
   auto e_bin = [](uint32_t bits) { return min(static_cast<int>(kOneBits >> kBinShift) - static_cast<int>(bits >> kBinShift), kBins - 1); };
   auto bin_bits = [](int bin) { return ((kOneBits >> kBinShift) - static_cast<uint32_t>(bin)) << kBinShift; };  // its smallest
@@ -350,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
   // again where there are too many.  The same pass sums the weights of those
   // with bits of at least `from`: `kept_sum` is what of it lies in the warp's segment.
   bool all_listed = false, short_list = false;
+  float hidden = -INFINITY;  // logits below it are not counted (where all others are listed)
   u64 kept_sum = 0;
   auto pass = [&](uint32_t klo, uint32_t khi, uint32_t from, auto what) {
     const float skip = below(min(klo, from));
@@ -357,12 +353,16 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
     const int s0 = segment_at(warp), s1 = segment_at(warp + 1);
     for (int q = s0 + lane; q < s1; q += 128) {
       SplitSum part;
-      for_four(q, 32, s1, [&](int i, float l) {
-        if (!(l > skip)) return;
-        const float e = logit_weight(l, rs);
-        const uint32_t b = __float_as_uint(e);
-        part.add(b >= from ? e : 0.0f);
-        if (b >= klo && b <= khi && l > -INFINITY) what(i, b);
+      for_four(q, 32, s1, [&](int i, float4 l) {
+        if (!(max4(l) > skip)) return;  // most quads, where few tokens hold the mass
+        float e[4];
+        weights(l, e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t b = __float_as_uint(e[j]);
+          part.add(b >= from ? e[j] : 0.0f);
+          if (b - klo <= khi - klo && b) what(i + j, b);
+        }
       });
       sum += part.value();
     }
@@ -455,10 +455,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
       if (q < q1) {
         const float4 l4 = load(q);
         const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+        float e[4];
+        weights(l4, e);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t b = __float_as_uint(logit_weight(l[j], rs));
-          if (l[j] > -INFINITY && b >= floor) w[j] = weight(4 * q + j, b);
+          const uint32_t b = __float_as_uint(e[j]);
+          if (b && b >= floor && l[j] >= hidden) w[j] = weight(4 * q + j, b);
         }
       }
       const u64 mine = (w[0] + w[1]) + (w[2] + w[3]);
@@ -550,23 +552,32 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
   if (by_k || by_p) {
     for (int q0 = qa; q0 < qb; q0 += 4 * kThreads) {  // 2^14 logits between two folds
       const int q = q0 + tid;
-      for_four(q, kThreads, qb, [&](int i, float l) {
-        if (l == -INFINITY && (hidden || i >= 4 * qb)) return;
-        const uint32_t b = __float_as_uint(logit_weight(l, rs));
-        const int bin = e_bin(b);
-        if (hidden) {
-          const int at = atomicAdd(&sh.listed, 1);
-          if (at < kListMax) sh.list[at] = static_cast<uint32_t>(i), sh.list_bits[at] = b;
+      for_four(q, kThreads, qb, [&](int i, float4 l) {
+        if (hides && !(max4(l) >= least)) return;
+        const float x4[4] = {l.x, l.y, l.z, l.w};
+        float e[4];
+        weights(l, e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t b = __float_as_uint(e[j]);
+          const int bin = e_bin(b);
+          const bool counts = bin < kWeighty && (!hides || x4[j] >= least);
+          if (hides && counts) {
+            const int at = atomicAdd(&sh.listed, 1);
+            if (at < kListMax) sh.list[at] = static_cast<uint32_t>(i + j), sh.list_bits[at] = b;
+          }
+          if (counts) {
+            atomicAdd(&sh.cnt[bin], 1u);
+            atomicAdd(&sh.low[bin], (b & ((1u << kBinShift) - 1)) >> low_shift(b));
+          }
         }
-        atomicAdd(&sh.cnt[bin], 1u);
-        atomicAdd(&sh.low[bin], (b & ((1u << kBinShift) - 1)) >> min(low_shift(b), 31));
       });
       __syncthreads();
       for (int b = tid; b < kBins; b += kThreads) {
         const uint32_t count = sh.cnt[b];
         if (!count) continue;
         const int r = b / per, at = b - r * per;
-        const u64 mass = by_p && b < kWeighty ? bin_mass(bin_bits(b), count, sh.low[b]) : 0;
+        const u64 mass = by_p ? bin_mass(bin_bits(b), count, sh.low[b]) : 0;
         if (C == 1) {
           sh.count[b] += count, sh.mass[b] += mass;
         } else {
@@ -577,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
       }
       __syncthreads();
     }
-    if (hidden && sh.listed <= kListMax) all_listed = short_list = true;
+    if (hides && sh.listed <= kListMax) all_listed = short_list = true, hidden = least;
     cl.sync();
     // the cluster's bins: two to a thread, in the order of the candidates
     constexpr int PER = (kBins + kThreads - 1) / kThreads;
@@ -647,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       ahead = sum;
     } else {
-      pass(0xffffffffu, 0u, floor, [](int, uint32_t) {});
+      pass(0xffffffffu, 0xffffffffu, floor, [](int, uint32_t) {});
       ahead = kept_sum;
     }
     __syncthreads();
