@@ -89,6 +89,13 @@ KIB_DEV u64 fixed_weight(float e) {
 // histogram's share take turns: a copy is cleared behind the barrier after the
 // one it was gathered behind, a barrier before its next use.
 
+// Bound by instructions where rows fill the GPU (a logit costs about 50 in the
+// passes of top-p, most of them the exponential and the histogram's), by the
+// latency of barriers and scans where few rows are spread wide.  At 248320
+// logits, all rows alike: 256 rows with top-k 50 111 us and with top-p 0.9
+// besides 124 (the logits move at HBM's rate in 39), top-p 0.9 alone 272,
+// neither 114; 32 rows 26, 33, 46, 21 us; one row 21, 31, 27, 15 us.
+
 constexpr int kClusterMax = 16;
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
@@ -550,7 +557,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
   };
 
   if (by_k || by_p) {
-    for (int q0 = qa; q0 < qb; q0 += 4 * kThreads) {  // 2^14 logits between two folds
+    // 2^14 logits between two folds; backwards, as the slice's end is what L2 surely still holds
+    for (int q0 = qa + (Q - 1) / (4 * kThreads) * (4 * kThreads); q0 >= qa; q0 -= 4 * kThreads) {
       const int q = q0 + tid;
       for_four(q, kThreads, qb, [&](int i, float4 l) {
         if (hides && !(max4(l) >= least)) return;
@@ -680,7 +688,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
 }
 
 // CTAs of a row: as many as leave all rows on the GPU at once, with slices of
-// 2048 logits at least.
+// 2048 logits at least.  More rows than that take one each: 256 rows with top-k
+// 50 and top-p 0.9 124 us by one CTA and 172 by two, with top-p alone 272 and
+// 302 (rows with settings of every kind mixed even out better by two: 223 and
+// 205).
 int cluster_of(const SampleParams& p, int num_sms) {
   int c = 1;
   while (c < kClusterMax && static_cast<int64_t>(p.rows) * c * 2 <= num_sms && p.vocab / (2 * c) >= 2048) c *= 2;

@@ -305,3 +305,31 @@ def test_sample_refusals(ctx):
             ctx.sample(x, u, tok, **bad)
     with pytest.raises(ValueError):
         ctx.sample(x[:, ::2], u, tok)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 5, 18, 37, 74, 75])
+@pytest.mark.parametrize("vocab", [40003, 8192])
+def test_sample_every_split_of_a_row(ctx, rows, vocab):
+    """Row counts that give a row 16, 8, 4, 2 and 1 CTAs; top-k around the
+    number of a CTA's threads and of the tokens that are left."""
+    r = np.random.default_rng(rows + vocab)
+    x = (r.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    x[rows // 2, r.random(vocab) < 0.95] = -np.inf
+    x[rows // 3] = np.round(x[rows // 3])  # groups of equals
+    pick = lambda *a: r.choice(np.float32(a), rows)  # noqa: E731
+    for k in (1, 7, 1023, 1024, 1025, 5000, vocab - 1, vocab):
+        u = r.random(rows).astype(np.float32)
+        args = dict(t=pick(0.7, 1, 1.3), k=np.full(rows, k, np.float32), p=pick(0.3, 0.9, 1), m=pick(0, 0.02))
+        assert np.array_equal(sample(ctx, x, u, **args)[0], by_torch(x, u, **args))
+
+
+@pytest.mark.gpu
+def test_sample_where_no_logit_stands_out(ctx):
+    """Weights that fill one bin, or spread over every value of it."""
+    r = np.random.default_rng(21)
+    x = (1.0 + r.random((4, 100000)) * np.float32([[0.0], [1e-6], [1e-3], [0.02]])).astype(np.float32)
+    for k, p in ((0, 0.37), (700, 0.9), (30000, 1.0), (30000, 0.61)):
+        u = r.random(4).astype(np.float32)
+        args = dict(t=np.ones(4), k=np.full(4, k), p=np.full(4, p), m=np.zeros(4))
+        assert np.array_equal(sample(ctx, x, u, **args)[0], by_torch(x, u, **args))
