@@ -488,26 +488,33 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), st_desc = umma_desc_sw128(smem_u32(s_st));
       auto scores = [&](uint32_t jj) {
         const uint32_t d = tmem + 256 + 128 * (jj & 1);
+        // q's low halves first: the tensor core's sums lose up to their last
+        // bits toward zero at every step, least while they are small
 #pragma unroll 1
-        for (int i = 0; i < Sh::kPer && ok; ++i, ++it) {
-          const int s = static_cast<int>(it % Sh::kStages);
-          ok = warp_ok(tc_wait(&full[s], (it / Sh::kStages) & 1, p.err));
-          if (!ok) break;
-          tc_fence_after();
-          constexpr int STEPS = HD / 16 / Sh::kPer;
-          const uint64_t b0 = st_desc + static_cast<uint64_t>(s * (Sh::kStage / 16)), a0 = q_desc + static_cast<uint64_t>(i * (STEPS / 4) * 1024);
-          if (elect_one()) {
+        for (int pl = PL - 1; pl >= 0 && ok; --pl) {
+#pragma unroll 1
+          for (int i = 0; i < Sh::kPer && ok; ++i) {
+            const int s = static_cast<int>((it + i) % Sh::kStages);
+            if (pl == PL - 1) {
+              ok = warp_ok(tc_wait(&full[s], ((it + i) / Sh::kStages) & 1, p.err));
+              if (!ok) break;
+              tc_fence_after();
+            }
+            constexpr int STEPS = HD / 16 / Sh::kPer;
+            const uint64_t b0 = st_desc + static_cast<uint64_t>(s * (Sh::kStage / 16)),
+                           a0 = q_desc + static_cast<uint64_t>(i * (STEPS / 4) * 1024 + pl * (kManyRows * HD * 2 / 16));
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-              for (int pl = 0; pl < PL; ++pl)
-                umma_f16(d, a0 + (k / 4) * 1024 + 2 * (k % 4) + pl * (kManyRows * HD * 2 / 16), b0 + (k / 4) * 1024 + 2 * (k % 4),
-                         idesc_s, (k | pl) != 0 ? 1u : (i != 0 ? 1u : 0u));
-            umma_commit(&empty[s]);
-            if (i + 1 == Sh::kPer) umma_commit(&s_full[jj & 1]);
+              for (int k = 0; k < STEPS; ++k)
+                umma_f16(d, a0 + (k / 4) * 1024 + 2 * (k % 4), b0 + (k / 4) * 1024 + 2 * (k % 4), idesc_s,
+                         k != 0 ? 1u : (i != 0 || pl != PL - 1 ? 1u : 0u));
+              if (pl == 0) umma_commit(&empty[s]);
+              if (pl == 0 && i + 1 == Sh::kPer) umma_commit(&s_full[jj & 1]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
+        it += Sh::kPer;
       };
       auto outputs = [&](uint32_t jj, bool begin) {
         ok = warp_ok(ok && tc_wait(&p_full[jj & 1], (jj >> 1) & 1, p.err));
