@@ -391,7 +391,20 @@ size_t few_workspace(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_
 
 // Rows (times the group) up to which a sequence is the few-row kernel's.
 constexpr int kFewLimit = 64;
-bool any_many(const Kvq8Batch& b, int group) { return static_cast<int64_t>(b.max_rows) * group > kFewLimit; }
+// The most granules of 128 keys (for 16 query rows of a KV head) per SM that
+// the few-row kernel takes in their stead, whatever the rows: the many-row path
+// begins with three kernels' latencies.  Few against many rows' kernels, one
+// sequence, head_dim 256, 8 query heads, 2 KV heads, fp32: 32 tokens 9.9 and
+// 30.1 us, 200 tokens (1.4 granules) 23 and 34, 64 after 1000 (1.7) 21 and 38,
+// 40 after 4000 (4.3) 28 and 53; 300 after 300 (5.1) 42 and 38, 500 (6.8) 55
+// and 38; four sequences of 100 (1.4) 33 and 35.  Halves and other head sizes
+// cross over at the same place.
+constexpr int kFewGranules = 5;
+bool any_many(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_sms) {
+  if (static_cast<int64_t>(b.max_rows) * group <= kFewLimit) return false;
+  const int64_t units = (static_cast<int64_t>(b.rows) * group / 16 + b.sequences) * c.kv_heads;
+  return units * ((static_cast<int64_t>(b.max_length) + kFewGranule - 1) / kFewGranule) > static_cast<int64_t>(kFewGranules) * num_sms;
+}
 
 // The workspace of the many-row path, in this order behind the records.
 struct ManyLayout {
@@ -659,7 +672,7 @@ int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, cons
   KIB_ARG(static_cast<uint64_t>(b.rows) * heads < (1ull << 31), "kvq8_attention: rows times heads out of range");
   const int group = static_cast<int>(heads) / c.kv_heads;
   *bytes = few_workspace(c, b, group, ctx->num_sms);
-  if (any_many(b, group)) {
+  if (any_many(c, b, group, ctx->num_sms)) {
     const ManyLayout m = many_layout(c, b, static_cast<int64_t>(batch->total_length), group, ctx->num_sms);
     KIB_ARG(m.tot_pad * c.kv_heads < (1ll << 31) && m.max_units < (1ll << 27),
             "kvq8_attention: total_length or rows too large for one call");
@@ -693,7 +706,7 @@ int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8
   p.partial = static_cast<float*>(workspace);
   p.err = ctx->d_err;
   const cudaStream_t st = op_stream(ctx, stream);
-  const bool many = any_many(p.b, p.group);
+  const bool many = any_many(p.c, p.b, p.group, ctx->num_sms);
   // one sequence of many rows needs one path; a mixed batch takes both, each its own sequences
   p.few_limit = many ? (p.b.sequences == 1 ? 0 : kFewLimit) : 0x7fffffff;
   cudaError_t e = cudaSuccess;

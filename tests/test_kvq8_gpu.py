@@ -566,3 +566,22 @@ def test_a_cache_whose_offsets_pass_32_bits(ctx, rows):
     c.cache = kib.KvQ8Cache(*c.dev)
     check_attend(ctx, c)
     check_append(ctx, c)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 256), (8, 1, 64), (6, 2, 128)])
+def test_attention_short_sequences_beside_long_ones(ctx, dtype, heads, kv, hd):
+    """Enough work that long runs go to the tensor-core path, with sequences
+    of every short kind in the same batch."""
+    new = [500, 1, 65, 0, 128, 129, 16, 33, 300]
+    lengths = [900, 1, 65, 40, 128, 200, 16, 1000, 300]
+    check_attend(ctx, Case(lengths, new, heads, kv, hd, 16, dtype, seed=hd))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows", [140, 200, 260])
+def test_attention_around_the_work_that_one_kernel_takes_alone(ctx, dtype, rows):
+    for length in (rows, rows + 250):
+        check_attend(ctx, Case([length], [rows], 8, 2, 256, 64, dtype, seed=rows + length))
