@@ -325,9 +325,12 @@ int kib_kvq8_read_pages(kib_ctx* ctx, const kib_kvq8_cache* cache, const int32_t
 /* Causal attention of every row over its sequence's keys 0 .. its own
  * position: out = softmax(scale * q . K) V per head, query head h on KV head
  * h / (heads / kv_heads).  Rows without any key give zeros.  q and out
- * [rows][heads][head_dim] of one type: F32 rows are computed to fp32 accuracy,
- * F16 rows with the softmax weights rounded to half for the product with V
- * (sums and statistics in fp32).  workspace: kib_kvq8_attention_workspace
+ * [rows][heads][head_dim] of one type: F32 rows take q and the softmax weights
+ * as two halves each (22 bits), F16 rows the weights as one half; sums and
+ * statistics are fp32.  The tensor core's sums are cut, not rounded, so an F32
+ * result is off by about 1e-6 of itself, in the prompts' path by 3e-6 after
+ * 3000 keys and 6e-6 after 6000 (weights alike, V alike: up to three times
+ * that).  workspace: kib_kvq8_attention_workspace
  * bytes, 256-byte aligned; calls that may overlap need one each. */
 int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_batch* batch, int type,
                                  uint64_t heads, uint64_t* bytes);

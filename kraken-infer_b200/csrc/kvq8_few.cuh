@@ -34,6 +34,11 @@
 // of a K row are the A fragments of four mma k-steps (the dimensions of a dot
 // product may be taken in any order, and q is laid out the same way); of V,
 // two byte permutes transpose 4 keys x 2 dimensions into a fragment.
+// Measured, 2 KV heads of 256 with 4 query heads each: 64 sequences of up to
+// 32768, half rows: 209-217 us, 6.2 to 6.5 TB/s; 32 of about 2048, fp32: 24.5 us;
+// one of 4096: 12.1 us.  17 sequences of up to 8190 with up to 5 fp32 rows each
+// of 16 heads of 128: 50 us, 1.6 TB/s, there by the MMAs (three groups of
+// rows, two halves of q and of p).
 #pragma once
 
 #include "gemm_tc.cuh"

@@ -27,6 +27,13 @@
 // for the 2^8); fp32 rows use q and p as high + low halves, twice the MMAs.
 // TMEM: O in columns 0 .. head_dim - 1, S in 256.. and 384..
 //
+// Bound by the tensor pipe where runs are long (1024 half rows of 8 heads of
+// 256 after 32768 keys: 230-258 us by the machine, up to 1170 TFLOP/s, pipe 70 %
+// active), by what a unit costs besides its tiles where they are short (prompts
+// of up to 3001 tokens: halves 178 us, fp32 271 us).  Two turns of softmax
+// warps on alternate tiles instead of two halves of each took 280 us for the
+// former, asking for the next stage before a tile's products 252.
+//
 // Every wait is bounded; one that gives up raises *err, and all roles still
 // walk their loops to the end (without touching TMEM) so that no barrier is
 // left short of threads.
@@ -56,10 +63,11 @@ constexpr int kManyUnitCost = 6;
 // bits, of O and a step: 4.3e-8 where all V are alike, 2.3e-8 for random V and
 // scores (deviation 1.4), 0.9e-8 for random V and equal weights, where O is a
 // small rest of what was added.  For fp32 rows l is made smaller by the middle
-// of that, which leaves half of the loss at most: without it, 2.9e-6 of the
-// result after 7 tiles of random keys.  (Moving O into rounded sums in memory
-// keeps all bits; every 16 tiles it cost 11 % of the time of prompts, and runs
-// of 2 tiles are what it would have to be.)
+// of that, which leaves about half of the loss: after 7 tiles of random keys
+// 1.4e-6 of the result instead of 3.2e-6, after 24 tiles 2.9e-6, after 48
+// 5.5e-6 (V alike: 1.8e-5).  Moving O into rounded sums in memory every 16 or 8
+// tiles and adding those up took 8 and 13 % longer (prompts of up to 3001
+// tokens) and left as much with random V.
 constexpr float kManyStepLoss = 2.0e-8f;
 
 struct Kvq8ManyParams {
