@@ -327,10 +327,8 @@ int kib_kvq8_read_pages(kib_ctx* ctx, const kib_kvq8_cache* cache, const int32_t
  * h / (heads / kv_heads).  Rows without any key give zeros.  q and out
  * [rows][heads][head_dim] of one type: F32 rows take q and the softmax weights
  * as two halves each (22 bits), F16 rows the weights as one half; sums and
- * statistics are fp32.  The tensor core's sums are cut, not rounded, so an F32
- * result is off by about 1e-6 of itself, in the prompts' path by 3e-6 after
- * 3000 keys and 6e-6 after 6000 (weights alike, V alike: up to three times
- * that).  workspace: kib_kvq8_attention_workspace
+ * statistics are fp32: an F32 result is off by about 1e-6 of itself, by up to
+ * 2.5e-6 where values and weights are all alike.  workspace: kib_kvq8_attention_workspace
  * bytes, 256-byte aligned; calls that may overlap need one each. */
 int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_batch* batch, int type,
                                  uint64_t heads, uint64_t* bytes);

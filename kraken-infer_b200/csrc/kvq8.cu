@@ -411,11 +411,11 @@ bool any_many(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_sms) {
 
 // The workspace of the many-row path, in this order behind the records.
 struct ManyLayout {
-  size_t k16, v16, scales, seq_off, units, cum, cta_unit, split, count, bytes;
+  size_t k16, v16, scales, seq_off, units, cum, cta_unit, split, count, sums, bytes;
   int64_t tot_pad, max_units;
 };
 size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
-ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_length, int group, int num_sms) {
+ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_length, int type, int group, int num_sms) {
   ManyLayout m = {};
   const int64_t bound = static_cast<int64_t>(b.max_length) * b.sequences;
   if (total_length <= 0 || total_length > bound) total_length = bound;
@@ -434,6 +434,8 @@ ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_len
   m.cta_unit = at, at = up256(at + static_cast<size_t>(num_sms) * sizeof(int));
   m.split = at, at = up256(at + static_cast<size_t>(num_sms) * sizeof(int4));
   m.count = at, at = up256(at + 2 * sizeof(int));
+  m.sums = at;  // of fp32 rows
+  if (type == KIB_TYPE_F32) at = up256(at + static_cast<size_t>(num_sms) * kManyRows * c.head_dim * sizeof(float));
   m.bytes = at;
   return m;
 }
@@ -459,6 +461,7 @@ cudaError_t many_launch(const Kvq8AttnParams& a, const ManyLayout& w, uint8_t* w
   p.cta_unit = reinterpret_cast<int*>(ws + w.cta_unit);
   p.split = reinterpret_cast<int4*>(ws + w.split);
   p.count = reinterpret_cast<int*>(ws + w.count);
+  p.sums = reinterpret_cast<float4*>(ws + w.sums);
   p.ctas = num_sms;
   p.err = err;
   const int kvh = a.c.kv_heads;
@@ -676,7 +679,7 @@ int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, cons
   const int group = static_cast<int>(heads) / c.kv_heads;
   *bytes = few_workspace(c, b, group, ctx->num_sms);
   if (any_many(c, b, group, ctx->num_sms)) {
-    const ManyLayout m = many_layout(c, b, static_cast<int64_t>(batch->total_length), group, ctx->num_sms);
+    const ManyLayout m = many_layout(c, b, static_cast<int64_t>(batch->total_length), type, group, ctx->num_sms);
     KIB_ARG(m.tot_pad * c.kv_heads < (1ll << 31) && m.max_units < (1ll << 27),
             "kvq8_attention: total_length or rows too large for one call");
     *bytes = m.bytes;
@@ -719,7 +722,7 @@ int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8
 #undef CALL
   }
   if (many && e == cudaSuccess) {
-    const ManyLayout m = many_layout(p.c, p.b, static_cast<int64_t>(batch->total_length), p.group, ctx->num_sms);
+    const ManyLayout m = many_layout(p.c, p.b, static_cast<int64_t>(batch->total_length), type, p.group, ctx->num_sms);
 #define CALL(T, HD) e = many_launch<T, HD>(p, m, static_cast<uint8_t*>(workspace), ctx->num_sms, ctx->d_err, st)
     KVQ8_DISPATCH(type, p.c.head_dim, CALL);
 #undef CALL

@@ -30,7 +30,7 @@
 // Bound by the tensor pipe where runs are long (1024 half rows of 8 heads of
 // 256 after 32768 keys: 230-258 us by the machine, up to 1170 TFLOP/s, pipe 70 %
 // active), by what a unit costs besides its tiles where they are short (prompts
-// of up to 3001 tokens: halves 178 us, fp32 271 us).  Two turns of softmax
+// of up to 3001 tokens: halves 178 us, fp32 306 us).  Two turns of softmax
 // warps on alternate tiles instead of two halves of each took 280 us for the
 // former, asking for the next stage before a tile's products 252.
 //
@@ -60,14 +60,15 @@ constexpr int kManyUnitCost = 6;
 
 // The tensor core's fp32 sums are cut toward zero: O loses a little at each
 // step (16 keys, and again for p's low halves).  What was measured against 64
-// bits, of O and a step: 4.3e-8 where all V are alike, 2.3e-8 for random V and
+// bits, of O and a step: 4e-8 where all V are alike, 2e-8 for random V and
 // scores (deviation 1.4), 0.9e-8 for random V and equal weights, where O is a
-// small rest of what was added.  For fp32 rows l is made smaller by the middle
-// of that, which leaves about half of the loss: after 7 tiles of random keys
-// 1.4e-6 of the result instead of 3.2e-6, after 24 tiles 2.9e-6, after 48
-// 5.5e-6 (V alike: 1.8e-5).  Moving O into rounded sums in memory every 16 or 8
-// tiles and adding those up took 8 and 13 % longer (prompts of up to 3001
-// tokens) and left as much with random V.
+// small rest of what was added.  So for fp32 rows O moves into rounded sums in
+// memory every kManyFlush tiles, and what a run loses until then is taken off
+// l by the middle of those figures.  Error after 6144 random keys, of the
+// result, and time of prompts of up to 3001 tokens: about 13e-6 and 271 us with
+// neither, 5.5e-6 and 271 us without the moves, 2.0e-6 and 301 us with moves
+// every 12 tiles, 1.4e-6 and 306 us every 8 (all V alike: 2.4e-6).
+constexpr int kManyFlush = 8;
 constexpr float kManyStepLoss = 2.0e-8f;
 
 struct Kvq8ManyParams {
@@ -81,6 +82,7 @@ struct Kvq8ManyParams {
   int4* units;      // [max_units] sequence, row tile, head, granules
   int64_t* cum;     // [max_units + 1] running cost; cum[count[0]] is the total
   int* cta_unit;    // [ctas] unit at which a CTA begins
+  float4* sums;     // fp32 rows: [ctas][head_dim / 4][128 rows] what O moves into
   int4* split;      // [ctas] units that cross CTAs: unit, first CTA, CTAs, whether its first record is a CTA's second
   int* count;       // [2] units, split units
   int ctas;
@@ -397,6 +399,30 @@ struct ManyShape {
   static constexpr size_t kSmem = static_cast<size_t>(kQ) + kStages * kStage + sizeof(ManyShared);
 };
 
+// The sums that O moves into: 32 of a row's columns, each thread's own, 16
+// bytes of a warp's rows side by side.
+KIB_DEV float4* many_sums(float4* sums, int c0, int hd, int row) {
+  return sums + (static_cast<int64_t>(blockIdx.x) * (hd / 4) + c0 / 4) * kManyRows + row;
+}
+KIB_DEV void many_add(float4* sums, int c0, int hd, int row, float f, uint32_t (&o)[32]) {
+  const float4* s = many_sums(sums, c0, hd, row);
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    const float4 v = s[i / 4 * kManyRows];
+    o[i] = __float_as_uint(fmaf(v.x, f, __uint_as_float(o[i])));
+    o[i + 1] = __float_as_uint(fmaf(v.y, f, __uint_as_float(o[i + 1])));
+    o[i + 2] = __float_as_uint(fmaf(v.z, f, __uint_as_float(o[i + 2])));
+    o[i + 3] = __float_as_uint(fmaf(v.w, f, __uint_as_float(o[i + 3])));
+  }
+}
+KIB_DEV void many_move(float4* sums, int c0, int hd, int row, bool more, float f, uint32_t (&o)[32]) {
+  if (more) many_add(sums, c0, hd, row, f, o);
+  float4* s = many_sums(sums, c0, hd, row);
+#pragma unroll
+  for (int i = 0; i < 32; i += 4)
+    s[i / 4 * kManyRows] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+}
+
 template <int HD, int PL>
 __global__ void __launch_bounds__(kManyThreads, 1)
     kvq8_many_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -672,7 +698,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int end = row_end(row);
       const int all_see = row_end(0);  // keys below it are seen by every row (of the dead ones nothing is kept)
 
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY, l = 0.0f, m_sums = -INFINITY;  // m_sums: m at the last move of O
       const int n = r.g1 - r.g0;
       float2 sc[4];
 #pragma unroll
@@ -719,7 +745,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         sh.x[buf][half][row] = top;
         // m follows only a growth of more than 2^8: p stays below 2^8, its half below 2^15
-        if (soft_any(top > m + 8.0f)) {
+        const bool move = PL == 2 && j > 0 && j % kManyFlush == 0;
+        if (soft_any(top > m + 8.0f) || move) {
           const float mn = fmaxf(m, fmaxf(top, sh.x[buf][half ^ 1][row]));
           const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
           m = mn;
@@ -736,10 +763,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 tmem_ld(addr, o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                if (PL == 2 && move) {
+                  many_move(p.sums, half * (HD / 2) + c0, HD, row, j > kManyFlush, m_sums == -INFINITY ? 0.0f : ex2(m_sums - mn), o);
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) o[i] = 0u;
+                }
                 tmem_st32(addr, o);
               }
               tmem_st_wait();
             }
+            if (move) m_sums = mn;
           }
         }
         const float mm = fmaxf(m, -1e30f);
@@ -787,7 +820,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       l += s_l[(half ^ 1) * kManyRows + row];
       if constexpr (PL == 2) {
         const int seen = min(max(end - r.g0 * kManyKeys, 0), n * kManyKeys);
-        l = fmaf(l, -kManyStepLoss * static_cast<float>(seen / 8), l);
+        l = fmaf(l, -kManyStepLoss * static_cast<float>(min(seen, kManyFlush * kManyKeys) / 8), l);
       }
       const float back = __uint_as_float(static_cast<uint32_t>(max(ve - 6, 1)) << 23);  // 2^(ve - 126) / 2^7
       const float inv = r.whole ? (l > 0.0f ? back / l : (l == 0.0f ? 0.0f : l)) : back;
@@ -799,6 +832,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       for (int c0 = half * (HD / 2); c0 < (half + 1) * (HD / 2); c0 += 32) {
         uint32_t o[32];
         if (ok) tmem_ld(tmem + lanes + c0, o);
+        if (PL == 2 && ok && n > kManyFlush) many_add(p.sums, c0, HD, row, m_sums == -INFINITY ? 0.0f : ex2(m_sums - m), o);
         if (row < live) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
