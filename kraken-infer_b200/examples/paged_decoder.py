@@ -121,11 +121,12 @@ class PagedDecoder:
                             top_p=per("top_p", torch.float32), min_p=per("min_p", torch.float32))
             uniform = torch.tensor(uniform, dtype=torch.float32).cuda()
             token, prob = torch.empty(count, dtype=torch.int32, device="cuda"), new(count)
-            logits = new(count, cfg.vocab)
+            logits, tail, normed = new(count, cfg.vocab), new(count, cfg.width), new(count, cfg.width)
             mul = lambda w, a, o, rows=n: ctx.matmul_kquant(*w, rows, a, o)  # noqa: E731
             norm = lambda w, a, o, rows=n: ctx.call("kib_rms_norm_f32_f32_batched", a, w, rows, cfg.width, cfg.eps, o)  # noqa: E731
             add = lambda a, b: ctx.call("kib_binary_f32_in_place", 0, a, b, a.numel(), cfg.width)  # noqa: E731
 
+            # captured from here on: nothing may allocate
             ctx.begin_graph()
             qtype, weight, rows, cols = self.embed
             ctx.dequantize_rows(qtype, weight, rows, ids, n, cols, x)
@@ -144,7 +145,7 @@ class PagedDecoder:
                 ctx.call("kib_silu_mul_f32_in_place", gate, up, gate.numel())
                 mul(layer["down"], gate, h)
                 add(x, h)
-            tail, normed = x[last], new(count, cfg.width)
+            torch.index_select(x, 0, last, out=tail)
             norm(self.norm, tail, normed, count)
             mul(self.head, normed, logits, count)
             ctx.sample(logits, uniform, token, prob, **settings)

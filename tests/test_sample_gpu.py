@@ -133,7 +133,7 @@ def test_sample_random_settings(ctx, vocab):
 @pytest.mark.gpu
 @pytest.mark.parametrize("vocab,rows,stride", [(300001, 9, 0), (262145, 3, 262150), (262144, 75, 0), (40000, 400, 0), (99999, 150, 100003)])
 def test_sample_long_rows_and_large_batches(ctx, vocab, rows, stride):
-    """The path of rows too long or too many for clusters, next to its limits."""
+    """Long rows, odd strides, and more rows than SMs."""
     r = np.random.default_rng(vocab)
     x = (r.standard_normal((rows, vocab)) * 3).astype(np.float32)
     x[0] = 1.25                      # all equal
