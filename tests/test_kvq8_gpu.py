@@ -585,3 +585,33 @@ def test_attention_short_sequences_beside_long_ones(ctx, dtype, heads, kv, hd):
 def test_attention_around_the_work_that_one_kernel_takes_alone(ctx, dtype, rows):
     for length in (rows, rows + 250):
         check_attend(ctx, Case([length], [rows], 8, 2, 256, 64, dtype, seed=rows + length))
+
+
+@gpu
+@pytest.mark.parametrize("hd,spread", [(64, 1.0), (128, 2.0), (256, 2.0), (256, 0.0)])
+@pytest.mark.parametrize("alike", [False, True])
+def test_attention_long_prompts_keep_fp32_accuracy(ctx, hd, spread, alike):
+    """A prompt so long that a CTA's runs are up to 48 tiles.  The cut sums of
+    the tensor core may lose 4.3e-8 of O at each of 128 steps between two
+    roundings, of which 2e-8 is made up for, and 1.5e-6 is left for q's, p's and
+    the scores' 22 bits: 4.4e-6 of the result's norm."""
+    n, heads, kv, page = 6144, 8, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    codes = [(rnd(n // page, kv, page, hd) * 34).clamp_(-127, 127).round_().to(torch.int8) for _ in range(2)]
+    if alike:
+        codes[1].fill_(100)
+    scales = [0.012 * torch.exp(0.3 * rnd(n // page, kv)) + 0.012 for _ in range(2)]
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = kib.KvQ8Batch(torch.randperm(n // page, generator=g, device="cuda").to(torch.int32)[None], i32([n]), i32([0, n]), n, n)
+    q = rnd(n, heads, hd) * spread
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    ctx.kvq8_attention(kib.KvQ8Cache(*codes, *scales), batch, q, out, hd ** -0.5)
+    order = batch.tensors[0][0].long()
+    k, v = ((c.double() * s.double()[..., None, None])[order].permute(1, 0, 2, 3).reshape(kv, n, hd) for c, s in zip(codes, scales))
+    for rows in (torch.arange(n - 64, n, device="cuda"), torch.arange(3000, 3064, device="cuda")):
+        s = torch.einsum("rgxd,gkd->rgxk", q[rows].double().view(64, kv, heads // kv, hd), k) * hd ** -0.5
+        s.masked_fill_(torch.arange(n, device="cuda") > rows[:, None, None, None], -torch.inf)
+        want = torch.einsum("rgxk,gkd->rgxd", s.softmax(-1), v).reshape(64, heads, hd)
+        assert (out[rows] - want).norm() <= 4.4e-6 * want.norm()
