@@ -339,6 +339,8 @@ def _row_type(x):
     st = x.stride()
     if st[2] != 1 or (heads > 1 and st[1] != hd):
         raise ValueError("the heads of a row must be contiguous")
+    if rows > 1 and st[0] < heads * hd:  # an expanded tensor's 0 would mean packed rows below
+        raise ValueError("rows must not overlap")
     return code, (st[0] if rows > 1 else 0)
 
 
@@ -362,6 +364,8 @@ class KvQ8Cache:
         if k.shape != v.shape or k.stride() != v.stride():
             raise ValueError("k and v must have the same shape and strides")
         pages, kv, page, hd = k.shape
+        if any(n > 1 and st < hd for n, st in zip(k.shape[:3], k.stride())):  # (strides of 0 would mean packed pages below)
+            raise ValueError("codes must not overlap")
         self.shape = (pages, kv, page, hd)
         self.tensors = (k, v, k_scale, v_scale)  # kept alive
         self.c = _KvQ8CacheC(k.data_ptr(), v.data_ptr(), _vector(k_scale, "k_scale", "float32", pages * kv),
@@ -539,6 +543,8 @@ class Context:
         rows, vocab = logits.shape
         if _dtype(logits) != "float32" or (vocab > 1 and logits.stride(1) != 1):
             raise ValueError("logits must be float32 [rows][vocab], the last stride 1")
+        if rows > 1 and logits.stride(0) < vocab:  # an expanded row's 0 would mean packed rows below
+            raise ValueError("rows of logits must not overlap")
         self.check(self.lib.kib_sample_f32(self.h, ptr(logits), rows, vocab, logits.stride(0) if rows > 1 else 0,
                                            _vector(uniform, "uniform", "float32", rows),
                                            _vector(temperature, "temperature", "float32", rows),
