@@ -352,6 +352,14 @@ def _vector(x, name, dtype, size):
     return x.data_ptr()
 
 
+def _one_device(*tensors) -> int:
+    """The GPU that the tensors are on; -1: host memory."""
+    at = {x.get_device() for x in tensors if x is not None}
+    if len(at) != 1:
+        raise ValueError("tensors must be on one device")
+    return at.pop()
+
+
 class KvQ8Cache:
     """A paged 8-bit KV cache over the caller's tensors (kib_kvq8_cache): codes
     k, v int8 [pages][kv_heads][page_tokens][head_dim] with any strides whose
@@ -368,6 +376,7 @@ class KvQ8Cache:
             raise ValueError("codes must not overlap")
         self.shape = (pages, kv, page, hd)
         self.tensors = (k, v, k_scale, v_scale)  # kept alive
+        self.device = _one_device(*self.tensors)
         self.c = _KvQ8CacheC(k.data_ptr(), v.data_ptr(), _vector(k_scale, "k_scale", "float32", pages * kv),
                              _vector(v_scale, "v_scale", "float32", pages * kv), pages, kv, page, hd, *k.stride()[:3])
 
@@ -384,6 +393,7 @@ class KvQ8Batch:
                 block_table.shape[1] > 1 and block_table.stride(1) != 1):
             raise ValueError("block_table must be int32 [sequences][pages], rows contiguous")
         self.tensors = (block_table, lengths, row_start)
+        self.device = _one_device(*self.tensors)
         if n > 1 and block_table.stride(0) != block_table.shape[1]:
             raise ValueError("block_table must be contiguous")
         self.rows = rows
@@ -401,6 +411,7 @@ class Rope:
     def __init__(self, inv_freq, sections=(0, 0, 0, 0), positions=None):
         pairs = inv_freq.numel()
         self.tensors = (inv_freq, positions)
+        self.device = _one_device(*self.tensors)
         self.positions = positions
         self.c = _RopeC(_vector(inv_freq, "inv_freq", "float32", pairs), pairs, (c_uint64 * 4)(*sections),
                         None if positions is None else _vector(positions, "positions", "int32", positions.numel()))
@@ -416,6 +427,7 @@ class Context:
         if rc != KIB_OK:
             raise KibError(rc, "kib_create failed (no sm_100 device?)")
         self.h = h
+        self.device = device
         self.children = weakref.WeakSet()  # models on this context: freed before it
         self._workspace = (None, 0)  # attention's, grown on demand
 
@@ -442,6 +454,13 @@ class Context:
     def call(self, name, *args):
         fn = getattr(self.lib, name)
         self.check(fn(self.h, *[ptr(a) if not isinstance(a, (float, int)) or isinstance(a, bool) else a for a in args]))
+
+    def _here(self, *objects):
+        """Refuses tensors, caches, batches and rotations that are not on this
+        context's GPU: a kernel would fault on their addresses."""
+        for x in objects:
+            if x is not None and (x.get_device() if hasattr(x, "get_device") else x.device) != self.device:
+                raise ValueError(f"tensors must be on the context's device {self.device}")
 
     # graph scope (begin_graph / commit_graph)
     def begin_graph(self):
@@ -486,6 +505,7 @@ class Context:
                 raise ValueError("q and q_out must be [rows][heads][head_dim] of the type of k")
         if rope is not None and rope.positions is not None and rope.positions.numel() != 4 * batch.rows:
             raise ValueError("positions must be [4][rows]")
+        self._here(cache, batch, rope, k, v, q, q_out)
         self.check(self.lib.kib_kvq8_append(self.h, byref(cache.c), byref(batch.c), byref(rope.c) if rope else None,
                                             kind, heads, ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(q_out), os_,
                                             _stream(stream)))
@@ -497,6 +517,7 @@ class Context:
         for x in (k_out, v_out):
             if tuple(x.shape) != want or not x.is_contiguous() or x.dtype != k_out.dtype:
                 raise ValueError(f"outputs must be contiguous {want} of one type")
+        self._here(cache, page_ids, k_out, v_out)
         self.check(self.lib.kib_kvq8_read_pages(self.h, byref(cache.c), _vector(page_ids, "page_ids", "int32", want[0]),
                                                 want[0], kind, ptr(k_out), ptr(v_out), _stream(stream)))
 
@@ -521,6 +542,7 @@ class Context:
         shape = q.shape
         if okind != kind or shape != out.shape or shape[0] != batch.rows or shape[2] != cache.shape[3]:
             raise ValueError("q and out must be [rows][heads][head_dim] of one type")
+        self._here(cache, batch, q, out, workspace)
         if workspace is None:
             need = self._kvq8_need(cache, batch, kind, shape[1])
             if need > self._workspace[1]:
@@ -545,6 +567,7 @@ class Context:
             raise ValueError("logits must be float32 [rows][vocab], the last stride 1")
         if rows > 1 and logits.stride(0) < vocab:  # an expanded row's 0 would mean packed rows below
             raise ValueError("rows of logits must not overlap")
+        self._here(logits, uniform, token_out, prob_out, temperature, top_k, top_p, min_p)
         self.check(self.lib.kib_sample_f32(self.h, ptr(logits), rows, vocab, logits.stride(0) if rows > 1 else 0,
                                            _vector(uniform, "uniform", "float32", rows),
                                            _vector(temperature, "temperature", "float32", rows),

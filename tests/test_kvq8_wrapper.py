@@ -62,3 +62,25 @@ def test_expanded_tensors_are_not_taken_for_packed_ones(ctx):
     ctx.sample(torch.zeros(ROWS, 120)[:, :100], torch.zeros(ROWS), i32(ROWS))
     ctx.sample(torch.zeros(1, 100).expand(1, 100), torch.zeros(1), i32(1))
     assert [c[1][4] for c in ctx.lib.calls] == [120, 0]
+
+
+def test_tensors_on_another_device_are_refused(ctx):
+    """A kernel would fault on a host tensor's address."""
+    full = lambda heads: torch.zeros(ROWS, heads, HD)  # noqa: E731
+    ctx.device = 0
+    rope = kib.Rope(torch.ones(8))
+    for call in (lambda: ctx.kvq8_append(cache(), batch(), full(KV), full(KV), rope=rope),
+                 lambda: ctx.kvq8_attention(cache(), batch(), full(4), full(4), 0.1),
+                 lambda: ctx.kvq8_attention(cache(), batch(), full(4), full(4), 0.1, workspace=torch.zeros(4096, dtype=torch.uint8)),
+                 lambda: ctx.kvq8_read_pages(cache(), i32(1), torch.zeros(1, KV, PAGE, HD), torch.zeros(1, KV, PAGE, HD)),
+                 lambda: ctx.sample(torch.zeros(ROWS, 100), torch.zeros(ROWS), i32(ROWS))):
+        with pytest.raises(ValueError, match="device"):
+            call()
+    assert not ctx.lib.calls
+
+    class Elsewhere(torch.Tensor):
+        def get_device(self):
+            return 1
+
+    with pytest.raises(ValueError, match="device"):
+        kib.KvQ8Cache(codes(), codes(), torch.zeros(4, KV), torch.zeros(4, KV).as_subclass(Elsewhere))
