@@ -332,6 +332,10 @@ int kib_kvq8_read_pages(kib_ctx* ctx, const kib_kvq8_cache* cache, const int32_t
  * bytes, 256-byte aligned; calls that may overlap need one each. */
 int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_batch* batch, int type,
                                  uint64_t heads, uint64_t* bytes);
+/* Whether an attention call that was captured into a CUDA graph used this
+ * workspace (its replays will: the memory has to outlive the graph), and
+ * whether the stream is being captured now (then nothing may be allocated). */
+int kib_kvq8_attention_captured(kib_ctx* ctx, const void* workspace, void* stream, int* captured, int* capturing);
 int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_batch* batch, int type,
                        uint64_t heads, const void* q, uint64_t q_stride, float scale, void* out, uint64_t out_stride,
                        void* workspace, uint64_t workspace_bytes, void* stream);

@@ -5,6 +5,7 @@
 
 #include <cstdlib>
 #include <string>
+#include <vector>
 
 #include "../../include/kib.h"
 #include "kquant_gemv.cuh"
@@ -21,6 +22,7 @@ struct kib_ctx {
   float* d_cand_sum = nullptr;
   int* d_cand_idx = nullptr;
   unsigned* d_counter = nullptr;
+  std::vector<const void*> captured;  // workspaces of attention calls that were captured into graphs
 };
 
 namespace kib {

@@ -558,6 +558,11 @@ int finish(kib_ctx* ctx, void* stream, const char* what) {
   return check_cuda(ctx, cudaGetLastError(), what);
 }
 
+bool is_capturing(cudaStream_t st) {
+  cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(st, &s) == cudaSuccess && s != cudaStreamCaptureStatusNone;
+}
+
 #define KIB_TRY(expr)          \
   do {                         \
     const int st_ = (expr);    \
@@ -687,6 +692,14 @@ int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, cons
   return KIB_OK;
 }
 
+int kib_kvq8_attention_captured(kib_ctx* ctx, const void* workspace, void* stream, int* captured, int* capturing) {
+  KIB_REQUIRE_CTX(ctx);
+  KIB_ARG(captured && capturing, "kvq8_attention_captured: null result");
+  *captured = workspace && std::find(ctx->captured.begin(), ctx->captured.end(), workspace) != ctx->captured.end();
+  *capturing = is_capturing(op_stream(ctx, stream));
+  return KIB_OK;
+}
+
 int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_batch* batch, int type,
                        uint64_t heads, const void* q, uint64_t q_stride, float scale, void* out, uint64_t out_stride,
                        void* workspace, uint64_t workspace_bytes, void* stream) {
@@ -712,6 +725,9 @@ int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8
   p.partial = static_cast<float*>(workspace);
   p.err = ctx->d_err;
   const cudaStream_t st = op_stream(ctx, stream);
+  // a graph will replay on this workspace
+  if (is_capturing(st) && workspace && std::find(ctx->captured.begin(), ctx->captured.end(), workspace) == ctx->captured.end())
+    ctx->captured.push_back(workspace);
   const bool many = any_many(p.c, p.b, p.group, ctx->num_sms);
   // one sequence of many rows needs one path; a mixed batch takes both, each its own sequences
   p.few_limit = many ? (p.b.sequences == 1 ? 0 : kFewLimit) : 0x7fffffff;

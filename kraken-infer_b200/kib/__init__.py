@@ -242,6 +242,7 @@ def _declare(lib):
         "kib_kvq8_read_pages": (c_int, [_P, POINTER(_KvQ8CacheC), _P, _U64, c_int, _P, _P, _P]),
         "kib_kvq8_attention_workspace": (c_int, [_P, POINTER(_KvQ8CacheC), POINTER(_KvQ8BatchC), c_int, _U64,
                                                  POINTER(c_uint64)]),
+        "kib_kvq8_attention_captured": (c_int, [_P, _P, _P, POINTER(c_int), POINTER(c_int)]),
         "kib_kvq8_attention": (c_int, [_P, POINTER(_KvQ8CacheC), POINTER(_KvQ8BatchC), c_int, _U64, _P, _U64, c_float,
                                        _P, _U64, _P, _U64, _P]),
         "kib_sample_f32": (c_int, [_P, _P, _U64, _U64, _U64, _P, _P, _P, _P, _P, _P, _P, _P]),
@@ -430,13 +431,15 @@ class Context:
         self.device = device
         self.children = weakref.WeakSet()  # models on this context: freed before it
         self._workspace = (None, 0)  # attention's, grown on demand
+        self._kept = []  # outgrown ones that captured graphs replay on
 
     def close(self):
         if getattr(self, "h", None):
             for c in list(self.children):
                 c.close()
-            if self._workspace[0]:
-                self.lib.kib_free_buffer(self.h, self._workspace[0])
+            for w in self._kept + [self._workspace[0]]:
+                if w:
+                    self.lib.kib_free_buffer(self.h, w)
             self.lib.kib_destroy(self.h)
             self.h = None
 
@@ -533,10 +536,28 @@ class Context:
             batch.workspace[key] = need.value
         return batch.workspace[key]
 
+    def _grow_workspace(self, need, stream):
+        old = self._workspace[0]
+        captured, capturing = c_int(), c_int()
+        self.check(self.lib.kib_kvq8_attention_captured(self.h, old, _stream(stream), byref(captured), byref(capturing)))
+        if capturing.value:
+            raise ValueError(f"a call that is being captured cannot allocate: give it a workspace of {need} bytes")
+        self._workspace = (None, 0)
+        if captured.value:
+            self._kept.append(old)
+        elif old:
+            self.check(self.lib.kib_free_buffer(self.h, old))
+        h = c_void_p()
+        self.check(self.lib.kib_make_buffer(self.h, need, byref(h)))
+        self._workspace = (h.value, need)
+
     def kvq8_attention(self, cache: KvQ8Cache, batch: KvQ8Batch, q, out, scale, workspace=None, stream=None):
         """Causal attention of q [rows][heads][head_dim] over the cache.
         workspace: a device tensor of kvq8_attention_workspace bytes; None: one
-        that this context keeps and grows (then calls must not overlap)."""
+        that this context keeps and grows (then calls must not overlap, replays
+        of captured ones included; a call that is being captured cannot grow it
+        and is refused where that would be needed; what a captured call has used
+        stays until the context is closed)."""
         kind, qs = _row_type(q)
         okind, os_ = _row_type(out)
         shape = q.shape
@@ -546,12 +567,7 @@ class Context:
         if workspace is None:
             need = self._kvq8_need(cache, batch, kind, shape[1])
             if need > self._workspace[1]:
-                old, self._workspace = self._workspace[0], (None, 0)
-                if old:
-                    self.check(self.lib.kib_free_buffer(self.h, old))
-                h = c_void_p()
-                self.check(self.lib.kib_make_buffer(self.h, need, byref(h)))
-                self._workspace = (h.value, need)
+                self._grow_workspace(need, stream)
             where, size = self._workspace
         else:
             where, size = ptr(workspace), workspace.numel() * workspace.element_size()

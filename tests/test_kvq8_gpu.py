@@ -615,3 +615,37 @@ def test_attention_long_prompts_keep_fp32_accuracy(ctx, hd, spread, alike):
         s.masked_fill_(torch.arange(n, device="cuda") > rows[:, None, None, None], -torch.inf)
         want = torch.einsum("rgxk,gkd->rgxd", s.softmax(-1), v).reshape(64, heads, hd)
         assert (out[rows] - want).norm() <= 4.4e-6 * want.norm()
+
+
+@gpu
+def test_a_graph_on_the_contexts_workspace_outlives_its_growth():
+    """A small call captured on the context's own workspace, then a larger call
+    that outgrows it, then the replay."""
+    own = kib.Context(0)
+    small, large = Case([300, 140], [1, 1], 8, 2, 128, 32, seed=15), Case([900, 700], [900, 300], 8, 2, 128, 32, seed=16)
+    q = small.q.cuda()
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def step(stream):
+        own.kvq8_attention(small.cache, small.batch, q, out, 0.09, stream=stream)
+
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(ValueError, match="captured"):  # nothing there yet, and no allocation now
+        with torch.cuda.graph(g, stream=side):
+            step(torch.cuda.current_stream().cuda_stream)
+    step(side.cuda_stream)
+    torch.cuda.synchronize()
+    want, at = out.clone(), own._workspace[0]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        step(torch.cuda.current_stream().cuda_stream)
+    run_attend(own, large, 0.09)
+    assert own._workspace[0] != at and own._kept == [at]  # only then may the graph run
+    out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    del g
+    own.close()

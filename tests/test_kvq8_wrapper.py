@@ -22,7 +22,7 @@ class Entries:
 @pytest.fixture
 def ctx():
     c = kib.Context.__new__(kib.Context)
-    c.lib, c.h, c.device, c._workspace, c.children = Entries(), None, -1, (None, 0), ()  # -1: tensors in host memory
+    c.lib, c.h, c.device, c._workspace, c._kept, c.children = Entries(), None, -1, (None, 0), [], ()  # -1: tensors in host memory
     return c
 
 
@@ -84,3 +84,74 @@ def test_tensors_on_another_device_are_refused(ctx):
 
     with pytest.raises(ValueError, match="device"):
         kib.KvQ8Cache(codes(), codes(), torch.zeros(4, KV), torch.zeros(4, KV).as_subclass(Elsewhere))
+
+
+class Memory(Entries):
+    """The entries that the context's own workspace needs, with buffers that are only numbers."""
+
+    def __init__(self):
+        super().__init__()
+        self.need, self.live, self.made, self.used, self.captured, self.capturing = 0, set(), 0, [], set(), False
+
+    def kib_kvq8_attention_workspace(self, h, cache, batch, kind, heads, need):
+        need._obj.value = self.need
+        return kib.KIB_OK
+
+    def kib_make_buffer(self, h, size, out):
+        assert not self.capturing
+        self.made += 1
+        out._obj.value = 4096 * self.made
+        self.live.add(out._obj.value)
+        return kib.KIB_OK
+
+    def kib_free_buffer(self, h, where):
+        assert not self.capturing
+        self.live.remove(where)
+        return kib.KIB_OK
+
+    def kib_kvq8_attention_captured(self, h, where, stream, captured, capturing):
+        captured._obj.value, capturing._obj.value = where in self.captured, self.capturing
+        return kib.KIB_OK
+
+    def kib_kvq8_attention(self, *args):
+        where = args[10]
+        assert where in self.live
+        self.used.append(where)
+        if self.capturing:
+            self.captured.add(where)
+        return kib.KIB_OK
+
+    def kib_destroy(self, h):
+        pass
+
+
+def test_a_workspace_that_a_graph_replays_on_is_not_freed(ctx):
+    """The context's own workspace: outgrown, it goes, but not while a captured
+    call's graph holds its address; and nothing is allocated during a capture."""
+    ctx.lib = m = Memory()
+    q = torch.zeros(ROWS, 4, HD)
+
+    def call(need, capturing=False):
+        m.need, m.capturing = need, capturing
+        try:
+            ctx.kvq8_attention(cache(), batch(), q, torch.zeros_like(q), 0.1, stream=7)
+        finally:
+            m.capturing = False
+
+    call(100)
+    call(200)
+    assert len(m.live) == 1 and len(m.used) == 2  # outgrown and never captured: freed
+    call(150, capturing=True)
+    graph = m.used[-1]
+    call(1000)
+    assert graph in m.live and m.used[-1] != graph  # a replay may still write there
+    call(5000)
+    assert graph in m.live and len(m.live) == 2
+    with pytest.raises(ValueError, match="workspace of 9000 bytes"):
+        call(9000, capturing=True)
+    call(4000, capturing=True)
+    call(9000)
+    assert len(m.live) == 3
+    ctx.h = 1
+    ctx.close()
+    assert not m.live
