@@ -324,7 +324,8 @@ int kib_kvq8_read_pages(kib_ctx* ctx, const kib_kvq8_cache* cache, const int32_t
                         void* k_out, void* v_out, void* stream);
 /* Causal attention of every row over its sequence's keys 0 .. its own
  * position: out = softmax(scale * q . K) V per head, query head h on KV head
- * h / (heads / kv_heads).  Rows without any key give zeros.  q and out
+ * h / (heads / kv_heads).  Rows without any key give zeros, rows whose scores
+ * are not all numbers NaN.  q and out
  * [rows][heads][head_dim] of one type: F32 rows take q and the softmax weights
  * as two halves each (22 bits), F16 rows the weights as one half; sums and
  * statistics are fp32: an F32 result is off by about 1e-6 of itself, by up to

@@ -645,7 +645,10 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
       for (int e = 0; e < V; ++e) x[e] = 0.0f;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        if (s_m[w][rr] == -INFINITY) continue;  // no tile for this warp
+        if (s_m[w][rr] == -INFINITY) {
+          sum += s_l[w][rr];  // 0: no key for this warp; NaN: scores that are no numbers, as the result then is
+          continue;
+        }
         const float f = ex2(s_m[w][rr] - top);
         sum += f * s_l[w][rr];
 #pragma unroll

@@ -649,3 +649,42 @@ def test_a_graph_on_the_contexts_workspace_outlives_its_growth():
     assert torch.equal(out, want)
     del g
     own.close()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("lengths,rows", [([300, 90], [1, 1]), ([2500, 40], [3, 1]), ([400, 150], [140, 140]), ([3000, 2900], [2000, 900])])
+def test_attention_rows_that_are_not_numbers(ctx, dtype, lengths, rows):
+    """A query with a NaN, or an infinity (whose scores are infinite of both
+    signs), gives NaN, whichever kernel and however many CTAs take the row; its
+    neighbours and other heads are as ever."""
+    c = Case(lengths, rows, 8, 2, 128, 32, dtype, seed=41)
+    bad = {(0, 1): math.nan, (rows[0] - 1, 6): math.inf, (c.rows - 1, 3): -math.inf, (c.rows // 2, 0): math.nan}
+    clean = c.q.clone()
+    for (row, head), x in bad.items():
+        c.q[row, head, 77] = x
+    got = run_attend(ctx, c, 0.09)
+    c.q = clean
+    plain = run_attend(ctx, c, 0.09)
+    for row, head in bad:
+        assert got[row, head].isnan().all()
+        got[row, head] = plain[row, head]
+    # a neighbour's reference may move at another tile: 22-bit (half: 11-bit) weights, rounded differently
+    step = 2.0 ** -10 if dtype == "f16" else 2.0 ** -18
+    assert (got - plain).abs().max() <= step * 127 * max(float(s.max()) for s in c.dev[3:])
+
+
+@gpu
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("lengths,rows", [([300, 90], [1, 1]), ([5000, 40], [2, 1]), ([400, 150], [140, 140])])
+def test_attention_over_a_page_whose_scale_is_not_a_number(ctx, lengths, rows, which):
+    """Every row that sees such a page gives NaN, wherever the page's keys fall
+    among the warps and CTAs; sequences without it are as ever."""
+    for at in (0, 1, lengths[0] // 32):
+        c = Case(lengths, rows, 8, 2, 128, 32, seed=42)
+        clean = run_attend(ctx, c, 0.09)
+        c.dev[which][c.table[0, at], 1] = math.nan
+        got = run_attend(ctx, c, 0.09)
+        sees = torch.from_numpy(c.positions(0) >= at * 32).cuda()
+        assert got[:rows[0], 4:][sees].isnan().all()
+        assert torch.equal(got[rows[0]:], clean[rows[0]:]) and not got[:rows[0], :4].isnan().any()
