@@ -36,10 +36,11 @@ KIB_DEV float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.0f;
 }
 
-// code = rint(x / s) held to [-127, 127]; NaN gives 0.
+// code = rint(x / s) held to [-127, 127]; NaN (an infinity over a scale of 0
+// among it) gives 0.
 KIB_DEV int quantise(float x, float inv) {
-  const float y = fminf(fmaxf(__fmul_rn(x, inv), -127.0f), 127.0f);
-  return x == x ? __float2int_rn(y) : 0;
+  const float y = __fmul_rn(x, inv);
+  return y == y ? __float2int_rn(fminf(fmaxf(y, -127.0f), 127.0f)) : 0;
 }
 
 // A CTA takes a span of positions, whole pages (64 positions, or a page of
@@ -244,7 +245,17 @@ __global__ void __launch_bounds__(512, AppendShape<T, HD>::MINB) kvq8_append_ker
   if (page >= 0) {
     const float now = fmaxf(old, __fmul_rn(big, 1.0f / 127.0f));
     if (wi == 0 && lane == 0) *scale = now;
-    const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f;
+    // the reciprocal of a scale below 2^-128 would be infinite: such rows and their scale are taken 2^64 times
+    const bool tiny = now < 0x1p-100f;
+    const float inv = now > 0.0f ? __fdiv_rn(1.0f, tiny ? now * 0x1p64f : now) : 0.0f;
+    if (tiny) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[i][n][e] *= 0x1p64f;
+    }
     const float ratio = now > 0.0f ? __fdiv_rn(old, now) : 0.0f;
     const bool again = now != old || now == 0.0f;
     int8_t* codes = (is_v ? p.c.v : p.c.k) + page * p.c.page_stride + head * p.c.head_stride + cl * E;

@@ -688,3 +688,28 @@ def test_attention_over_a_page_whose_scale_is_not_a_number(ctx, lengths, rows, w
         sees = torch.from_numpy(c.positions(0) >= at * 32).cuda()
         assert got[:rows[0], 4:][sees].isnan().all()
         assert torch.equal(got[rows[0]:], clean[rows[0]:]) and not got[:rows[0], :4].isnan().any()
+
+
+@gpu
+@pytest.mark.parametrize("size", [1e-30, 3e-36, 2e-37, 1e-38, 2e-41, 1e-43, 1e-45])
+def test_append_of_tiny_values(ctx, size):
+    """Pages whose largest value is so small that the scale is subnormal (its
+    reciprocal infinite) or 0.  A scale is then known to half of 2^-149 only, and
+    so is every value read back to 127 of those and half a scale; zeros stay 0."""
+    c = Case([20], [20], kv=2, heads=1, seed=43)
+    c.v = (c.k.double().clamp(-2, 2) / 2 * size).float()
+    c.v[::3, :, ::5] = 0.0
+    c.v[2, 1, 7] = math.inf
+    run_append(ctx, c, pairs=0)
+    v = c.v.numpy().astype(np.float64)
+    ulp = 2.0 ** -149
+    for head in range(2):
+        for page, lo, hi in ((c.table[0, 0], 0, 16), (c.table[0, 1], 16, 20)):
+            part = v[lo:hi, head]
+            big = np.where(np.isfinite(part), np.abs(part), 0).max()
+            s = float(c.dev[3][page, head].double())
+            assert abs(s - big / 127) <= 1e-6 * big / 127 + ulp / 2
+            got = c.dev[1][page, head, :hi - lo].cpu().numpy().astype(np.int64)
+            assert (got[part == 0] == 0).all() and (got[np.isinf(part)] == (127 if s > 0 else 0)).all()
+            ok = np.isfinite(part)
+            assert (np.abs(got * s - part)[ok] <= 0.5 * s * (1 + 1e-4) + (128 * ulp if s < 1e-36 else 0)).all()
