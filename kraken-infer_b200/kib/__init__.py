@@ -377,7 +377,7 @@ class KvQ8Cache:
             raise ValueError("codes must not overlap")
         self.shape = (pages, kv, page, hd)
         self.tensors = (k, v, k_scale, v_scale)  # kept alive
-        self.device = _one_device(*self.tensors)
+        self.get_device = _one_device(*self.tensors).__index__  # asked like a tensor
         self.c = _KvQ8CacheC(k.data_ptr(), v.data_ptr(), _vector(k_scale, "k_scale", "float32", pages * kv),
                              _vector(v_scale, "v_scale", "float32", pages * kv), pages, kv, page, hd, *k.stride()[:3])
 
@@ -394,7 +394,7 @@ class KvQ8Batch:
                 block_table.shape[1] > 1 and block_table.stride(1) != 1):
             raise ValueError("block_table must be int32 [sequences][pages], rows contiguous")
         self.tensors = (block_table, lengths, row_start)
-        self.device = _one_device(*self.tensors)
+        self.get_device = _one_device(*self.tensors).__index__  # asked like a tensor
         if n > 1 and block_table.stride(0) != block_table.shape[1]:
             raise ValueError("block_table must be contiguous")
         self.rows = rows
@@ -412,7 +412,7 @@ class Rope:
     def __init__(self, inv_freq, sections=(0, 0, 0, 0), positions=None):
         pairs = inv_freq.numel()
         self.tensors = (inv_freq, positions)
-        self.device = _one_device(*self.tensors)
+        self.get_device = _one_device(*self.tensors).__index__  # asked like a tensor
         self.positions = positions
         self.c = _RopeC(_vector(inv_freq, "inv_freq", "float32", pairs), pairs, (c_uint64 * 4)(*sections),
                         None if positions is None else _vector(positions, "positions", "int32", positions.numel()))
@@ -461,8 +461,9 @@ class Context:
     def _here(self, *objects):
         """Refuses tensors, caches, batches and rotations that are not on this
         context's GPU: a kernel would fault on their addresses."""
+        here = self.device
         for x in objects:
-            if x is not None and (x.get_device() if hasattr(x, "get_device") else x.device) != self.device:
+            if x is not None and x.get_device() != here:
                 raise ValueError(f"tensors must be on the context's device {self.device}")
 
     # graph scope (begin_graph / commit_graph)
