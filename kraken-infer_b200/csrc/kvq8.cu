@@ -10,6 +10,7 @@
 #include <cudaTypedefs.h>
 
 #include "kvq8_many.cuh"
+#include "per_device.hpp"
 
 namespace kib {
 namespace {
@@ -316,12 +317,14 @@ __global__ void __launch_bounds__(256) kvq8_read_kernel(const __grid_constant__ 
   }
 }
 
-// Dynamic shared memory above 48 KB has to be asked for, once per kernel.
+// Dynamic shared memory above 48 KB has to be asked for, once per kernel and device.
 template <typename... KArgs>
-cudaError_t allow_smem(void (*kernel)(KArgs...), size_t bytes, bool* done) {
-  if (*done) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-  *done = e == cudaSuccess;
+cudaError_t allow_smem(int device, void (*kernel)(KArgs...), size_t bytes, PerDevice* done) {
+  cudaError_t e = cudaSuccess;
+  done->once(device, [&] {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    return e == cudaSuccess;
+  });
   return e;
 }
 
@@ -369,11 +372,11 @@ bool codes_map(CUtensorMap* map, const int8_t* base, const Kvq8Cache& c) {
 }
 
 template <typename T, int HD, int NT>
-cudaError_t few_launch(const Kvq8AttnParams& p, int num_sms, cudaStream_t st) {
-  static bool ready = false;
-  cudaError_t e = allow_smem(kvq8_few_kernel<T, HD, NT>, few_smem<T, HD, NT>(), &ready);
+cudaError_t few_launch(const Kvq8AttnParams& p, const kib_ctx* ctx, cudaStream_t st) {
+  static PerDevice ready;
+  cudaError_t e = allow_smem(ctx->device, kvq8_few_kernel<T, HD, NT>, few_smem<T, HD, NT>(), &ready);
   if (e != cudaSuccess) return e;
-  const int ctas = std::min(num_sms, kMergeMaxCtas);
+  const int ctas = std::min(ctx->num_sms, kMergeMaxCtas);
   CUtensorMap kmap, vmap;
   if (!codes_map(&kmap, p.c.k, p.c) || !codes_map(&vmap, p.c.v, p.c)) return cudaErrorInvalidValue;
   kvq8_few_kernel<T, HD, NT><<<ctas, few_warps<HD, NT>() * 32, few_smem<T, HD, NT>(), st>>>(kmap, vmap, p);
@@ -389,13 +392,13 @@ int few_nt(const Kvq8Cache& c, const Kvq8Batch& b, int group) {
   return static_cast<int>(std::min<int64_t>((static_cast<int64_t>(b.max_rows) * group + 7) / 8, few_max_nt(c.head_dim)));
 }
 template <typename T, int HD>
-cudaError_t few_launch_nt(const Kvq8AttnParams& p, int num_sms, cudaStream_t st) {
+cudaError_t few_launch_nt(const Kvq8AttnParams& p, const kib_ctx* ctx, cudaStream_t st) {
   const int nt = few_nt(p.c, p.b, p.group);
-  if (nt == 1) return few_launch<T, HD, 1>(p, num_sms, st);
+  if (nt == 1) return few_launch<T, HD, 1>(p, ctx, st);
   if constexpr (few_max_nt(HD) > 2) {
-    if (nt == 3) return few_launch<T, HD, 3>(p, num_sms, st);
+    if (nt == 3) return few_launch<T, HD, 3>(p, ctx, st);
   }
-  return few_launch<T, HD, 2>(p, num_sms, st);
+  return few_launch<T, HD, 2>(p, ctx, st);
 }
 
 size_t few_workspace(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_sms) {
@@ -452,11 +455,12 @@ ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_len
 }
 
 template <typename T, int HD>
-cudaError_t many_launch(const Kvq8AttnParams& a, const ManyLayout& w, uint8_t* ws, int num_sms, int* err, cudaStream_t st) {
+cudaError_t many_launch(const Kvq8AttnParams& a, const ManyLayout& w, uint8_t* ws, const kib_ctx* ctx, cudaStream_t st) {
   constexpr int PL = sizeof(T) == 4 ? 2 : 1;
   using Sh = ManyShape<HD, PL>;
-  static bool ready = false;
-  cudaError_t e = allow_smem(kvq8_many_kernel<HD, PL>, Sh::kSmem, &ready);
+  const int num_sms = ctx->num_sms;
+  static PerDevice ready;
+  cudaError_t e = allow_smem(ctx->device, kvq8_many_kernel<HD, PL>, Sh::kSmem, &ready);
   if (e != cudaSuccess) return e;
   Kvq8ManyParams p;
   p.a = a;
@@ -474,7 +478,7 @@ cudaError_t many_launch(const Kvq8AttnParams& a, const ManyLayout& w, uint8_t* w
   p.count = reinterpret_cast<int*>(ws + w.count);
   p.sums = reinterpret_cast<float4*>(ws + w.sums);
   p.ctas = num_sms;
-  p.err = err;
+  p.err = ctx->d_err;
   const int kvh = a.c.kv_heads;
   CUtensorMap kmap, vmap;
   if (!tile_map(&kmap, p.k16, static_cast<int64_t>(kvh) * w.tot_pad, HD, kManyKeys) ||
@@ -649,8 +653,8 @@ int kib_kvq8_append(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_ba
   cudaError_t e = cudaSuccess;
 #define CALL(T, HD)                                                                                \
   do {                                                                                             \
-    static bool ready = false;                                                                     \
-    e = allow_smem(kvq8_append_kernel<T, HD>, static_cast<size_t>(128) * (HD / 2) * sizeof(float2), &ready); \
+    static PerDevice ready;                                                                        \
+    e = allow_smem(ctx->device, kvq8_append_kernel<T, HD>, static_cast<size_t>(128) * (HD / 2) * sizeof(float2), &ready); \
     if (e == cudaSuccess) kvq8_append_kernel<T, HD><<<grid, threads, smem, op_stream(ctx, stream)>>>(p);   \
   } while (0)
   KVQ8_DISPATCH(type, p.c.head_dim, CALL);
@@ -744,13 +748,13 @@ int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8
   p.few_limit = many ? (p.b.sequences == 1 ? 0 : kFewLimit) : 0x7fffffff;
   cudaError_t e = cudaSuccess;
   if (p.few_limit > 0) {
-#define CALL(T, HD) e = few_launch_nt<T, HD>(p, ctx->num_sms, st)
+#define CALL(T, HD) e = few_launch_nt<T, HD>(p, ctx, st)
     KVQ8_DISPATCH(type, p.c.head_dim, CALL);
 #undef CALL
   }
   if (many && e == cudaSuccess) {
     const ManyLayout m = many_layout(p.c, p.b, static_cast<int64_t>(batch->total_length), type, p.group, ctx->num_sms);
-#define CALL(T, HD) e = many_launch<T, HD>(p, m, static_cast<uint8_t*>(workspace), ctx->num_sms, ctx->d_err, st)
+#define CALL(T, HD) e = many_launch<T, HD>(p, m, static_cast<uint8_t*>(workspace), ctx, st)
     KVQ8_DISPATCH(type, p.c.head_dim, CALL);
 #undef CALL
   }

@@ -16,6 +16,7 @@
 #include <cooperative_groups.h>
 
 #include "kib_ctx.cuh"
+#include "per_device.hpp"
 
 namespace cg = cooperative_groups;
 
@@ -698,15 +699,16 @@ int cluster_of(const SampleParams& p, int num_sms) {
   return c;
 }
 
-cudaError_t sample_launch(const SampleParams& p, int num_sms, cudaStream_t st) {
-  static bool ready = false;
-  if (!ready) {
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(SampleShared)));
+cudaError_t sample_launch(const SampleParams& p, const kib_ctx* ctx, cudaStream_t st) {
+  static PerDevice ready;
+  cudaError_t e = cudaSuccess;
+  ready.once(ctx->device, [&] {
+    e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(SampleShared)));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    ready = true;
-  }
-  const unsigned c = static_cast<unsigned>(cluster_of(p, num_sms));
+    return e == cudaSuccess;
+  });
+  if (e != cudaSuccess) return e;
+  const unsigned c = static_cast<unsigned>(cluster_of(p, ctx->num_sms));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * c);
   cfg.blockDim = dim3(kThreads);
@@ -748,7 +750,7 @@ extern "C" int kib_sample_f32(kib_ctx* ctx, const float* logits, uint64_t rows, 
   p.token = token_out;
   p.prob = prob_out;
   const cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-  const cudaError_t e = sample_launch(p, ctx->num_sms, st);
+  const cudaError_t e = sample_launch(p, ctx, st);
   if (e != cudaSuccess) return check_cuda(ctx, e, "sample");
   if (!stream) return finish_op(ctx, "sample");
   return check_cuda(ctx, cudaGetLastError(), "sample");
