@@ -37,7 +37,7 @@ KIB_DEV Kvq8Seq kvq8_seq(const Kvq8Batch& b, int s) {
   Kvq8Seq q;
   q.first = max(0, min(b.row_start[s], b.rows));
   q.n = max(0, min(b.row_start[s + 1], b.rows) - q.first);
-  q.length = min(b.lengths[s], 1 << 30);
+  q.length = max(-(1 << 30), min(b.lengths[s], 1 << 30));
   return q;
 }
 

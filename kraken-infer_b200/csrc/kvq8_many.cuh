@@ -107,19 +107,18 @@ KIB_DEV ManySeq many_seq(const Kvq8AttnParams& p, int s) {
 }
 
 // Exclusive scan of v over the block's threads; *total gets the sum.
-template <typename V>
-KIB_DEV V many_scan(V v, V* s, V* total) {
+KIB_DEV int64_t many_scan(int64_t v, int64_t* s, int64_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  V inc = v;
+  int64_t inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const V n = __shfl_up_sync(0xffffffffu, inc, o);
+    const int64_t n = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += n;
   }
   __syncthreads();
   if (lane == 31) s[warp] = inc;
   __syncthreads();
-  V base = 0, all = 0;
+  int64_t base = 0, all = 0;
   for (int w = 0; w < warps; ++w) {
     if (w < warp) base += s[w];
     all += s[w];
@@ -140,39 +139,38 @@ __global__ void __launch_bounds__(kGatherThreads) kvq8_gather_kernel(const __gri
   __shared__ __align__(16) uint8_t s_raw[OFF > VB ? OFF : VB];
   int* s_off = reinterpret_cast<int*>(s_raw);
   uint8_t* s_v = s_raw;
-  __shared__ int64_t s_scan[kGatherThreads / 32];
-  __shared__ int s_scan32[kGatherThreads / 32];
+  __shared__ int64_t s_scan[kGatherThreads / 32];  // 64 bits: lengths and row starts may be wrong, their sums too
   const int tid = threadIdx.x, S = p.a.b.sequences, kvh = p.a.c.kv_heads, head = blockIdx.y;
   const bool plan = blockIdx.x + 1 == gridDim.x;
   if (plan && head) return;
 
   // first padded keys; in the planning CTA then first units
-  int base = 0;
+  int64_t base = 0;
   for (int s0 = 0; s0 < S; s0 += kGatherThreads) {
     const int s = s0 + tid;
-    const int v = s < S ? many_seq(p.a, s).pad : 0;
-    int all;
-    const int x = base + many_scan(v, s_scan32, &all);
+    const int64_t v = s < S ? many_seq(p.a, s).pad : 0;
+    int64_t all;
+    const int64_t x = base + many_scan(v, s_scan, &all);
     // a sequence that the workspace has no room for keeps no keys
-    if (s < S) s_off[s] = min(x, p.tot_pad);
-    base = min(base + all, p.tot_pad + 1);
+    if (s < S) s_off[s] = static_cast<int>(min(x, static_cast<int64_t>(p.tot_pad)));
+    base += all;
   }
-  if (tid == 0) s_off[S] = min(base, p.tot_pad);
+  if (tid == 0) s_off[S] = static_cast<int>(min(base, static_cast<int64_t>(p.tot_pad)));
   __syncthreads();
 
   if (plan) {
     for (int s = tid; s <= S; s += kGatherThreads) p.seq_off[s] = s_off[s];
     __syncthreads();
-    int units = 0;
+    int64_t all_units = 0;
     for (int s0 = 0; s0 < S; s0 += kGatherThreads) {
       const int s = s0 + tid;
-      const int v = s < S ? many_seq(p.a, s).tiles * kvh : 0;
-      int all;
-      const int x = units + many_scan(v, s_scan32, &all);
-      if (s < S) s_off[s] = x;
-      units += all;
+      const int64_t v = s < S ? static_cast<int64_t>(many_seq(p.a, s).tiles) * kvh : 0;
+      int64_t all;
+      const int64_t x = all_units + many_scan(v, s_scan, &all);
+      if (s < S) s_off[s] = static_cast<int>(min(x, static_cast<int64_t>(p.max_units)));
+      all_units += all;
     }
-    units = min(units, p.max_units);
+    const int units = static_cast<int>(min(all_units, static_cast<int64_t>(p.max_units)));
     if (tid == 0) s_off[S] = units, p.count[0] = units, p.count[1] = 0;
     __syncthreads();
     int64_t total = 0;

@@ -713,3 +713,41 @@ def test_append_of_tiny_values(ctx, size):
             assert (got[part == 0] == 0).all() and (got[np.isinf(part)] == (127 if s > 0 else 0)).all()
             ok = np.isfinite(part)
             assert (np.abs(got * s - part)[ok] <= 0.5 * s * (1 + 1e-4) + (128 * ulp if s < 1e-36 else 0)).all()
+
+
+@gpu
+def test_attention_of_few_rows_with_lengths_that_the_host_did_not_announce(ctx):
+    """Wrong lengths on the device read nothing outside the tensors: keys past
+    the table's span are none, positions before the first see nothing."""
+    c = Case([100, 64, 80, 33], [1, 3, 2, 1], 8, 2, 128, 16, seed=44)
+    want = run_attend(ctx, c, 0.1)
+    c.lengths_dev[1:].copy_(torch.tensor([1 << 30, -2 ** 31, -7], dtype=torch.int32))
+    got = run_attend(ctx, c, 0.1)
+    assert torch.equal(got[:1], want[:1]) and not got[4:].any() and got.isfinite().all()
+    # a length past the table sees every key of it
+    c.lengths_dev[1] = c.width * c.page + 2
+    assert torch.equal(got[1:4], run_attend(ctx, c, 0.1)[1:4])
+
+
+@gpu
+def test_attention_of_many_rows_with_lengths_that_the_host_did_not_announce(ctx):
+    """300 sequences whose lengths (and their sums, past 32 bits) the workspace
+    has no room for, row starts that go back and past the rows: the sequences
+    that fit are right, the others read nothing outside the tensors."""
+    n, rows = 300, 70
+    c = Case([200] + [rows] * (n - 1), [rows] * n, 4, 2, 64, 128, seed=45)
+    table = torch.full((n, 1 << 17), -1, dtype=torch.int32, device="cuda")  # spans 2^24 positions
+    table[:, :c.width] = torch.from_numpy(c.table).cuda()
+    starts = c.start.copy()
+    starts[200], starts[250], starts[n] = 100, 1 << 30, 2 ** 31 - 1
+    lengths = [200] + [1 << 30] * 149 + [-2 ** 31] * 75 + [1 << 24] * 75
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = kib.KvQ8Batch(table, i32(lengths), i32(starts.tolist()), c.rows, rows, total_length=rows * n + 200)
+    q = c.q.cuda()
+    out = torch.full_like(q, 77.0)
+    torch.cuda.synchronize()
+    ctx.kvq8_attention(c.cache, batch, q, out, 0.1)
+    torch.cuda.synchronize()
+    want, tol = oracle_attend(c, 0.1)
+    assert (np.abs(out[:rows].cpu().numpy() - want[:rows]).max(-1) <= tol[:rows]).all()
+    assert out.isfinite().all()
