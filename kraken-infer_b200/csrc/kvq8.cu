@@ -723,7 +723,7 @@ int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8
   Kvq8AttnParams p = {};
   KIB_TRY(make_cache(ctx, cache, &p.c));
   KIB_TRY(make_batch(ctx, batch, p.c, &p.b));
-  if (p.b.rows == 0) return KIB_OK;
+  if (p.b.sequences == 0 || p.b.rows == 0) return KIB_OK;
   KIB_ARG(q && out, "kvq8_attention: null rows");
   KIB_ARG(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 256))),
           "kvq8_attention: workspace too small or not 256-byte aligned");

@@ -751,3 +751,15 @@ def test_attention_of_many_rows_with_lengths_that_the_host_did_not_announce(ctx)
     want, tol = oracle_attend(c, 0.1)
     assert (np.abs(out[:rows].cpu().numpy() - want[:rows]).max(-1) <= tol[:rows]).all()
     assert out.isfinite().all()
+
+
+@gpu
+def test_rows_of_no_sequence_are_nothing_to_do(ctx):
+    c = Case([40], [20], seed=46)
+    q, none = c.q.cuda(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 7.0)
+    for rows in (20, 1):
+        batch = kib.KvQ8Batch(torch.zeros(0, 3, dtype=torch.int32, device="cuda"), none[:0], none, rows, rows)
+        ctx.kvq8_append(c.cache, batch, c.k.cuda()[:rows], c.v.cuda()[:rows])
+        ctx.kvq8_attention(c.cache, batch, q[:rows], out[:rows], 0.1)
+    assert (out == 7.0).all()
