@@ -401,9 +401,17 @@ cudaError_t few_launch_nt(const Kvq8AttnParams& p, const kib_ctx* ctx, cudaStrea
   return few_launch<T, HD, 2>(p, ctx, st);
 }
 
-size_t few_workspace(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_sms) {
-  return static_cast<size_t>(std::min(num_sms, kMergeMaxCtas)) * 2 * 8 * few_nt(c, b, group) *
-         static_cast<size_t>(c.head_dim + 2) * sizeof(float);
+// The workspace of the few-row path: records, then fp32 rows' sums.
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+size_t few_records(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_sms) {
+  return up256(static_cast<size_t>(std::min(num_sms, kMergeMaxCtas)) * 2 * 8 * few_nt(c, b, group) *
+               static_cast<size_t>(c.head_dim + 2) * sizeof(float));
+}
+size_t few_workspace(const Kvq8Cache& c, const Kvq8Batch& b, int type, int group, int num_sms) {
+  size_t bytes = few_records(c, b, group, num_sms);
+  if (type == KIB_TYPE_F32 && few_banks<float>(c.head_dim))
+    bytes += static_cast<size_t>(std::min(num_sms, kMergeMaxCtas)) * kFewMaxWarps * 8 * few_nt(c, b, group) * c.head_dim * sizeof(float);
+  return bytes;
 }
 
 // Rows (times the group) up to which a sequence is the few-row kernel's.
@@ -428,7 +436,6 @@ struct ManyLayout {
   size_t k16, v16, scales, seq_off, units, cum, cta_unit, split, count, sums, bytes;
   int64_t tot_pad, max_units;
 };
-size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_length, int type, int group, int num_sms) {
   ManyLayout m = {};
   const int64_t bound = static_cast<int64_t>(b.max_length) * b.sequences;
@@ -437,7 +444,7 @@ ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_len
   m.max_units = (static_cast<int64_t>(b.rows) * group / kManyRows + b.sequences) * c.kv_heads;
   const size_t codes = static_cast<size_t>(m.tot_pad) * c.kv_heads * c.head_dim * sizeof(__half);
   size_t at = up256(std::max(static_cast<size_t>(num_sms) * 2 * kManyRows * (c.head_dim + 2) * sizeof(float),
-                             few_workspace(c, b, group, num_sms)));
+                             few_workspace(c, b, type, group, num_sms)));
   m.k16 = at, at = up256(at + codes);
   m.v16 = at, at = up256(at + codes);
   // one tile more: a unit without keys still reads the scales of one granule
@@ -697,7 +704,7 @@ int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, cons
           "kvq8_attention: heads must be a multiple of kv_heads, at most 4096");
   KIB_ARG(static_cast<uint64_t>(b.rows) * heads < (1ull << 31), "kvq8_attention: rows times heads out of range");
   const int group = static_cast<int>(heads) / c.kv_heads;
-  *bytes = few_workspace(c, b, group, ctx->num_sms);
+  *bytes = few_workspace(c, b, type, group, ctx->num_sms);
   if (any_many(c, b, group, ctx->num_sms)) {
     const ManyLayout m = many_layout(c, b, static_cast<int64_t>(batch->total_length), type, group, ctx->num_sms);
     KIB_ARG(m.tot_pad * c.kv_heads < (1ll << 31) && m.max_units < (1ll << 27),
@@ -738,6 +745,7 @@ int kib_kvq8_attention(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8
   p.group = p.heads / p.c.kv_heads;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.partial = static_cast<float*>(workspace);
+  p.bank = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + few_records(p.c, p.b, p.group, ctx->num_sms));
   p.err = ctx->d_err;
   const cudaStream_t st = op_stream(ctx, stream);
   // a graph will replay on this workspace

@@ -35,10 +35,10 @@
 // product may be taken in any order, and q is laid out the same way); of V,
 // two byte permutes transpose 4 keys x 2 dimensions into a fragment.
 // Measured, 2 KV heads of 256 with 4 query heads each: 64 sequences of up to
-// 32768, half rows: 209-217 us, 6.2 to 6.5 TB/s; 32 of about 2048, fp32: 24.5 us;
-// one of 4096: 12.1 us.  17 sequences of up to 8190 with up to 5 fp32 rows each
-// of 16 heads of 128: 50 us, 1.6 TB/s, there by the MMAs (three groups of
-// rows, two halves of q and of p).
+// 32768, half rows: 209-217 us, 6.2 to 6.5 TB/s; 32 of about 2048, fp32: 26.5 us;
+// one of 4096: 13 us.  17 sequences of up to 8190 with up to 5 fp32 rows each
+// of 16 heads of 128: 54.5 us, 1.5 TB/s, where three groups of rows with two
+// halves of q and of p leave more instructions a key than bytes.
 #pragma once
 
 #include "gemm_tc.cuh"
@@ -58,8 +58,9 @@ constexpr int kFewMaxSeqs = 4096;
 
 // Warps of a CTA (one CTA per SM), by what the accumulators (head_dim / 16 x
 // NT x 4 registers a lane) leave.
+constexpr int kFewMaxWarps = 12;
 template <int HD, int NT>
-constexpr int few_warps() { return HD / 16 * NT * 4 >= 96 ? 8 : 12; }
+constexpr int few_warps() { return HD / 16 * NT * 4 >= 96 ? 8 : kFewMaxWarps; }
 // A warp's tile: this many blocks of 16 keys, 2 or 4 KB of K and as much of V.
 __host__ __device__ constexpr int few_blocks(int hd) { return hd == 256 ? 1 : 2; }
 // Tiles in a warp's ring, within 192 KB for all warps.
@@ -68,6 +69,19 @@ constexpr int few_ring() {
   constexpr int n = 196608 / (few_warps<HD, NT>() * 32 * HD * few_blocks(HD));
   return n < 4 ? n : 4;
 }
+// The MMA's fp32 sums are cut toward zero, up to an ulp at every step: a chain
+// of them over 32768 keys would be off by 3.9e-6 of a random result, by 33e-6 where
+// one key holds the weight and all V are alike.  So a tile of fp32 rows is
+// summed from zero, low halves first, and added to O with rounding; l takes
+// along what its additions round off (after one key of weight 1, the rest may
+// be smaller than l's last bit); and where a tile is 16 keys only, O moves into
+// sums in memory every kFewBank tiles, so that a long tail of small tiles is
+// not rounded off either.  Error then: 0.1e-6 to 0.6e-6 of the result.  Cost:
+// 32 slots of about 2048 24.5 -> 26.7 us, verify 49.4 -> 54.5 us, 64 sequences
+// to 32768 with fp32 rows 229 -> 266 us (without the moves 258).
+constexpr int kFewBank = 64;  // tiles
+template <typename T>
+__host__ __device__ constexpr bool few_banks(int hd) { return sizeof(T) == 4 && few_blocks(hd) == 1; }
 // Groups of 8 rows a unit may have.
 __host__ __device__ constexpr int few_max_nt(int hd) { return hd == 256 ? 2 : 3; }
 
@@ -80,6 +94,7 @@ struct Kvq8AttnParams {
   int64_t q_stride, out_stride;
   float scale_log2;  // softmax scale times log2(e)
   float* partial;    // [ctas][2][rows of a unit][head_dim + 2]
+  float4* bank;      // fp32 rows: [ctas][warps][head_dim / 16][groups of 8 rows][32 lanes] sums that O moves into
   int few_limit;     // sequences of at most this many rows * group are this kernel's
   int* err;
 };
@@ -94,6 +109,12 @@ KIB_DEV void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same onto zeros.
+KIB_DEV void mma_16816_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 KIB_DEV uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
@@ -172,6 +193,7 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
   constexpr int PL = sizeof(T) == 4 ? 2 : 1;      // half planes of q and p
   constexpr int QB = HD * 2 + 16;                 // bytes of a q row: conflict-free 16-byte reads
   constexpr int OF = HD + 4;                      // floats of an O row in shared memory
+  constexpr bool BANK = few_banks<T>(HD);         // O moves into sums in memory now and then
   constexpr int W = few_warps<HD, NT>(), D = few_ring<HD, NT>(), MK = few_blocks(HD), BLOCK = 16 * HD, PIECE = MK * BLOCK;
   constexpr size_t RING = static_cast<size_t>(W) * D * 2 * PIECE, JOIN = static_cast<size_t>(W) * RG * OF * 4;
   extern __shared__ __align__(1024) uint8_t few_raw[];
@@ -384,17 +406,52 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][j][e] = 0.0f;
-    float m[NT][2], l[NT][2], qs[NT][2];
+    float m[NT][2], l[NT][2], lc[NT][2], qs[NT][2];  // lc: what the last addition to l rounded off (fp32 rows)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) m[j][e] = -INFINITY, l[j][e] = 0.0f, qs[j][e] = s_qs[8 * j + 2 * c + e];
+      for (int e = 0; e < 2; ++e) m[j][e] = -INFINITY, l[j][e] = lc[j][e] = 0.0f, qs[j][e] = s_qs[8 * j + 2 * c + e];
     int vexp = 20;  // exponent field of the power of two that p is relative to
+
+    // O's sums of long runs: bank = bank * 2^(what m and vexp grew by) + O (`into`), or O += that
+    float m_bank[BANK ? NT : 1][2];  // m and vexp at the last move
+    int vexp_bank = 0;               // 0: none yet
+    auto bank = [&](bool into) {
+      if constexpr (BANK) {
+        float4* at_bank = p.bank + (static_cast<int64_t>(blockIdx.x) * W + warp) * (HD / 16 * NT * 32) + lane;
+        float f[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float vf = __uint_as_float(static_cast<uint32_t>(max(127 + vexp_bank - vexp, 0)) << 23);
+            f[j][e] = vexp_bank && m_bank[j][e] != -INFINITY ? ex2(m_bank[j][e] - m[j][e]) * vf : 0.0f;
+            m_bank[j][e] = m[j][e];
+          }
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            float (&x)[4] = o[i][j];
+            if (vexp_bank) {
+              const float4 s = at_bank[(i * NT + j) * 32];
+              x[0] = fmaf(s.x, f[j][0], x[0]), x[1] = fmaf(s.y, f[j][1], x[1]);
+              x[2] = fmaf(s.z, f[j][0], x[2]), x[3] = fmaf(s.w, f[j][1], x[3]);
+            }
+            if (into) {
+              at_bank[(i * NT + j) * 32] = make_float4(x[0], x[1], x[2], x[3]);
+              x[0] = x[1] = x[2] = x[3] = 0.0f;
+            }
+          }
+        vexp_bank = vexp;
+      }
+    };
 
     auto wait_piece = [&](int half) { ok = ok && mbar_wait_bounded(&s_bar[warp][slot][half], phase, p.err); };
 #pragma unroll 1
     for (int t = 0; t < tiles; ++t) {
       const int blk = t * MK;
+      if (BANK && t % kFewBank == 0 && t) bank(true);
       if (blk == batch + 32) {
         batch = blk;
         page_l = page_n, page_n = page_nn;
@@ -526,7 +583,7 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
             const float mn = fmaxf(m[j][e], x);
             const float f = m[j][e] == -INFINITY ? 0.0f : ex2(m[j][e] - mn);
             m[j][e] = mn;
-            l[j][e] *= f;
+            l[j][e] *= f, lc[j][e] *= f;
             const float fo = f * vf;
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) o[i][j][e] *= fo, o[i][j][e + 2] *= fo;
@@ -535,6 +592,7 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
       // 2^7 / 2^(vexp - 126)
       const float vup = __uint_as_float(static_cast<uint32_t>(min(260 - vexp, 254)) << 23);
       uint32_t pb[PL][MK][NT][2];
+      float lt[NT][2] = {};
 #pragma unroll
       for (int b = 0; b < MK; ++b) {
         const float vmul = vs[b] * vup;
@@ -545,7 +603,7 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
           for (int e = 0; e < 2; ++e) {
             const float mm = fmaxf(m[j][e], -1e30f);
             const float x = ex2(sc[b][j][e] - mm), y = ex2(sc[b][j][e + 2] - mm);
-            l[j][e] += x + y;
+            lt[j][e] += x + y;
             w[e] = x * vmul;
             w[e + 2] = y * vmul;
           }
@@ -561,41 +619,76 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
         }
       }
 
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if constexpr (PL == 2) {
+            const float y = __fsub_rn(lt[j][e], lc[j][e]), t2 = __fadd_rn(l[j][e], y);
+            lc[j][e] = __fsub_rn(__fsub_rn(t2, l[j][e]), y);
+            l[j][e] = t2;
+          } else {
+            l[j][e] += lt[j][e];
+          }
+        }
+
       // O^T += V^T P^T
       wait_piece(1);
       constexpr int WORDS = HD >= 128 ? 4 : 2, VL = HD >= 128 ? HD / 128 : 1;
+      // half rows: block by block; fp32 rows: all blocks of the tile, low halves first, onto zeros, and these sums onto O
+      constexpr int BB = PL == 2 ? MK : 1;
 #pragma unroll
-      for (int b = 0; b < MK; ++b) {
-        const uint8_t* vt = ring + (slot * 2 + 1) * PIECE + b * BLOCK;
+      for (int b0 = 0; b0 < MK; b0 += BB) {
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
-          uint32_t x[4][4];
+          uint32_t x[BB][4][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int row = 2 * c + (e & 1) + 8 * (e >> 1);
-            if constexpr (WORDS == 4) {
-              const uint4 v = *reinterpret_cast<const uint4*>(vt + 2048 * i + 128 * row + ((g ^ (row & 7)) << 4));
-              x[e][0] = v.x, x[e][1] = v.y, x[e][2] = v.z, x[e][3] = v.w;
-            } else {
-              const uint2 v = *reinterpret_cast<const uint2*>(vt + 64 * row + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
-              x[e][0] = v.x, x[e][1] = v.y;
+          for (int b = 0; b < BB; ++b) {
+            const uint8_t* vt = ring + (slot * 2 + 1) * PIECE + (b0 + b) * BLOCK;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int row = 2 * c + (e & 1) + 8 * (e >> 1);
+              if constexpr (WORDS == 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(vt + 2048 * i + 128 * row + ((g ^ (row & 7)) << 4));
+                x[b][e][0] = v.x, x[b][e][1] = v.y, x[b][e][2] = v.z, x[b][e][3] = v.w;
+              } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(vt + 64 * row + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
+                x[b][e][0] = v.x, x[b][e][1] = v.y;
+              }
             }
           }
 #pragma unroll
           for (int u = 0; u < WORDS; ++u) {
-            const uint32_t lo01 = prmt(x[0][u], x[1][u], 0x5140u) ^ 0x80808080u, hi01 = prmt(x[0][u], x[1][u], 0x7362u) ^ 0x80808080u;
-            const uint32_t lo23 = prmt(x[2][u], x[3][u], 0x5140u) ^ 0x80808080u, hi23 = prmt(x[2][u], x[3][u], 0x7362u) ^ 0x80808080u;
-            const uint32_t a0 = codes_to_half2(lo01, 0x4140u), a1 = codes_to_half2(lo01, 0x4342u);
-            const uint32_t a2 = codes_to_half2(lo23, 0x4140u), a3 = codes_to_half2(lo23, 0x4342u);
-            const uint32_t c0 = codes_to_half2(hi01, 0x4140u), c1 = codes_to_half2(hi01, 0x4342u);
-            const uint32_t c2 = codes_to_half2(hi23, 0x4140u), c3 = codes_to_half2(hi23, 0x4342u);
+            uint32_t a[BB][2][4];  // fragments of 16 dimensions each
+#pragma unroll
+            for (int b = 0; b < BB; ++b) {
+              const uint32_t lo01 = prmt(x[b][0][u], x[b][1][u], 0x5140u) ^ 0x80808080u, hi01 = prmt(x[b][0][u], x[b][1][u], 0x7362u) ^ 0x80808080u;
+              const uint32_t lo23 = prmt(x[b][2][u], x[b][3][u], 0x5140u) ^ 0x80808080u, hi23 = prmt(x[b][2][u], x[b][3][u], 0x7362u) ^ 0x80808080u;
+              a[b][0][0] = codes_to_half2(lo01, 0x4140u), a[b][0][1] = codes_to_half2(lo01, 0x4342u);
+              a[b][0][2] = codes_to_half2(lo23, 0x4140u), a[b][0][3] = codes_to_half2(lo23, 0x4342u);
+              a[b][1][0] = codes_to_half2(hi01, 0x4140u), a[b][1][1] = codes_to_half2(hi01, 0x4342u);
+              a[b][1][2] = codes_to_half2(hi23, 0x4140u), a[b][1][3] = codes_to_half2(hi23, 0x4342u);
+            }
             const int mt = (i * WORDS + u) * 2;
 #pragma unroll
-            for (int pl = 0; pl < PL; ++pl)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                mma_16816(o[mt][j], a0, a1, a2, a3, pb[pl][b][j][0], pb[pl][b][j][1]);
-                mma_16816(o[mt + 1][j], c0, c1, c2, c3, pb[pl][b][j][0], pb[pl][b][j][1]);
+              for (int h = 0; h < 2; ++h) {
+                float (&d)[4] = o[mt + h][j];
+                if constexpr (PL == 2) {
+                  float t[4];
+#pragma unroll
+                  for (int b = 0; b < BB; ++b) {
+                    if (b == 0) mma_16816_new(t, a[b][h][0], a[b][h][1], a[b][h][2], a[b][h][3], pb[1][b][j][0], pb[1][b][j][1]);
+                    else mma_16816(t, a[b][h][0], a[b][h][1], a[b][h][2], a[b][h][3], pb[1][b][j][0], pb[1][b][j][1]);
+                  }
+#pragma unroll
+                  for (int b = 0; b < BB; ++b) mma_16816(t, a[b][h][0], a[b][h][1], a[b][h][2], a[b][h][3], pb[0][b][j][0], pb[0][b][j][1]);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) d[e] += t[e];
+                } else {
+                  mma_16816(d, a[0][h][0], a[0][h][1], a[0][h][2], a[0][h][3], pb[0][b0][j][0], pb[0][b0][j][1]);
+                }
               }
           }
         }
@@ -604,6 +697,8 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
       ask_v();
       if (++slot == D) slot = 0, phase ^= 1;
     }
+
+    if (BANK && vexp_bank) bank(false);
 
     // join the warps: common maximum, then sums in warp order
 #pragma unroll
