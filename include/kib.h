@@ -328,8 +328,11 @@ int kib_kvq8_read_pages(kib_ctx* ctx, const kib_kvq8_cache* cache, const int32_t
  * are not all numbers NaN.  q and out
  * [rows][heads][head_dim] of one type: F32 rows take q and the softmax weights
  * as two halves each (22 bits), F16 rows the weights as one half; sums and
- * statistics are fp32: an F32 result is off by about 1e-6 of itself, by up to
- * 2.5e-6 where values and weights are all alike.  workspace: kib_kvq8_attention_workspace
+ * statistics are fp32: an F32 result is off by up to about 1e-6 of itself (by
+ * 2.5e-6 where all values are alike and few keys hold the weight), besides what
+ * 22 bits of a score of many nats are.  Weights are held relative to the largest
+ * value scale among the keys of a unit's run: keys whose page's scale is below
+ * 2^-11 of it (F16 rows: 2^-21) lose bits.  workspace: kib_kvq8_attention_workspace
  * bytes, 256-byte aligned; calls that may overlap need one each. */
 int kib_kvq8_attention_workspace(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_batch* batch, int type,
                                  uint64_t heads, uint64_t* bytes);

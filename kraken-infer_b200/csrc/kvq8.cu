@@ -433,7 +433,7 @@ bool any_many(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_sms) {
 
 // The workspace of the many-row path, in this order behind the records.
 struct ManyLayout {
-  size_t k16, v16, scales, seq_off, units, cum, cta_unit, split, count, sums, bytes;
+  size_t k16, v16, scales, seq_off, units, cum, cta_unit, split, count, bytes;
   int64_t tot_pad, max_units;
 };
 ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_length, int type, int group, int num_sms) {
@@ -455,8 +455,6 @@ ManyLayout many_layout(const Kvq8Cache& c, const Kvq8Batch& b, int64_t total_len
   m.cta_unit = at, at = up256(at + static_cast<size_t>(num_sms) * sizeof(int));
   m.split = at, at = up256(at + static_cast<size_t>(num_sms) * sizeof(int4));
   m.count = at, at = up256(at + 2 * sizeof(int));
-  m.sums = at;  // of fp32 rows
-  if (type == KIB_TYPE_F32) at = up256(at + static_cast<size_t>(num_sms) * kManyRows * c.head_dim * sizeof(float));
   m.bytes = at;
   return m;
 }
@@ -469,6 +467,15 @@ cudaError_t many_launch(const Kvq8AttnParams& a, const ManyLayout& w, uint8_t* w
   static PerDevice ready;
   cudaError_t e = allow_smem(ctx->device, kvq8_many_kernel<HD, PL>, Sh::kSmem, &ready);
   if (e != cudaSuccess) return e;
+  if constexpr (Sh::kHeld) {
+    // (a build whose launch has fewer registers would wait for the rest without end)
+    static const bool enough = [] {
+      cudaFuncAttributes a{};
+      return cudaFuncGetAttributes(&a, kvq8_many_kernel<HD, PL>) == cudaSuccess &&
+             a.numRegs * Sh::kThreads >= 128 * kManyHelperRegs + kManySoft * kManySoftRegs;
+    }();
+    if (!enough) return cudaErrorInvalidConfiguration;
+  }
   Kvq8ManyParams p;
   p.a = a;
   p.a.partial = reinterpret_cast<float*>(ws);
@@ -483,7 +490,6 @@ cudaError_t many_launch(const Kvq8AttnParams& a, const ManyLayout& w, uint8_t* w
   p.cta_unit = reinterpret_cast<int*>(ws + w.cta_unit);
   p.split = reinterpret_cast<int4*>(ws + w.split);
   p.count = reinterpret_cast<int*>(ws + w.count);
-  p.sums = reinterpret_cast<float4*>(ws + w.sums);
   p.ctas = num_sms;
   p.err = ctx->d_err;
   const int kvh = a.c.kv_heads;
@@ -493,7 +499,7 @@ cudaError_t many_launch(const Kvq8AttnParams& a, const ManyLayout& w, uint8_t* w
     return cudaErrorInvalidValue;
   const dim3 tiles(static_cast<unsigned>(w.tot_pad / kManyKeys + 1), static_cast<unsigned>(kvh));
   kvq8_gather_kernel<HD><<<tiles, kGatherThreads, 0, st>>>(p);
-  kvq8_many_kernel<HD, PL><<<num_sms, kManyThreads, Sh::kSmem, st>>>(kmap, vmap, p);
+  kvq8_many_kernel<HD, PL><<<num_sms, Sh::kThreads, Sh::kSmem, st>>>(kmap, vmap, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_pdl(kvq8_many_merge<HD, PL>, dim3(static_cast<unsigned>(num_sms), kManyRows / 8), dim3(256), 0, st, p);

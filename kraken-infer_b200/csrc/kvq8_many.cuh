@@ -18,19 +18,33 @@
 //               (M = 128, N = 128), then O += P(j-1) V (N = head_dim) with P
 //               read from TMEM: the softmax of one tile runs under the
 //               products of its neighbours;
-//   warps 0-7   softmax: a thread holds 64 of a row's 128 scores, p =
+//   warps 0-7   softmax: a thread has 64 of a row's 128 scores, p =
 //               2^(s - m), and writes p * v_scale back over S as halves.  m
 //               moves only when a row's maximum grows by more than 2^8, so O
-//               is rarely rescaled in TMEM.
+//               is rarely rescaled.
 // Numerics as in the few-row kernel: codes are exact in half; half rows use q
 // as given and p as one half (2^7 above the largest v_scale of the run: room
 // for the 2^8); fp32 rows use q and p as high + low halves, twice the MMAs.
 // TMEM: O in columns 0 .. head_dim - 1, S in 256.. and 384..
 //
+// The tensor core's fp32 sums are cut toward zero: a step (16 keys) loses up
+// to 2^-22 of the sum where V are all alike, some 2e-8 where their signs are
+// random.  For half rows O is summed in TMEM all the same, under half's 2^-11
+// up to runs of 2000 steps.  Of fp32 rows a tile's products are summed from
+// zero, low halves first, and the softmax threads add them to O in their
+// registers with rounding (l takes along what its additions round off): two
+// warpgroups hold half a row of O each, 128 registers a thread at 256
+// dimensions, which the helpers' warpgroup gives up (setmaxnreg).  Error against 64
+// bits after 6144 keys: 0.35e-6 of a random result, 1.9e-6 at most where one key holds
+// the weight and V are alike.  (Summed in TMEM and moved into sums in memory
+// every 8 tiles: 1.4e-6 with a correction for random data, 13e-6 for the other;
+// prompts of up to 3001 tokens 307 us where this takes 268.  Halves by this
+// form: 258 us instead of 228 for the chunk below.)
+//
 // Bound by the tensor pipe where runs are long (1024 half rows of 8 heads of
-// 256 after 32768 keys: 230-258 us by the machine, up to 1170 TFLOP/s, pipe 70 %
-// active), by what a unit costs besides its tiles where they are short (prompts
-// of up to 3001 tokens: halves 178 us, fp32 306 us).  Two turns of softmax
+// 256 after 32768 keys: 228-252 us by the machine, up to 1190 TFLOP/s; fp32 391 us),
+// by what a unit costs besides its tiles where they are short (prompts
+// of up to 3001 tokens: halves 179 us, fp32 268 us).  Two turns of softmax
 // warps on alternate tiles instead of two halves of each took 280 us for the
 // former, asking for the next stage before a tile's products 252.
 //
@@ -47,7 +61,6 @@ namespace kib {
 constexpr int kManyRows = 128;   // query rows of a unit
 constexpr int kManyKeys = 128;   // keys of a granule
 constexpr int kManySoft = 256;   // softmax threads
-constexpr int kManyThreads = kManySoft + 64;
 
 // A unit costs about as much as this many granules besides its own (q in, the
 // pipeline filled and drained, O out), so runs are cut by granules plus this:
@@ -57,19 +70,6 @@ constexpr int kManyThreads = kManySoft + 64;
 // cost of 1, 261 / 412 with 2, 208 / 325 with 4, 178 / 273 with 6, 197 / 320
 // with 16 (head_dim 128: 6 is best too).
 constexpr int kManyUnitCost = 6;
-
-// The tensor core's fp32 sums are cut toward zero: O loses a little at each
-// step (16 keys, and again for p's low halves).  What was measured against 64
-// bits, of O and a step: 4e-8 where all V are alike, 2e-8 for random V and
-// scores (deviation 1.4), 0.9e-8 for random V and equal weights, where O is a
-// small rest of what was added.  So for fp32 rows O moves into rounded sums in
-// memory every kManyFlush tiles, and what a run loses until then is taken off
-// l by the middle of those figures.  Error after 6144 random keys, of the
-// result, and time of prompts of up to 3001 tokens: about 13e-6 and 271 us with
-// neither, 5.5e-6 and 271 us without the moves, 2.0e-6 and 301 us with moves
-// every 12 tiles, 1.4e-6 and 306 us every 8 (all V alike: 2.4e-6).
-constexpr int kManyFlush = 8;
-constexpr float kManyStepLoss = 2.0e-8f;
 
 struct Kvq8ManyParams {
   Kvq8AttnParams a;
@@ -82,7 +82,6 @@ struct Kvq8ManyParams {
   int4* units;      // [max_units] sequence, row tile, head, granules
   int64_t* cum;     // [max_units + 1] running cost; cum[count[0]] is the total
   int* cta_unit;    // [ctas] unit at which a CTA begins
-  float4* sums;     // fp32 rows: [ctas][head_dim / 4][128 rows] what O moves into
   int4* split;      // [ctas] units that cross CTAs: unit, first CTA, CTAs, whether its first record is a CTA's second
   int* count;       // [2] units, split units
   int ctas;
@@ -386,6 +385,12 @@ struct ManyShared {
 // TMEM instructions need the whole warp: one lane's failed wait is everyone's.
 KIB_DEV bool warp_ok(bool ok) { return __all_sync(0xffffffffu, ok) != 0; }
 
+// Of the 384 threads that fp32 rows are launched with, registers move from the
+// warpgroup of the helpers to the two that hold O: 168 each at launch, so the
+// shares may come to 384 * 168 together.
+constexpr int kManyHelperRegs = 64, kManySoftRegs = 216;
+static_assert(128 * kManyHelperRegs + 256 * kManySoftRegs <= 384 * 168, "more registers than the launch has");
+
 template <int HD, int PL>
 struct ManyShape {
   static constexpr int kTile = 128 * HD * 2;                      // bytes of a K or a V tile
@@ -393,36 +398,14 @@ struct ManyShape {
   static constexpr int kPer = kTile / kStage;                     // stages of a tile
   static constexpr int kQ = PL * kManyRows * HD * 2;
   static constexpr int kStages = HD == 256 ? (PL == 2 ? 3 : 5) : (HD == 128 ? (PL == 2 ? 5 : 6) : 8);
+  static constexpr bool kHeld = PL == 2;                          // O in the softmax threads' registers
+  static constexpr int kThreads = kManySoft + (kHeld ? 128 : 64);
   static constexpr int kPartial = kManyRows * (HD + 2);           // floats of a record
   static constexpr size_t kSmem = static_cast<size_t>(kQ) + kStages * kStage + sizeof(ManyShared);
 };
 
-// The sums that O moves into: 32 of a row's columns, each thread's own, 16
-// bytes of a warp's rows side by side.
-KIB_DEV float4* many_sums(float4* sums, int c0, int hd, int row) {
-  return sums + (static_cast<int64_t>(blockIdx.x) * (hd / 4) + c0 / 4) * kManyRows + row;
-}
-KIB_DEV void many_add(float4* sums, int c0, int hd, int row, float f, uint32_t (&o)[32]) {
-  const float4* s = many_sums(sums, c0, hd, row);
-#pragma unroll
-  for (int i = 0; i < 32; i += 4) {
-    const float4 v = s[i / 4 * kManyRows];
-    o[i] = __float_as_uint(fmaf(v.x, f, __uint_as_float(o[i])));
-    o[i + 1] = __float_as_uint(fmaf(v.y, f, __uint_as_float(o[i + 1])));
-    o[i + 2] = __float_as_uint(fmaf(v.z, f, __uint_as_float(o[i + 2])));
-    o[i + 3] = __float_as_uint(fmaf(v.w, f, __uint_as_float(o[i + 3])));
-  }
-}
-KIB_DEV void many_move(float4* sums, int c0, int hd, int row, bool more, float f, uint32_t (&o)[32]) {
-  if (more) many_add(sums, c0, hd, row, f, o);
-  float4* s = many_sums(sums, c0, hd, row);
-#pragma unroll
-  for (int i = 0; i < 32; i += 4)
-    s[i / 4 * kManyRows] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-}
-
 template <int HD, int PL>
-__global__ void __launch_bounds__(kManyThreads, 1)
+__global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
     kvq8_many_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                      const __grid_constant__ Kvq8ManyParams p) {
   using T = typename std::conditional<PL == 2, float, __half>::type;
@@ -482,8 +465,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     return r;
   };
 
-  if (warp == 8) {
-    {
+  if (warp >= 8) {
+    if constexpr (Sh::kHeld) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyHelperRegs));
+    if (warp == 8) {
       if (elect_one()) tma_prefetch_desc(&kmap), tma_prefetch_desc(&vmap);
       uint32_t it = 0;
       bool ok = true;
@@ -521,9 +505,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         if (ok) load(&vmap, false, r.head, off + (r.g1 - 1) * kManyKeys);
       }
-    }
-  } else if (warp == 9) {
-    {
+    } else if (warp == 9) {
       constexpr uint32_t idesc_s = umma_idesc_f16(kManyKeys), idesc_o = umma_idesc_f16(HD);
       uint32_t it = 0, jg = 0, piece = 0;
       bool ok = true;
@@ -563,26 +545,33 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         ok = warp_ok(ok && tc_wait(&p_full[jj & 1], (jj >> 1) & 1, p.err));
         tc_fence_after();
         const uint32_t a = tmem + 256 + 128 * (jj & 1);
+        // fp32 rows: every tile from zero, p's low halves first as q's above
 #pragma unroll 1
-        for (int i = 0; i < Sh::kPer && ok; ++i, ++it) {
-          const int s = static_cast<int>(it % Sh::kStages);
-          ok = warp_ok(tc_wait(&full[s], (it / Sh::kStages) & 1, p.err));
-          if (!ok) break;
-          tc_fence_after();
-          constexpr int STEPS = kManyKeys / 16 / Sh::kPer;
-          const uint64_t b0 = st_desc + static_cast<uint64_t>(s * (Sh::kStage / 16));
-          if (elect_one()) {
+        for (int pl = PL - 1; pl >= 0 && ok; --pl) {
+#pragma unroll 1
+          for (int i = 0; i < Sh::kPer && ok; ++i) {
+            const int s = static_cast<int>((it + i) % Sh::kStages);
+            if (pl == PL - 1) {
+              ok = warp_ok(tc_wait(&full[s], ((it + i) / Sh::kStages) & 1, p.err));
+              if (!ok) break;
+              tc_fence_after();
+            }
+            constexpr int STEPS = kManyKeys / 16 / Sh::kPer;
+            const uint64_t b0 = st_desc + static_cast<uint64_t>(s * (Sh::kStage / 16));
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-              for (int pl = 0; pl < PL; ++pl)
-                umma_f16_ts(tmem, a + 64 * pl + 8 * (i * STEPS + k), b0 + (k / 4) * (HD * 8) + 2 * (k % 4), idesc_o,
-                            (k | pl) != 0 ? 1u : (begin && i == 0 ? 0u : 1u));
-            umma_commit(&empty[s]);
-            if (i + 1 == Sh::kPer) umma_commit(&o_done[jj & 1]);
+              for (int k = 0; k < STEPS; ++k) {
+                const int ks = i * STEPS + k;  // 16 keys
+                umma_f16_ts(tmem, Sh::kHeld ? a + 32 * (ks / 2) + 8 * (ks % 2) + 16 * pl : a + 8 * ks, b0 + (k / 4) * (HD * 8) + 2 * (k % 4),
+                            idesc_o, k != 0 || i != 0 || pl != PL - 1 ? 1u : (Sh::kHeld || begin ? 0u : 1u));
+              }
+              if (pl == 0) umma_commit(&empty[s]);
+              if (pl == 0 && i + 1 == Sh::kPer) umma_commit(&o_done[jj & 1]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
+        it += Sh::kPer;
       };
       int unit = unit0;
       for (int64_t at = first; at < stop && ok; ++unit) {
@@ -600,7 +589,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         jg += n;
       }
     }
-  } else if (warp < 8) {
+  } else {
+    if constexpr (Sh::kHeld) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManySoftRegs));
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;  // columns 64 half .. of TMEM lane `row`
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     uint32_t jg = 0;
@@ -696,11 +686,33 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int end = row_end(row);
       const int all_see = row_end(0);  // keys below it are seen by every row (of the dead ones nothing is kept)
 
-      float m = -INFINITY, l = 0.0f, m_sums = -INFINITY;  // m_sums: m at the last move of O
+      float m = -INFINITY, l = 0.0f;
       const int n = r.g1 - r.g0;
       float2 sc[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) sc[g] = __ldg(scales + r.g0 * 8 + half * 4 + g);
+      // O of the product before last or last: complete when S of the tile after it is, or with this wait
+      auto wait_o = [&](uint32_t jj) {
+        ok = warp_ok(ok && tc_wait(&o_done[jj & 1], (jj >> 1) & 1, p.err));
+        tc_fence_after();
+      };
+      [[maybe_unused]] float held[Sh::kHeld ? HD / 2 : 1], lc = 0.0f;  // O; what the last addition to l rounded off
+      if constexpr (Sh::kHeld) {
+#pragma unroll
+        for (int i = 0; i < HD / 2; ++i) held[i] = 0.0f;
+      }
+      // O += f * the sum of one tile
+      auto add_tile = [&](float f) {
+        if constexpr (Sh::kHeld) {
+#pragma unroll
+          for (int c0 = 0; c0 < HD / 2; c0 += 32) {
+            uint32_t o[32];
+            tmem_ld(tmem + lanes + half * (HD / 2) + c0, o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) held[c0 + i] = fmaf(__uint_as_float(o[i]), f, held[c0 + i]);
+          }
+        }
+      };
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {
         const uint32_t jj = jg + j, buf = jj & 1;
@@ -713,46 +725,57 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           vc[g] = sc[g].y * vup;
           absent = absent || sc[g].y < 0.0f;
         }
-        float2 nx[4];
-        if (j + 1 < n) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) nx[g] = __ldg(scales + (r.g0 + j + 1) * 8 + half * 4 + g);
-        }
-        ok = warp_ok(ok && tc_wait(&s_full[buf], (jj >> 1) & 1, p.err));
-        tc_fence_after();
-        uint32_t s[64];
-        if (ok) tmem_ld(tmem + lanes + 256 + 128 * buf + 64 * half, s);
         // what is masked goes to -infinity; kc is not negative, so a group's largest score is that of its largest s
-        if (key + 64 > all_see || absent) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (key + i >= end || sc[i >> 4].y < 0.0f) s[i] = 0xff800000u;
+        const bool edge = key + 64 > all_see || absent;
+        if (edge) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) kc[g] = fmaxf(kc[g], 1e-38f);  // 0 times -infinity would be NaN
         }
+        ok = warp_ok(ok && tc_wait(&s_full[buf], (jj >> 1) & 1, p.err));
+        tc_fence_after();
+        const uint32_t src = tmem + lanes + 256 + 128 * buf + 64 * half;
+        // scores are held 64 at a time, or (next to O) read 32 at a time, for their maximum and again for their weights
+        constexpr int CH = Sh::kHeld ? 32 : 64;
+        uint32_t s[CH];
+        auto load = [&](int c0) {
+          if (ok) tmem_ld(src + c0, s);
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+              if (key + c0 + i >= end || sc[(c0 + i) >> 4].y < 0.0f) s[i] = 0xff800000u;
+          }
+        };
         float top = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float a = __uint_as_float(s[16 * g]), b = __uint_as_float(s[16 * g + 1]);
+        for (int c0 = 0; c0 < 64; c0 += CH) {
+          load(c0);
 #pragma unroll
-          for (int i = 2; i < 16; i += 4) {
-            a = fmaxf(fmaxf(a, __uint_as_float(s[16 * g + i])), i + 2 < 16 ? __uint_as_float(s[16 * g + i + 2]) : a);
-            b = fmaxf(fmaxf(b, __uint_as_float(s[16 * g + i + 1])), i + 3 < 16 ? __uint_as_float(s[16 * g + i + 3]) : b);
+          for (int g = 0; g < CH / 16; ++g) {
+            float a = __uint_as_float(s[16 * g]), b = __uint_as_float(s[16 * g + 1]);
+#pragma unroll
+            for (int i = 2; i < 16; i += 4) {
+              a = fmaxf(fmaxf(a, __uint_as_float(s[16 * g + i])), i + 2 < 16 ? __uint_as_float(s[16 * g + i + 2]) : a);
+              b = fmaxf(fmaxf(b, __uint_as_float(s[16 * g + i + 1])), i + 3 < 16 ? __uint_as_float(s[16 * g + i + 3]) : b);
+            }
+            top = fmaxf(top, fmaxf(a, b) * kc[c0 / 16 + g]);
           }
-          top = fmaxf(top, fmaxf(a, b) * kc[g]);
         }
         sh.x[buf][half][row] = top;
         // m follows only a growth of more than 2^8: p stays below 2^8, its half below 2^15
-        const bool move = PL == 2 && j > 0 && j % kManyFlush == 0;
-        if (soft_any(top > m + 8.0f) || move) {
+        [[maybe_unused]] float last_f = 1.0f;  // for the tile that is not in O yet
+        if (soft_any(top > m + 8.0f)) {
           const float mn = fmaxf(m, fmaxf(top, sh.x[buf][half ^ 1][row]));
           const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
           m = mn;
           l *= f;
-          if (j > 0) {
+          if constexpr (Sh::kHeld) {
+            lc *= f;
+            last_f = f;
+#pragma unroll
+            for (int i = 0; i < HD / 2; ++i) held[i] *= f;
+          } else if (j > 0) {
             // S(j) was issued after the product before last, so only the last one may still run
-            ok = warp_ok(ok && tc_wait(&o_done[(jj - 1) & 1], ((jj - 1) >> 1) & 1, p.err));
-            tc_fence_after();
+            wait_o(jj - 1);
             if (ok) {
 #pragma unroll 1
               for (int c0 = 0; c0 < HD / 2; c0 += 32) {
@@ -761,30 +784,25 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 tmem_ld(addr, o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                if (PL == 2 && move) {
-                  many_move(p.sums, half * (HD / 2) + c0, HD, row, j > kManyFlush, m_sums == -INFINITY ? 0.0f : ex2(m_sums - mn), o);
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) o[i] = 0u;
-                }
                 tmem_st32(addr, o);
               }
               tmem_st_wait();
             }
-            if (move) m_sums = mn;
           }
         }
         const float mm = fmaxf(m, -1e30f);
         // two scores an instruction: s * kc - m, and p * v_scale
         float2 lp[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         const float2 nm = make_float2(-mm, -mm);
-        const uint32_t pdst = tmem + lanes + 256 + 128 * buf + 32 * half;
 #pragma unroll
         for (int c0 = 0; c0 < 64; c0 += 32) {
+          if constexpr (Sh::kHeld) load(c0);
+          constexpr int B = CH == 64 ? 1 : 0;
           uint32_t ph[16], pl[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const int g = (c0 + i) >> 4;
-            float2 e = __ffma2_rn(make_float2(__uint_as_float(s[c0 + i]), __uint_as_float(s[c0 + i + 1])), make_float2(kc[g], kc[g]), nm);
+            const int g = (c0 + i) >> 4, at_s = B * c0 + i;
+            float2 e = __ffma2_rn(make_float2(__uint_as_float(s[at_s]), __uint_as_float(s[at_s + 1])), make_float2(kc[g], kc[g]), nm);
             e = make_float2(ex2(e.x), ex2(e.y));
             lp[(i >> 1) & 1] = __fadd2_rn(lp[(i >> 1) & 1], e);
             const float2 w = __fmul2_rn(e, make_float2(vc[g], vc[g]));
@@ -794,51 +812,83 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               pl[i >> 1] = pack_half2(w.x - f2.x, w.y - f2.y);
             }
           }
+          // halves: 64 columns of the tile's 128 keys; fp32 rows: 32 keys' high and low halves where their scores were
           if (ok) {
-            tmem_st16(pdst + c0 / 2, ph);
-            if constexpr (PL == 2) tmem_st16(pdst + 64 + c0 / 2, pl);
+            tmem_st16(Sh::kHeld ? src + c0 : tmem + lanes + 256 + 128 * buf + 32 * half + c0 / 2, ph);
+            if constexpr (PL == 2) tmem_st16(src + c0 + 16, pl);
           }
         }
-        l += (lp[0].x + lp[0].y) + (lp[1].x + lp[1].y);
+        const float lt = (lp[0].x + lp[0].y) + (lp[1].x + lp[1].y);
+        if constexpr (Sh::kHeld) {
+          const float y = __fsub_rn(lt, lc), t = __fadd_rn(l, y);
+          lc = __fsub_rn(__fsub_rn(t, l), y);
+          l = t;
+        } else {
+          l += lt;
+        }
+        if (j + 1 < n) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) sc[g] = __ldg(scales + (r.g0 + j + 1) * 8 + half * 4 + g);
+        }
         if (ok) tmem_st_wait();
+        if constexpr (Sh::kHeld) {
+          // the products of the tile before, while those of this one wait for it
+          if (j > 0) {
+            wait_o(jj - 1);
+            if (ok) add_tile(last_f);
+          }
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[buf]);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) sc[g] = nx[g];
       }
       jg += n;
 
       // the unit's or the run's end: O / l, or a record
-      ok = warp_ok(ok && tc_wait(&o_done[(jg - 1) & 1], ((jg - 1) >> 1) & 1, p.err));
-      tc_fence_after();
+      wait_o(jg - 1);
+      if constexpr (Sh::kHeld) {
+        if (ok) add_tile(1.0f);
+      }
       float* s_l = reinterpret_cast<float*>(s_q);  // q has been read by every product of the run
       s_l[half * kManyRows + row] = l;
       soft_any(false);
       l += s_l[(half ^ 1) * kManyRows + row];
-      if constexpr (PL == 2) {
-        const int seen = min(max(end - r.g0 * kManyKeys, 0), n * kManyKeys);
-        l = fmaf(l, -kManyStepLoss * static_cast<float>(min(seen, kManyFlush * kManyKeys) / 8), l);
-      }
       const float back = __uint_as_float(static_cast<uint32_t>(max(ve - 6, 1)) << 23);  // 2^(ve - 126) / 2^7
       const float inv = r.whole ? (l > 0.0f ? back / l : (l == 0.0f ? 0.0f : l)) : back;
       float* rec = p.a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (r.begin == first ? 0 : 1)) * Sh::kPartial;
       const int rr = row0 + row;
       T* out = static_cast<T*>(p.a.out) + static_cast<int64_t>(sq.first + rr / p.a.group) * p.a.out_stride +
                (static_cast<int64_t>(r.head) * p.a.group + rr % p.a.group) * HD;
-#pragma unroll 1
-      for (int c0 = half * (HD / 2); c0 < (half + 1) * (HD / 2); c0 += 32) {
-        uint32_t o[32];
-        if (ok) tmem_ld(tmem + lanes + c0, o);
-        if (PL == 2 && ok && n > kManyFlush) many_add(p.sums, c0, HD, row, m_sums == -INFINITY ? 0.0f : ex2(m_sums - m), o);
+      auto put = [&](int c0, const float (&x)[8]) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x[e] * inv;
+        if (r.whole) store_vec<T, 8>(out + c0, y);
+        else store_vec<float, 8>(rec + row * HD + c0, y);
+      };
+      if constexpr (Sh::kHeld) {
         if (row < live) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            float y[8];
+          for (int i = 0; i < HD / 2; i += 8) {
+            float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[i + e]) * inv;
-            if (r.whole) store_vec<T, 8>(out + c0 + i, y);
-            else store_vec<float, 8>(rec + row * HD + c0 + i, y);
+            for (int e = 0; e < 8; ++e) x[e] = held[i + e];
+            put(half * (HD / 2) + i, x);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c0 = half * (HD / 2); c0 < (half + 1) * (HD / 2); c0 += 32) {
+          uint32_t o[32];
+          if (ok) tmem_ld(tmem + lanes + c0, o);
+          if (row < live) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(o[i + e]);
+              put(c0 + i, x);
+            }
           }
         }
       }

@@ -823,3 +823,18 @@ def test_attention_of_few_rows_keeps_fp32_accuracy_on_long_runs(ctx, hd, rows, k
     deviate by sqrt(80) 2^-24 / sqrt(3) (3e-7), the normaliser's by 1e-7, the
     weights' 22 bits and the joins by less: together below 1e-6 of the result."""
     assert row_errors(ctx, [32768] * 64, [rows] * 64, hd, kind, alike) <= 1e-6
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n,rows", [(6144, 6144), (32768, 1024)])
+@pytest.mark.parametrize("kind", ["equal", "peak", "tail"])
+@pytest.mark.parametrize("alike", [False, True])
+def test_attention_of_many_rows_keeps_fp32_accuracy_on_long_runs(ctx, hd, n, rows, kind, alike):
+    """A prompt, and a chunk after a long context.  The tensor cores cut 16
+    products a step at a quarter of the sum's last bit, 2^-22 of it together:
+    eight steps of a tile lose 1.9e-6 at most where V are all alike, and random
+    signs cancel to a tenth of it.  Up to 110 rounded additions of tiles deviate
+    by sqrt(110) 2^-24 / sqrt(3) (4e-7), the weights' 22 bits and the joins by
+    less."""
+    assert row_errors(ctx, [n], [rows], hd, kind, alike) <= (2.5e-6 if alike else 1e-6)
