@@ -416,19 +416,33 @@ size_t few_workspace(const Kvq8Cache& c, const Kvq8Batch& b, int type, int group
 
 // Rows (times the group) up to which a sequence is the few-row kernel's.
 constexpr int kFewLimit = 64;
-// The most granules of 128 keys (for 16 query rows of a KV head) per SM that
-// the few-row kernel takes in their stead, whatever the rows: the many-row path
-// begins with three kernels' latencies.  Few against many rows' kernels, one
-// sequence, head_dim 256, 8 query heads, 2 KV heads, fp32: 32 tokens 9.9 and
-// 30.1 us, 200 tokens (1.4 granules) 23 and 34, 64 after 1000 (1.7) 21 and 38,
-// 40 after 4000 (4.3) 28 and 53; 300 after 300 (5.1) 42 and 38, 500 (6.8) 55
-// and 38; four sequences of 100 (1.4) 33 and 35.  Halves and other head sizes
-// cross over at the same place.
-constexpr int kFewGranules = 5;
+// Batches with a sequence of more rows than that go to the many-row path where
+// it is the faster one, reckoned in granules of 128 keys and 16 query rows per
+// SM.  The few-row kernel takes the granules and about six for the start and
+// end of each unit.  The many-row path takes eight for its three launches (ten
+// and twelve of the shorter ones of 128 and 64 dimensions), two for 128 rows of a
+// granule, and 0.2 (0.3, 0.4) for every CTA that a unit is spread over, whose
+// records are joined one after another.  8 query and 2 KV heads, few against
+// many, us (rows of each sequence, after its other tokens):
+//                              fp32 256    fp32 64     half 256    half 64
+//     1 x 100                  17   30     13   18     15   25     11   16
+//     1 x 32 after 16000       54   78     28   45     42   68     22   44
+//     1 x 64 after 8000        55   55     30   33     43   48     23   31
+//     4 x 100                  35   34     18   21     32   28     16   19
+//     4 x 64 after 1000        49   42     26   27     41   37     21   25
+//     1 x 200 after 1300       51   42     28   24     41   35     21   23
+//     1 x 500                  59   38     32   23     51   33     26   21
+//     30 x 20 after 480        72   49     39   30     62   42     31   27
+// Over 22 such batches, three head sizes and both types the rule takes 1 % more
+// time than the faster kernel would (16 % at most: 150 rows after 2850, fp32 128).
 bool any_many(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_sms) {
-  if (static_cast<int64_t>(b.max_rows) * group <= kFewLimit) return false;
-  const int64_t units = (static_cast<int64_t>(b.rows) * group / 16 + b.sequences) * c.kv_heads;
-  return units * ((static_cast<int64_t>(b.max_length) + kFewGranule - 1) / kFewGranule) > static_cast<int64_t>(kFewGranules) * num_sms;
+  if (static_cast<int64_t>(b.max_rows) * group <= kFewLimit || b.max_length == 0) return false;
+  const int64_t rows = static_cast<int64_t>(b.rows) * group, granules = (static_cast<int64_t>(b.max_length) + kFewGranule - 1) / kFewGranule;
+  const double few_units = static_cast<double>(rows / 16 + b.sequences) * c.kv_heads / num_sms;
+  const double units = static_cast<double>(rows / kManyRows + b.sequences) * c.kv_heads / num_sms;
+  const double spread = units < 1.0 ? std::min(1.0 / units, static_cast<double>(granules)) : 1.0;
+  const double start = c.head_dim == 256 ? 8.0 : (c.head_dim == 128 ? 10.0 : 12.0), join = c.head_dim == 256 ? 0.2 : (c.head_dim == 128 ? 0.3 : 0.4);
+  return few_units * static_cast<double>(granules + 6) > start + join * spread + 2.0 * units * static_cast<double>(granules);
 }
 
 // The workspace of the many-row path, in this order behind the records.

@@ -838,3 +838,41 @@ def test_attention_of_many_rows_keeps_fp32_accuracy_on_long_runs(ctx, hd, n, row
     by sqrt(110) 2^-24 / sqrt(3) (4e-7), the weights' 22 bits and the joins by
     less."""
     assert row_errors(ctx, [n], [rows], hd, kind, alike) <= (2.5e-6 if alike else 1e-6)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_batches_go_to_the_kernel_that_is_faster_for_them(ctx, hd, dtype):
+    """Told by the workspace, which holds unpacked keys for the many-row path
+    only: batches whose times by the two kernels differ by over a fifth."""
+    i32 = lambda *n: torch.zeros(*n, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def unpacks(n, rows, length):
+        pages = -(-length // 32)
+        cache = kib.KvQ8Cache(*(torch.empty(1, 2, 32, hd, dtype=torch.int8, device="cuda") for _ in range(2)),
+                              *(torch.empty(1, 2, device="cuda") for _ in range(2)))
+        batch = kib.KvQ8Batch(i32(n, pages), i32(n), i32(n + 1), n * rows, rows, length, n * length)
+        q = torch.empty(1, 8, hd, dtype=DT[dtype], device="cuda").expand(1, 8, hd)
+        one = kib.KvQ8Batch(i32(n, pages), i32(n), i32(n + 1), n * 16, 16, length, n * length)  # 64 rows a KV head: never
+        return ctx.kvq8_attention_workspace(cache, batch, q) > ctx.kvq8_attention_workspace(cache, one, q)
+
+    for few in ((1, 32, 32), (1, 32, 16000), (1, 24, 32000), (1, 100, 100), (1, 40, 4000), (1, 64, 1000)):
+        assert not unpacks(*few), few
+    for many in ((1, 500, 500), (30, 20, 500), (8, 200, 200), (3, 500, 500), (1, 1024, 32768), (5, 3001, 3001)):
+        assert unpacks(*many), many
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 256])
+def test_attention_of_many_rows_with_scales_far_apart_and_absent_pages(ctx, dtype, hd):
+    c = Case([1500, 700], [1300, 500], 2, 1, hd, 64, seed=47, dtype=dtype)
+    r = np.random.default_rng(4)
+    c.dev[3].copy_(torch.from_numpy((10.0 ** r.uniform(-6, -1, c.scales[1].shape)).astype(np.float32)))
+    c.dev[3][c.table[0, 3]] = 0.0
+    c.dev[2][c.table[0, 1]] = 0.0
+    c.table[0, 5], c.table[1, 0], c.table[1, 1] = -1, c.pages, 1 << 30
+    c.batch.tensors[0].copy_(torch.from_numpy(c.table))
+    for scale in (None, 2.0, -0.1, 0.0):
+        check_attend(ctx, c, scale)
