@@ -408,9 +408,10 @@ size_t few_records(const Kvq8Cache& c, const Kvq8Batch& b, int group, int num_sm
                static_cast<size_t>(c.head_dim + 2) * sizeof(float));
 }
 size_t few_workspace(const Kvq8Cache& c, const Kvq8Batch& b, int type, int group, int num_sms) {
+  const int nt = few_nt(c, b, group);
   size_t bytes = few_records(c, b, group, num_sms);
   if (type == KIB_TYPE_F32 && few_banks<float>(c.head_dim))
-    bytes += static_cast<size_t>(std::min(num_sms, kMergeMaxCtas)) * kFewMaxWarps * 8 * few_nt(c, b, group) * c.head_dim * sizeof(float);
+    bytes += static_cast<size_t>(std::min(num_sms, kMergeMaxCtas)) * few_warps_of(c.head_dim, nt) * 8 * nt * c.head_dim * sizeof(float);
   return bytes;
 }
 

@@ -58,9 +58,9 @@ constexpr int kFewMaxSeqs = 4096;
 
 // Warps of a CTA (one CTA per SM), by what the accumulators (head_dim / 16 x
 // NT x 4 registers a lane) leave.
-constexpr int kFewMaxWarps = 12;
+__host__ __device__ constexpr int few_warps_of(int hd, int nt) { return hd / 16 * nt * 4 >= 96 ? 8 : 12; }
 template <int HD, int NT>
-constexpr int few_warps() { return HD / 16 * NT * 4 >= 96 ? 8 : kFewMaxWarps; }
+constexpr int few_warps() { return few_warps_of(HD, NT); }
 // A warp's tile: this many blocks of 16 keys, 2 or 4 KB of K and as much of V.
 __host__ __device__ constexpr int few_blocks(int hd) { return hd == 256 ? 1 : 2; }
 // Tiles in a warp's ring, within 192 KB for all warps.
