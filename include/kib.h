@@ -268,8 +268,11 @@ int kib_attention_f32_f16_kv(kib_ctx* ctx, const float* query, const uint16_t* k
  *
  * stream: a cudaStream_t on which the op is only enqueued (the caller orders
  * it; (void*)1 is CUDA's legacy default stream), or NULL for the context's own
- * stream, where the call waits outside a graph scope like every op above.  All
- * pointers are device memory; 16-byte alignment is needed of codes and rows. */
+ * stream, where the call waits outside a graph scope like every op above.  A
+ * device-side wait that gives up leaves results unwritten; on a stream of the
+ * caller's that can only be told later, by KIB_ERR_TIMEOUT from the next call
+ * that waits on the context.  All pointers are device memory of the context's
+ * GPU; 16-byte alignment is needed of codes and rows. */
 typedef struct kib_kvq8_cache {
   int8_t *k, *v;            /* code of (page, head, token, d): page * page_stride + head * head_stride + token * token_stride + d */
   float *k_scale, *v_scale; /* [pages][kv_heads] */
@@ -311,10 +314,11 @@ typedef struct kib_rope {
 /* Rotates and quantises rows k, v [rows][kv_heads][head_dim] (type F32 or F16,
  * row strides in elements, 0: packed) into the cache, and writes the rotated
  * queries q [rows][heads][head_dim] to q_out (both NULL: none; q_out may be q).
- * Rows before position 0 (more rows than positions) are skipped.  A page's scale is max(old, largest finite |x| of its new rows / 127); where
- * it grows, the codes before the new rows are rounded again to it.  A page
- * whose first position is new starts afresh.  Infinities saturate, NaN gives
- * code 0.  rope may be NULL.  No two sequences may append to one page. */
+ * Rows before position 0 (more rows than positions) are skipped.  A page's
+ * scale is max(old, largest finite |x| of its new rows / 127); where it grows,
+ * the codes before the new rows are rounded again to it.  A page whose first
+ * position is new starts afresh.  Infinities saturate (over a scale of 0 they
+ * give code 0), NaN gives code 0.  rope may be NULL.  No two sequences may append to one page. */
 int kib_kvq8_append(kib_ctx* ctx, const kib_kvq8_cache* cache, const kib_kvq8_batch* batch, const kib_rope* rope,
                     int type, uint64_t heads, const void* q, uint64_t q_stride, const void* k, uint64_t k_stride,
                     const void* v, uint64_t v_stride, void* q_out, uint64_t q_out_stride, void* stream);

@@ -90,9 +90,12 @@ KIB_DEV u64 fixed_weight(float e) {
 // histogram's share take turns: a copy is cleared behind the barrier after the
 // one it was gathered behind, a barrier before its next use.
 
-// Bound by instructions where rows fill the GPU (a logit costs about 50 in the
-// passes of top-p, most of them the exponential and the histogram's), by the
-// latency of barriers and scans where few rows are spread wide.  At 248320
+// Bound by latency.  A CTA's 1024 threads of 64 registers are all that an SM
+// holds: of 223 us for 256 rows with settings of every kind its 39 warp
+// instructions for 32 logits issue in 66, loads and barriers stall the rest
+// (long scoreboard 5.0, barrier 2.2 issue slots an instruction), and 256 rows are two
+// waves.  Where few rows are spread wide it is the barriers and scans (32 rows:
+// 12 of 46 us issue; loads 3.6, barriers 3.5).  At 248320
 // logits, all rows alike: 256 rows with top-k 50 111 us and with top-p 0.9
 // besides 124 (the logits move at HBM's rate in 39), top-p 0.9 alone 272,
 // neither 114; 32 rows 26, 33, 46, 21 us; one row 21, 31, 27, 15 us.

@@ -126,7 +126,7 @@ class PagedDecoder:
             norm = lambda w, a, o, rows=n: ctx.call("kib_rms_norm_f32_f32_batched", a, w, rows, cfg.width, cfg.eps, o)  # noqa: E731
             add = lambda a, b: ctx.call("kib_binary_f32_in_place", 0, a, b, a.numel(), cfg.width)  # noqa: E731
 
-            # captured from here on: nothing may allocate
+            # the calls from here to commit_graph only enqueue: no waits, and nothing that waits (an allocation) between them
             ctx.begin_graph()
             qtype, weight, rows, cols = self.embed
             ctx.dequantize_rows(qtype, weight, rows, ids, n, cols, x)
