@@ -29,8 +29,10 @@
 //
 // The tensor core's fp32 sums are cut toward zero: a step (16 keys) loses up
 // to 2^-22 of the sum where V are all alike, some 2e-8 where their signs are
-// random.  For half rows O is summed in TMEM all the same, under half's 2^-11
-// up to runs of 2000 steps.  Of fp32 rows a tile's products are summed from
+// random.  For half rows O is summed in TMEM all the same, over at most 256
+// tiles, where that stays under half's 2^-11, and joined with rounding from
+// there on (two sequences of 2048 rows after 131072 keys of 64 dimensions: error
+// 2.6e-3 -> 1.1e-3 where values are alike, 7.1e-4 -> 5.3e-4 where not).  Of fp32 rows a tile's products are summed from
 // zero, low halves first, and the softmax threads add them to O in their
 // registers with rounding (l takes along what its additions round off): two
 // warpgroups hold half a row of O each, 128 registers a thread at 256
@@ -44,7 +46,7 @@
 // Bound by the tensor pipe where runs are long (1024 half rows of 8 heads of
 // 256 after 32768 keys: 228-252 us by the machine, up to 1190 TFLOP/s; fp32 391 us),
 // by what a unit costs besides its tiles where they are short (prompts
-// of up to 3001 tokens: halves 179 us, fp32 268 us).  Two turns of softmax
+// of up to 3001 tokens: halves 186 us, fp32 268 us).  Two turns of softmax
 // warps on alternate tiles instead of two halves of each took 280 us for the
 // former, asking for the next stage before a tile's products 252.
 //
@@ -70,6 +72,10 @@ constexpr int kManySoft = 256;   // softmax threads
 // cost of 1, 261 / 412 with 2, 208 / 325 with 4, 178 / 273 with 6, 197 / 320
 // with 16 (head_dim 128: 6 is best too).
 constexpr int kManyUnitCost = 6;
+
+// Tiles of a half rows' run at most: longer ones are cut, and joined as if by
+// another CTA, in this one's record.
+constexpr int kManyRun = 256;
 
 struct Kvq8ManyParams {
   Kvq8AttnParams a;
@@ -452,16 +458,24 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
   // every role walks the same runs: granules [g0, g1) of a unit
   struct Run {
     int seq, tile, head, g0, g1;
-    bool whole;
-    int64_t begin, next;
+    bool whole;        // the unit is all this CTA's
+    bool later, last;  // there is a run of the unit before this one here, this is its last
+    bool done;         // the unit ends with this run
+    int slot;          // its record
+    int64_t next;
   };
   auto run_at = [&](int unit, int64_t at) {
     const int4 u = p.units[unit];
-    const int64_t c0 = p.cum[unit] + kManyUnitCost, c1 = c0 + u.w;
-    Run r{u.x, u.y, u.z, 0, 0, false, at, min(c1, stop)};
+    const int64_t start = p.cum[unit], c0 = start + kManyUnitCost, c1 = c0 + u.w, mine = min(c1, stop);
+    Run r{u.x, u.y, u.z};
+    r.next = Sh::kHeld ? mine : min(mine, max(at, c0) + kManyRun);
     r.g0 = static_cast<int>(max(at - c0, static_cast<int64_t>(0)));
     r.g1 = static_cast<int>(max(r.next - c0, static_cast<int64_t>(0)));
-    r.whole = r.g0 == 0 && r.g1 == u.w;
+    r.whole = first <= c0 && c1 <= stop;
+    r.later = at > max(first, start);
+    r.last = r.next == mine;
+    r.done = r.next == c1;
+    r.slot = first >= start ? 0 : 1;
     return r;
   };
 
@@ -494,9 +508,10 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
         }
       };
       int unit = unit0;
-      for (int64_t at = first; at < stop && ok; ++unit) {
+      for (int64_t at = first; at < stop && ok;) {
         const Run r = run_at(unit, at);
         at = r.next;
+        unit += r.done;
         if (r.g0 == r.g1) continue;
         const int off = p.seq_off[r.seq];
         for (int j = r.g0; j < r.g1 && ok; ++j) {
@@ -574,9 +589,10 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
         it += Sh::kPer;
       };
       int unit = unit0;
-      for (int64_t at = first; at < stop && ok; ++unit) {
+      for (int64_t at = first; at < stop && ok;) {
         const Run r = run_at(unit, at);
         at = r.next;
+        unit += r.done;
         if (r.g0 == r.g1) continue;
         ok = warp_ok(tc_wait(&q_full, piece++ & 1, p.err));
         tc_fence_after();
@@ -596,9 +612,10 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
     uint32_t jg = 0;
     bool ok = true;
     int unit = unit0;
-    for (int64_t at = first; at < stop; ++unit) {
+    for (int64_t at = first; at < stop;) {
       const Run r = run_at(unit, at);
       at = r.next;
+      unit += r.done;
       if (r.g0 == r.g1) continue;
       const Kvq8Seq sq = kvq8_seq(p.a.b, r.seq);
       const ManySeq ms = many_seq(p.a, r.seq);
@@ -851,11 +868,36 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
       }
       float* s_l = reinterpret_cast<float*>(s_q);  // q has been read by every product of the run
       s_l[half * kManyRows + row] = l;
+      float* rec = p.a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + r.slot) * Sh::kPartial;
+      // the unit's run before this one left its m, l and O there
+      float2 before = make_float2(-INFINITY, 0.0f);
+      if (!Sh::kHeld && r.later && row < live) before = make_float2(rec[kManyRows * HD + 2 * row], rec[kManyRows * HD + 2 * row + 1]);
       soft_any(false);
       l += s_l[(half ^ 1) * kManyRows + row];
-      const float back = __uint_as_float(static_cast<uint32_t>(max(ve - 6, 1)) << 23);  // 2^(ve - 126) / 2^7
-      const float inv = r.whole ? (l > 0.0f ? back / l : (l == 0.0f ? 0.0f : l)) : back;
-      float* rec = p.a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (r.begin == first ? 0 : 1)) * Sh::kPartial;
+      float back = __uint_as_float(static_cast<uint32_t>(max(ve - 6, 1)) << 23);  // 2^(ve - 126) / 2^7
+      if (!Sh::kHeld && r.later) {
+        const float mn = fmaxf(m, before.x), f = m == -INFINITY ? 0.0f : ex2(m - mn) * back;
+        const float more = before.x == -INFINITY ? 0.0f : ex2(before.x - mn);
+        l = fmaf(l, m == -INFINITY ? 0.0f : ex2(m - mn), before.y * more);
+        m = mn;
+        back = 1.0f;
+#pragma unroll 1
+        for (int c0 = half * (HD / 2); ok && c0 < (half + 1) * (HD / 2); c0 += 32) {
+          uint32_t o[32];
+          tmem_ld(tmem + lanes + c0, o);
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float z[8] = {};
+            if (row < live) load_vec<float, 8>(rec + row * HD + c0 + i, z);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[i + e] = __float_as_uint(fmaf(z[e], more, __uint_as_float(o[i + e]) * f));
+          }
+          tmem_st32(tmem + lanes + c0, o);
+        }
+        if (ok) tmem_st_wait();
+      }
+      const bool out_now = r.whole && r.last;
+      const float inv = out_now ? (l > 0.0f ? back / l : (l == 0.0f ? 0.0f : l)) : back;
       const int rr = row0 + row;
       T* out = static_cast<T*>(p.a.out) + static_cast<int64_t>(sq.first + rr / p.a.group) * p.a.out_stride +
                (static_cast<int64_t>(r.head) * p.a.group + rr % p.a.group) * HD;
@@ -863,7 +905,7 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = x[e] * inv;
-        if (r.whole) store_vec<T, 8>(out + c0, y);
+        if (out_now) store_vec<T, 8>(out + c0, y);
         else store_vec<float, 8>(rec + row * HD + c0, y);
       };
       if constexpr (Sh::kHeld) {
@@ -892,7 +934,7 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
           }
         }
       }
-      if (!r.whole && row < live && half == 0) {
+      if (!out_now && row < live && half == 0) {
         rec[kManyRows * HD + 2 * row] = m;
         rec[kManyRows * HD + 2 * row + 1] = l;
       }

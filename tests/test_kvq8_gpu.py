@@ -765,8 +765,8 @@ def test_rows_of_no_sequence_are_nothing_to_do(ctx):
     assert (out == 7.0).all()
 
 
-def row_errors(ctx, n, new, hd, kind, alike):
-    """Errors against 64 bits, relative to the row's norm, of fp32 rows over
+def row_errors(ctx, n, new, hd, kind, alike, dtype="f32"):
+    """Errors against 64 bits, relative to the row's norm, of rows over
     long sequences whose scores are exact but for their last rounding: a query
     is a power of two in one dimension, so that a key's weight is the choice of
     its code there.  equal: all weights alike; peak: the fourth key holds over
@@ -795,6 +795,7 @@ def row_errors(ctx, n, new, hd, kind, alike):
     batch = kib.KvQ8Batch(table.cuda(), i32(n), i32(start.tolist()), int(start[-1]), max(new), max(n), sum(n))
     q = torch.zeros(int(start[-1]), heads, hd, device="cuda")
     q[..., 5] = 32.0
+    q = q.to(DT[dtype])
     out = torch.empty_like(q)
     torch.cuda.synchronize()
     ctx.kvq8_attention(kib.KvQ8Cache(k, v, ks, vs), batch, q, out, 0.125)
@@ -808,7 +809,7 @@ def row_errors(ctx, n, new, hd, kind, alike):
             want = torch.einsum("gk,gkd->gd", p, val[:, :end]).repeat_interleave(heads // kv, 0)
             if kind == "peak":
                 assert p.max(-1).values.min() > 0.999 or end < 4
-            errors.append(((out[start[i] + t] - want).norm(dim=-1) / want.norm(dim=-1)).max())
+            errors.append(((out[start[i] + t].double() - want).norm(dim=-1) / want.norm(dim=-1)).max())
     return float(torch.stack(errors).max())
 
 
@@ -876,3 +877,14 @@ def test_attention_of_many_rows_with_scales_far_apart_and_absent_pages(ctx, dtyp
     c.batch.tensors[0].copy_(torch.from_numpy(c.table))
     for scale in (None, 2.0, -0.1, 0.0):
         check_attend(ctx, c, scale)
+
+
+@gpu
+@pytest.mark.parametrize("sequences,n,rows,hd", [(1, 131072, 1024, 128), (2, 131072, 2048, 64), (3, 70000 // 64 * 64, 1500, 256)])
+@pytest.mark.parametrize("kind", ["equal", "peak", "tail"])
+@pytest.mark.parametrize("alike", [False, True])
+def test_attention_of_many_half_rows_over_very_long_runs(ctx, sequences, n, rows, hd, kind, alike):
+    """Runs of up to 900 tiles a CTA.  2^-11 each for the weights and the
+    result, and 256 tiles of eight steps that lose 2^-22 of the sum at most
+    (4.9e-4; a tenth of it where the values' signs are random)."""
+    assert row_errors(ctx, [n] * sequences, [rows] * sequences, hd, kind, alike, "f16") <= 2.0 ** -10 + (4.9e-4 if alike else 4.9e-5)
