@@ -31,17 +31,18 @@
 // to 2^-22 of the sum where V are all alike, some 2e-8 where their signs are
 // random.  For half rows O is summed in TMEM all the same, over at most 256
 // tiles, where that stays under half's 2^-11, and joined with rounding from
-// there on (two sequences of 2048 rows after 131072 keys of 64 dimensions: error
-// 2.6e-3 -> 1.1e-3 where values are alike, 7.1e-4 -> 5.3e-4 where not).  Of fp32 rows a tile's products are summed from
-// zero, low halves first, and the softmax threads add them to O in their
-// registers with rounding (l takes along what its additions round off): two
-// warpgroups hold half a row of O each, 128 registers a thread at 256
-// dimensions, which the helpers' warpgroup gives up (setmaxnreg).  Error against 64
-// bits after 6144 keys: 0.35e-6 of a random result, 1.9e-6 at most where one key holds
-// the weight and V are alike.  (Summed in TMEM and moved into sums in memory
-// every 8 tiles: 1.4e-6 with a correction for random data, 13e-6 for the other;
-// prompts of up to 3001 tokens 307 us where this takes 268.  Halves by this
-// form: 258 us instead of 228 for the chunk below.)
+// there on (two sequences of 2048 rows after 131072 keys of 64 dimensions:
+// error 2.6e-3 -> 1.1e-3 where values are alike, 7.1e-4 -> 5.3e-4 where not).
+// Of fp32 rows a tile's products are summed from zero, low halves first, and
+// the softmax threads add them to O in their registers with rounding (l takes
+// along what its additions round off): two warpgroups hold half a row of O
+// each, 128 registers a thread at 256 dimensions, which the helpers' warpgroup
+// gives up (setmaxnreg).  Error against 64 bits after 6144 keys: 0.35e-6 of a
+// random result, 1.9e-6 at most where one key holds the weight and V are alike.
+// (Summed in TMEM and moved into sums in memory every 8 tiles: 1.4e-6 with a
+// correction for random data, 13e-6 for the other; prompts of up to 3001
+// tokens 307 us where this takes 268.  Halves by this form: 258 us instead of
+// 228 for the chunk below.)
 //
 // Bound by the tensor pipe where runs are long (1024 half rows of 8 heads of
 // 256 after 32768 keys: 228-252 us by the machine, up to 1190 TFLOP/s; fp32 391 us),
