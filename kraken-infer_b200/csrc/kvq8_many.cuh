@@ -41,13 +41,13 @@
 // random result, 1.9e-6 at most where one key holds the weight and V are alike.
 // (Summed in TMEM and moved into sums in memory every 8 tiles: 1.4e-6 with a
 // correction for random data, 13e-6 for the other; prompts of up to 3001
-// tokens 307 us where this takes 268.  Halves by this form: 258 us instead of
+// tokens 307 us where this takes 278.  Halves by this form: 258 us instead of
 // 228 for the chunk below.)
 //
 // Bound by the tensor pipe where runs are long (1024 half rows of 8 heads of
 // 256 after 32768 keys: 228-252 us by the machine, up to 1190 TFLOP/s; fp32 391 us),
 // by what a unit costs besides its tiles where they are short (prompts
-// of up to 3001 tokens: halves 186 us, fp32 268 us).  Two turns of softmax
+// of up to 3001 tokens: halves 181 us, fp32 278 us).  Two turns of softmax
 // warps on alternate tiles instead of two halves of each took 280 us for the
 // former, asking for the next stage before a tile's products 252.
 //
@@ -705,6 +705,9 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
       const int all_see = row_end(0);  // keys below it are seen by every row (of the dead ones nothing is kept)
 
       float m = -INFINITY, l = 0.0f;
+      // m is a rounded product: where a score's last bit may be 2^-4 and above, s * kc is rounded by itself too
+      auto is_large = [](float x) { return fabsf(x) > 0x1p20f && x != -INFINITY; };
+      bool large = false;
       const int n = r.g1 - r.g0;
       float2 sc[4];
 #pragma unroll
@@ -785,6 +788,7 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
           const float mn = fmaxf(m, fmaxf(top, sh.x[buf][half ^ 1][row]));
           const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
           m = mn;
+          if constexpr (!Sh::kHeld) large = __any_sync(0xffffffffu, is_large(m));
           l *= f;
           if constexpr (Sh::kHeld) {
             lc *= f;
@@ -812,10 +816,19 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
         // two scores an instruction: s * kc - m, and p * v_scale
         float2 lp[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         const float2 nm = make_float2(-mm, -mm);
+        auto round_products = [&](int c0, int n) {
+#pragma unroll
+          for (int i = 0; i < n; ++i) s[i] = __float_as_uint(__fmul_rn(__uint_as_float(s[i]), kc[(c0 + i) >> 4]));
+#pragma unroll
+          for (int g = 0; g < n / 16; ++g) kc[c0 / 16 + g] = 1.0f;
+        };
+        if constexpr (Sh::kHeld) large = is_large(m);
+        else if (large) round_products(0, CH);
 #pragma unroll
         for (int c0 = 0; c0 < 64; c0 += 32) {
           if constexpr (Sh::kHeld) load(c0);
           constexpr int B = CH == 64 ? 1 : 0;
+          if (Sh::kHeld && large) round_products(c0, CH);
           uint32_t ph[16], pl[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {

@@ -888,3 +888,26 @@ def test_attention_of_many_half_rows_over_very_long_runs(ctx, sequences, n, rows
     result, and 256 tiles of eight steps that lose 2^-22 of the sum at most
     (4.9e-4; a tenth of it where the values' signs are random)."""
     assert row_errors(ctx, [n] * sequences, [rows] * sequences, hd, kind, alike, "f16") <= 2.0 ** -10 + (4.9e-4 if alike else 4.9e-5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("length,rows", [(700, 2), (1500, 1400)])
+def test_attention_where_scores_are_huge(ctx, dtype, hd, length, rows):
+    """Scores far beyond 2^24: the largest take all the weight (equals share it).
+    They are exact but for their last rounding, being single products."""
+    c = Case([length], [rows], 4, 1, hd, 64, dtype, seed=48)
+    for x in (c.dev[2], c.dev[3]):
+        x.fill_(2.0 ** -5)
+    c.q.zero_()
+    c.q[..., 3] = torch.tensor([1.0, -0.5, 2.0, -4.0])
+    pages = torch.from_numpy(c.table[0][:-(-length // 64)]).long().cuda()
+    key, val = (x[pages, 0].reshape(-1, hd)[:length].double() / 32 for x in c.dev[:2])
+    masked = torch.arange(length, device="cuda") > torch.arange(length - rows, length, device="cuda")[:, None, None]
+    for scale in (1e4, 3e6, 1e7, -2e8, 1e12, 1e30):
+        got = run_attend(ctx, c, scale).double()
+        score = (c.q.cuda().double()[..., 3, None] * key[:, 3] * scale).masked_fill(masked, -math.inf)
+        want = torch.softmax(score, -1) @ val
+        # rounding a result and its weights to half, or fp32 rows' 22 bits of a weight
+        assert (got - want).abs().max() <= (2.0 ** -10 if dtype == "f16" else 2.0 ** -19) * val.abs().max(), scale
