@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(few_warps<HD, NT>() * 32, 1)
           float w[4];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float mm = fmaxf(m[j][e], -1e30f);
+            const float mm = m[j][e] == -INFINITY ? 0.0f : m[j][e];
             const float x = ex2(sc[b][j][e] - mm), y = ex2(sc[b][j][e + 2] - mm);
             lt[j][e] += x + y;
             w[e] = x * vmul;

@@ -812,7 +812,7 @@ __global__ void __launch_bounds__(ManyShape<HD, PL>::kThreads, 1)
             }
           }
         }
-        const float mm = fmaxf(m, -1e30f);
+        const float mm = m == -INFINITY ? 0.0f : m;
         // two scores an instruction: s * kc - m, and p * v_scale
         float2 lp[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         const float2 nm = make_float2(-mm, -mm);

@@ -911,3 +911,22 @@ def test_attention_where_scores_are_huge(ctx, dtype, hd, length, rows):
         want = torch.softmax(score, -1) @ val
         # rounding a result and its weights to half, or fp32 rows' 22 bits of a weight
         assert (got - want).abs().max() <= (2.0 ** -10 if dtype == "f16" else 2.0 ** -19) * val.abs().max(), scale
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("length,rows", [(1, 1), (300, 3), (1500, 1500)])
+def test_attention_where_every_score_is_far_below_zero(ctx, dtype, length, rows):
+    c = Case([length], [rows], 4, 1, 64, 64, dtype, seed=49)
+    c.dev[0][..., 3] = -torch.randint(40, 127, c.dev[0].shape[:3], device="cuda").to(torch.int8)
+    for x in (c.dev[2], c.dev[3]):
+        x.fill_(2.0 ** -5)
+    c.q.zero_()
+    c.q[..., 3] = 1.0
+    pages = torch.from_numpy(c.table[0][:-(-length // 64)]).long().cuda()
+    key, val = (x[pages, 0].reshape(-1, 64)[:length].double() / 32 for x in c.dev[:2])
+    masked = torch.arange(length, device="cuda") > torch.arange(length - rows, length, device="cuda")[:, None]
+    for scale in (1.0, 1e10, 1e31, 1e36):
+        got = run_attend(ctx, c, scale).double()
+        want = torch.softmax((key[:, 3] * scale).expand(rows, -1).masked_fill(masked, -math.inf), -1) @ val
+        assert (got - want[:, None]).abs().max() <= (2.0 ** -10 if dtype == "f16" else 2.0 ** -19) * val.abs().max(), scale
